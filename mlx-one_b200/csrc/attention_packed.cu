@@ -1,0 +1,648 @@
+// Attention of single tokens over a cache held in 4 bits (packed_cache.cuh has the format).
+//
+//   s_j = scale q . k_j = scale sum_g (step_jg (q_g . code_jg) + lowest_jg sum(q_g))
+//   o   = sum_j p_j v_j,  v_jg = step_jg code_jg + lowest_jg,  p = softmax of s over the keys seen (and a sink)
+//
+// Codes are whole numbers of 0..15, exact in bfloat16, so they go into the matrix instructions as they are:
+// the steps and lowest values stay outside, in 32 bits, four multiplications and additions a key and pair of
+// heads. Scores are computed transposed (keys are the 16 rows of a product, up to eight query heads that share
+// the key head its 8 columns), so that GQA's few heads waste no rows, and a unit's codes are operand
+// registers after one shift, one AND and one OR a pair: 0x4300 | code is 128 + code in bfloat16. The
+// scores' accumulators start at -128 sum(q); the values' product has sum(128 p) taken off at the end, the sum
+// of the rounded p coming from one more product with a matrix of ones.
+//
+// float32 queries: every value cut into three bfloat16 parts, which hold its 24 bits, and so are the weights
+// of the values; the codes are centred (code - 8, exact) and the outputs added up in 32-bit registers, tile by
+// tile, so that no sum is longer or larger than it must be.
+//
+// What bounds it: the bytes of the codes, 72 a key and key head of 64 (keys and values), against about 240
+// instructions of a warp for 32 keys. One block = one (request, key head, up to 8 of its query heads,
+// split of the keys); its 8 warps take tiles of 32 keys in turn, each through a ring of its own that bulk
+// copies fill (one copy brings the keys and values of 16 tokens). The warps are merged in shared
+// memory, the splits of up to 8 blocks through a cluster's shared memory, more by a second kernel.
+//
+// The running maximum moves only when a score passes it by more than 2^8 (in powers of two): most tiles
+// then need no exchange between lanes and no pass over the output.
+#include <cooperative_groups.h>
+
+#include "packed_cache.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace {
+
+using bf16 = __nv_bfloat16;
+constexpr int KEYS = 32;               // keys of a tile: two units
+constexpr int WARPS = 8;
+constexpr int HEADS = 8;               // query heads of a block
+constexpr int WAIT_LIMIT = 1 << 22;
+constexpr int ERROR_WAIT = 9;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float NOTHING = -1e30f;      // a maximum of no scores: finite, so that differences stay numbers
+constexpr float LAZY = 8.f;
+
+template <int HD>
+struct Ring {
+    static constexpr int STAGES = HD <= 64 ? 4 : 3;
+    static constexpr int STAGE = 2 * Packed<HD>::UNIT;
+    static constexpr int BYTES = WARPS * STAGES * STAGE;
+    // what the merge needs: a maximum, a sum and an output per head, for every warp and then for the block
+    static constexpr int MERGE = (WARPS + 1) * HEADS * (HD + 2) * 4;
+    static constexpr int SHARED = (BYTES > MERGE ? BYTES : MERGE) + 128;
+};
+
+__device__ __forceinline__ uint32_t shared_address(const void* p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void barrier_init(uint32_t bar) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar));
+}
+__device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool barrier_test(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.b32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+        ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+        : "memory");
+}
+// d += a (16x16, row) * b (16x8, col), bfloat16 in, float accumulate
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float low_of(uint32_t pair) { return __uint_as_float(pair << 16); }
+__device__ __forceinline__ float high_of(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
+
+// The operand pairs of a word's eight codes, in the order of its shifts: 128 + code, or with CENTRED
+// code - 8.
+template <bool CENTRED>
+__device__ __forceinline__ void expand(uint32_t word, uint32_t (&pair)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        pair[i] = ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+        if (CENTRED) {
+            const uint32_t middle = 0x43084308u;                     // 136
+            const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&pair[i]),
+                                             *reinterpret_cast<const __nv_bfloat162*>(&middle));
+            pair[i] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+    }
+}
+
+// Cuts a pair of 32-bit values into NP pairs of bfloat16 parts, the largest first: their sum is the value.
+template <int NP>
+__device__ __forceinline__ void parts_of(float a, float b, uint32_t (&part)[NP]) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        part[i] = pack_pair(a, b);
+        a -= low_of(part[i]);
+        b -= high_of(part[i]);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_pair(T* dst, float a, float b);
+template <>
+__device__ __forceinline__ void store_pair<float>(float* dst, float a, float b) {
+    *reinterpret_cast<float2*>(dst) = make_float2(a, b);
+}
+template <>
+__device__ __forceinline__ void store_pair<bf16>(bf16* dst, float a, float b) {
+    *reinterpret_cast<uint32_t*>(dst) = pack_pair(a, b);
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(WARPS * 32, HD <= 64 ? 2 : 1)
+attention_packed_kernel(const T* q, const unsigned char* cache,
+                        const int* block_table, int table_width, int page_shift, int pages,
+                        const int* positions, T* out, float* partial,
+                        int heads, int kv_heads, int splits, float scale_log2, int window,
+                        const float* sinks, int* error_flag) {
+    using P = Packed<HD>;
+    using R = Ring<HD>;
+    constexpr bool WIDE = sizeof(T) == 4;                  // 32-bit queries
+    constexpr int NP = WIDE ? 3 : 1;                       // bfloat16 parts of a value
+    constexpr int RUNS = P::RUNS, GROUPS = P::GROUPS, GROUP_RUNS = P::GROUP / 16;
+    constexpr float MIDDLE = WIDE ? 8.f : 128.f;
+    extern __shared__ unsigned char shared_raw[];
+    __shared__ __align__(8) unsigned long long barriers[WARPS * R::STAGES];
+    unsigned char* shared = reinterpret_cast<unsigned char*>((reinterpret_cast<size_t>(shared_raw) + 127) &
+                                                             ~(size_t)127);
+    const int group = heads / kv_heads;
+    const int blocks_of_heads = (group + HEADS - 1) / HEADS;
+    const int kv_head = blockIdx.y / blocks_of_heads;
+    const int head0 = kv_head * group + (blockIdx.y % blocks_of_heads) * HEADS;
+    const int rows = min(HEADS, kv_head * group + group - head0);
+    const int request = blockIdx.z, split = blockIdx.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int r = lane >> 2, c = lane & 3;
+
+    griddep_launch();
+    if (threadIdx.x < WARPS * R::STAGES) barrier_init(shared_address(&barriers[threadIdx.x]));
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncthreads();
+    // Queries, and pages: the kernel before this one may have written this step's tokens there.
+    griddep_wait();
+    const T* queries = settled(q);
+    const unsigned char* codes = settled(cache);
+
+    const int position = positions[request];
+    const int lowest_key = first_visible_key(position, window);
+    const int tile_first = lowest_key / KEYS;
+    const int tiles = position < 0 ? 0 : position / KEYS - tile_first + 1;
+    const int share = (tiles + splits - 1) / splits;
+    const int from = tile_first + min(split * share, tiles), to = tile_first + min(split * share + share, tiles);
+
+    const int* table = block_table + (size_t)request * table_width;
+    const int units_per_page = 1 << (page_shift - 4);
+    unsigned char* ring = shared + warp * R::STAGES * R::STAGE;
+    auto barrier = [&](int stage) { return shared_address(&barriers[warp * R::STAGES + stage]); };
+    // lanes 0 and 1 look after the two units of a tile: where it lies, or -1 if no key of it is seen
+    auto look_up = [&](int tile) -> long long {
+        const int key = tile * KEYS + 16 * lane;
+        if (lane > 1 || tile >= to || key > position || key + 15 < lowest_key) return -1;
+        const int block = key >> page_shift;
+        const int page = block < table_width ? table[block] : -1;
+        if (page < 0 || page >= pages) return -1;
+        return ((long long)page * kv_heads + kv_head) * units_per_page + ((key & ((1 << page_shift) - 1)) >> 4);
+    };
+    uint32_t live_units = 0;               // two bits a stage: which units it holds
+    auto fetch = [&](int stage, long long unit) {
+        const unsigned live = __ballot_sync(0xffffffffu, unit >= 0);
+        live_units = (live_units & ~(3u << (2 * stage))) | live << (2 * stage);
+        if (lane == 0) barrier_expect(barrier(stage), (uint32_t)__popc(live) * P::UNIT);
+        __syncwarp();
+        if (unit >= 0)
+            bulk_load(shared_address(ring + stage * R::STAGE + lane * P::UNIT), codes + (size_t)unit * P::UNIT,
+                      P::UNIT, barrier(stage));
+    };
+    int tile = from + warp;
+#pragma unroll
+    for (int ahead = 0; ahead < R::STAGES - 1; ++ahead)
+        if (tile + ahead * WARPS < to) fetch(ahead, look_up(tile + ahead * WARPS));
+    long long coming = look_up(tile + (R::STAGES - 1) * WARPS);
+
+    // q^T as the 8-column operand (head r, dims 16 s + 2c, + 1 and + 8), in NP parts
+    uint32_t qb[RUNS][2][NP];
+    {
+        const bool live = r < rows;
+        const T* row = queries + ((size_t)request * heads + head0 + (live ? r : 0)) * HD;
+#pragma unroll
+        for (int s = 0; s < RUNS; ++s)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const T* at = row + 16 * s + 8 * half + 2 * c;
+                if constexpr (WIDE) {
+                    const float2 v = *reinterpret_cast<const float2*>(at);
+                    parts_of<NP>(live ? v.x : 0.f, live ? v.y : 0.f, qb[s][half]);
+                } else {
+                    qb[s][half][0] = live ? *reinterpret_cast<const uint32_t*>(at) : 0u;
+                }
+            }
+    }
+    // sum(q) of every group for heads 2c and 2c + 1, by a product with ones
+    constexpr uint32_t ONES = 0x3f803f80u;
+    float sums[GROUPS][2];
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+        float small[4] = {0.f, 0.f, 0.f, 0.f}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = g * GROUP_RUNS; s < (g + 1) * GROUP_RUNS; ++s)
+#pragma unroll
+            for (int n = NP - 1; n >= 0; --n)
+                mma_16816(n ? small : sum, ONES, ONES, ONES, ONES, qb[s][0][n], qb[s][1][n]);
+        sums[g][0] = sum[0] + small[0];
+        sums[g][1] = sum[1] + small[1];
+    }
+
+    float m[2] = {NOTHING, NOTHING}, l[2] = {0.f, 0.f};      // heads 2c, 2c + 1; l: this lane's share
+    if (sinks != nullptr && split == 0 && warp == 0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (2 * c + i < rows) {
+                // a sink: a term of the denominator with neither key nor value
+                const float sink = sinks[head0 + 2 * c + i] * LOG2E;
+                m[i] = fmaxf(sink, NOTHING);
+                if (r == 0) l[i] = fast_exp2(sink - m[i]);
+            }
+    }
+    float o[RUNS][4], lows[GROUPS][2], weights[GROUPS][4];   // outputs, sums of p lowest, sums of p step
+#pragma unroll
+    for (int s = 0; s < RUNS; ++s)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[s][k] = 0.f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+        lows[g][0] = lows[g][1] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) weights[g][k] = 0.f;
+    }
+
+    bool ok = true;
+    int stage = 0;
+    uint32_t parity = 0;
+    for (; tile < to; tile += WARPS) {
+        {
+            const int next = tile + (R::STAGES - 1) * WARPS;
+            __syncwarp();                  // every lane is done with the stage that is filled now
+            if (next < to) fetch(stage == 0 ? R::STAGES - 1 : stage - 1, coming);
+            coming = look_up(next + WARPS);
+        }
+        for (int i = 0; !barrier_test(barrier(stage), parity); ++i)
+            if (i >= WAIT_LIMIT) { ok = false; break; }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const unsigned char* held = ring + stage * R::STAGE;
+        const uint32_t live = live_units >> (2 * stage) & 3u;
+        const int first = tile * KEYS;
+
+        float s[2][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const unsigned char* part = held + u * P::UNIT;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[u][k] = 0.f;
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                float acc[4], small[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[k] = WIDE ? 0.f : -MIDDLE * sums[g][k & 1];
+                uint32_t words[GROUP_RUNS];
+                const unsigned char* at = part + P::word_at(lane, g * GROUP_RUNS);
+                if constexpr (GROUP_RUNS == 4) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(at);
+                    words[0] = w.x; words[1] = w.y; words[2] = w.z; words[3] = w.w;
+                } else {
+                    const uint2 w = *reinterpret_cast<const uint2*>(at);
+                    words[0] = w.x; words[1] = w.y;
+                }
+#pragma unroll
+                for (int k = 0; k < GROUP_RUNS; ++k) {
+                    uint32_t a[4];
+                    expand<WIDE>(words[k], a);
+#pragma unroll
+                    for (int n = NP - 1; n >= 0; --n)
+                        mma_16816(n ? small : acc, a[0], a[2], a[1], a[3], qb[g * GROUP_RUNS + k][0][n],
+                                  qb[g * GROUP_RUNS + k][1][n]);
+                }
+                const uint2 scale = *reinterpret_cast<const uint2*>(part + P::scale_at(r, g));
+                const float step[2] = {packed_step(scale.x) * scale_log2, packed_step(scale.y) * scale_log2};
+                float low[2] = {packed_lowest(scale.x) * scale_log2, packed_lowest(scale.y) * scale_log2};
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (WIDE) low[i] = fmaf(MIDDLE, step[i], low[i]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    s[u][k] = fmaf(low[k >> 1], sums[g][k & 1], s[u][k]);
+                    s[u][k] = fmaf(step[k >> 1], NP > 1 ? acc[k] + small[k] : acc[k], s[u][k]);
+                }
+            }
+        }
+        // (a tile whose keys are all seen needs no mask)
+        const bool open = live == 3u && first >= lowest_key && first + KEYS - 1 <= position;
+        uint32_t seen = 0xffu;
+        if (!open) {
+            seen = 0;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int key = first + 16 * u + 8 * half + r;
+                    if ((live >> u & 1u) && key >= lowest_key && key <= position) seen |= 3u << (4 * u + 2 * half);
+                }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (!(seen >> (4 * u + k) & 1u)) s[u][k] = -INFINITY;
+        }
+        float top[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) top[i] = fmaxf(fmaxf(s[0][i], s[0][i + 2]), fmaxf(s[1][i], s[1][i + 2]));
+        if (__any_sync(0xffffffffu, top[0] > m[0] + LAZY || top[1] > m[1] + LAZY)) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int offset = 4; offset < 32; offset <<= 1)
+                    top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], offset));
+                const float raised = fmaxf(m[i], top[i]);
+                const float by = fast_exp2(m[i] - raised);
+                m[i] = raised;
+                l[i] *= by;
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g) {
+                    lows[g][i] *= by;
+                    weights[g][i] *= by;
+                }
+#pragma unroll
+                for (int k = 0; k < RUNS; ++k) {
+                    o[k][i] *= by;
+                    o[k][i + 2] *= by;
+                }
+            }
+        }
+        float p[2][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                p[u][k] = fast_exp2(s[u][k] - m[k & 1]);
+                l[k & 1] += p[u][k];
+            }
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            // the group's weights p step, transposed: keys 2c, + 1 (and + 8), head r
+            uint32_t pb[2][2][NP];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint2 scale = *reinterpret_cast<const uint2*>(held + u * P::UNIT + P::PART + P::scale_at(r, g));
+                const float step[2] = {packed_step(scale.x), packed_step(scale.y)};
+                float low[2] = {packed_lowest(scale.x), packed_lowest(scale.y)};
+                float weight[4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (WIDE) low[i] = fmaf(MIDDLE, step[i], low[i]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    weight[k] = p[u][k] * step[k >> 1];
+                    float taken = p[u][k] * low[k >> 1];
+                    if (!open && !(seen >> (4 * u + k) & 1u)) weight[k] = taken = 0.f;   // whatever lies there
+                    lows[g][k & 1] += taken;
+                }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    parts_of<NP>(weight[2 * half], weight[2 * half + 1], pb[u][half]);
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) pb[u][half][n] = transpose_8x8(pb[u][half][n]);
+                }
+                if (!WIDE) mma_16816(weights[g], ONES, ONES, ONES, ONES, pb[u][0][0], pb[u][1][0]);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const unsigned char* at = held + u * P::UNIT + P::PART + P::word_at(lane, g * GROUP_RUNS);
+                uint32_t words[GROUP_RUNS];
+                if constexpr (GROUP_RUNS == 4) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(at);
+                    words[0] = w.x; words[1] = w.y; words[2] = w.z; words[3] = w.w;
+                } else {
+                    const uint2 w = *reinterpret_cast<const uint2*>(at);
+                    words[0] = w.x; words[1] = w.y;
+                }
+#pragma unroll
+                for (int k = 0; k < GROUP_RUNS; ++k) {
+                    uint32_t a[4];
+                    expand<WIDE>(words[k], a);
+                    if constexpr (WIDE) {
+                        float small[4] = {0.f, 0.f, 0.f, 0.f}, large[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int n = NP - 1; n >= 0; --n)
+                            mma_16816(n ? small : large, a[0], a[1], a[2], a[3], pb[u][0][n], pb[u][1][n]);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) o[g * GROUP_RUNS + k][x] += large[x] + small[x];
+                    } else {
+                        mma_16816(o[g * GROUP_RUNS + k], a[0], a[1], a[2], a[3], pb[u][0][0], pb[u][1][0]);
+                    }
+                }
+            }
+        }
+        stage = stage + 1 == R::STAGES ? 0 : stage + 1;
+        if (stage == 0) parity ^= 1;
+    }
+    if (!ok && lane == 0) atomicExch(error_flag, ERROR_WAIT);
+
+    // the lanes' shares of the sums; every lane has its own dimensions of the output
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int offset = 4; offset < 32; offset <<= 1) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], offset);
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) lows[g][i] += __shfl_xor_sync(0xffffffffu, lows[g][i], offset);
+        }
+    }
+    // A warp that gave up leaves no copy of its own behind: a bounded wait for the stages that it had asked for.
+    if (!ok)
+        for (int k = 0; k < R::STAGES; ++k)
+            for (int i = 0; i < WAIT_LIMIT / 16 && !barrier_test(barrier(k), k >= stage ? parity : parity ^ 1); ++i) {}
+    __syncthreads();
+    // [warp][head][HD + 2]: outputs, maximum, sum, where the rings were
+    float* merge = reinterpret_cast<float*>(shared);
+    constexpr int ROW = HD + 2;
+    {
+        float* mine = merge + warp * HEADS * ROW;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float* row = mine + (2 * c + i) * ROW;
+#pragma unroll
+            for (int k = 0; k < RUNS; ++k) {
+                const int g = k / GROUP_RUNS;
+                const float base = lows[g][i] - (WIDE ? 0.f : MIDDLE * weights[g][i]);
+                row[16 * k + r] = o[k][i] + base;
+                row[16 * k + r + 8] = o[k][i + 2] + base;
+            }
+            if (r == 0) {
+                row[HD] = m[i];
+                row[HD + 1] = l[i];
+            }
+        }
+    }
+    __syncthreads();
+    // the block's result behind the warps' rows
+    float* block_row = merge + WARPS * HEADS * ROW;
+    for (int i = threadIdx.x; i < HEADS * HD; i += WARPS * 32) {
+        const int head = i / HD, d = i % HD;
+        float top = NOTHING;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, merge[(w * HEADS + head) * ROW + HD]);
+        float sum = 0.f, value = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float* row = merge + (w * HEADS + head) * ROW;
+            const float by = fast_exp2(row[HD] - top);
+            sum = fmaf(by, row[HD + 1], sum);
+            value = fmaf(by, row[d], value);
+        }
+        block_row[head * ROW + d] = value;
+        if (d == 0) {
+            block_row[head * ROW + HD] = top;
+            block_row[head * ROW + HD + 1] = sum;
+        }
+    }
+    if (partial != nullptr) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < rows * ROW; i += WARPS * 32)
+            partial[(((size_t)request * heads + head0 + i / ROW) * splits + split) * ROW + i % ROW] = block_row[i];
+        return;
+    }
+    // the splits are a cluster: block `split` adds up every splits-th pair of dimensions
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    for (int i = split * WARPS * 32 + threadIdx.x; i < rows * HD / 2; i += splits * WARPS * 32) {
+        const int head = i / (HD / 2), d = i % (HD / 2) * 2;
+        float top = NOTHING;
+        for (int k = 0; k < splits; ++k) top = fmaxf(top, cluster.map_shared_rank(block_row, k)[head * ROW + HD]);
+        float sum = 0.f, a = 0.f, b = 0.f;
+        for (int k = 0; k < splits; ++k) {
+            const float* row = cluster.map_shared_rank(block_row, k) + head * ROW;
+            const float by = fast_exp2(row[HD] - top);
+            sum = fmaf(by, row[HD + 1], sum);
+            a = fmaf(by, row[d], a);
+            b = fmaf(by, row[d + 1], b);
+        }
+        // (no key and no sink: zeros; a sum that is no number stays one)
+        const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+        store_pair(out + ((size_t)request * heads + head0 + head) * HD + d, a * inverse, b * inverse);
+    }
+    cluster.sync();                        // nobody leaves while its rows are read
+}
+
+// The merge of more splits than a cluster holds: partial [rows, splits, HD + 2] -> out [rows, HD], a warp a row.
+template <typename T, int HD>
+__global__ void __launch_bounds__(128)
+merge_kernel(const float* partial, T* out, int rows, int splits) {
+    griddep_launch();
+    griddep_wait();
+    const float* written = settled(partial);
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (row >= rows) return;
+    const float* from = written + (size_t)row * splits * (HD + 2);
+    float top = NOTHING;
+    for (int k = lane; k < splits; k += 32) top = fmaxf(top, from[k * (HD + 2) + HD]);
+    top = warp_max(top);
+    float sum = 0.f, value[HD / 32];
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) value[i] = 0.f;
+    for (int k = 0; k < splits; ++k) {
+        const float* at = from + k * (HD + 2);
+        const float by = fast_exp2(at[HD] - top);
+        sum = fmaf(by, at[HD + 1], sum);
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) value[i] = fmaf(by, at[lane + 32 * i], value[i]);
+    }
+    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) out[(size_t)row * HD + lane + 32 * i] = from_float<T>(value[i] * inverse);
+}
+
+template <typename T, int HD>
+int launch_packed(const void* q, const void* cache, const int* block_table, int table_width, int page_shift,
+                  int pages, const int* positions, void* out, float* partial, int requests, int heads,
+                  int kv_heads, int splits, float scale, int window, const float* sinks, int* error_flag,
+                  cudaStream_t stream) {
+    auto kernel = attention_packed_kernel<T, HD>;
+    static thread_local int prepared = -1;                 // (the device that the attribute was set on)
+    int device = 0;
+    cudaGetDevice(&device);
+    if (prepared != device) {
+        const cudaError_t error =
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<HD>::SHARED);
+        MLXONE_REQUIRE(error == cudaSuccess, "attention_packed: %s", cudaGetErrorString(error));
+        prepared = device;
+    }
+    const int groups = kv_heads * ceil_div_host(heads / kv_heads, HEADS);
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(splits, groups, requests);
+    config.blockDim = dim3(WARPS * 32);
+    config.dynamicSmemBytes = Ring<HD>::SHARED;
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2];
+    int count = 0;
+    if (partial == nullptr) {
+        attributes[count].id = cudaLaunchAttributeClusterDimension;
+        attributes[count].val.clusterDim.x = splits;
+        attributes[count].val.clusterDim.y = 1;
+        attributes[count].val.clusterDim.z = 1;
+        ++count;
+    }
+    if (mlxone_pdl_enabled()) {
+        attributes[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attributes[count].val.programmaticStreamSerializationAllowed = 1;
+        ++count;
+    }
+    config.attrs = attributes;
+    config.numAttrs = count;
+    cudaLaunchKernelEx(&config, kernel, (const T*)q, (const unsigned char*)cache, block_table, table_width,
+                       page_shift, pages, positions, (T*)out, partial, heads, kv_heads, splits,
+                       scale * LOG2E, window, sinks, error_flag);
+    MLXONE_LAUNCH_CHECK("attention_packed");
+    if (partial != nullptr) {
+        const int rows = requests * heads;
+        launch_kernel(merge_kernel<T, HD>, dim3(ceil_div_host(rows, 4)), dim3(128), 0, stream, true,
+                      (const float*)partial, (T*)out, rows, splits);
+        MLXONE_LAUNCH_CHECK("attention_packed merge");
+    }
+    return 0;
+}
+
+}  // namespace
+
+// Splits that a cluster merges; more need `partial`.
+MLXONE_API int mlxone_attention_packed_cluster() { return 8; }
+
+// Blocks of the kernel that an SM holds at once.
+MLXONE_API int mlxone_attention_packed_resident(int head_dim) { return head_dim <= 64 ? 2 : 1; }
+
+// One token a request: q [requests, heads, head_dim], positions [requests] (each token's own position: the last key
+// that it sees; below 0: none). window: as first_visible_key's span. sinks: float32 [heads] or null. partial:
+// null where `splits` is at most mlxone_attention_packed_cluster(), else requests * heads * splits *
+// (head_dim + 2) floats. Keys without a page are not seen.
+MLXONE_API int mlxone_attention_packed(const void* q, const void* cache, const int* block_table, int table_width,
+                                       int page_size, int pages, const int* positions, void* out, float* partial,
+                                       int requests, int heads, int kv_heads, int head_dim, int splits, float scale,
+                                       int window, const float* sinks, int dtype, int* error_flag,
+                                       cudaStream_t stream) {
+    if (requests == 0) return 0;
+    MLXONE_REQUIRE(requests > 0 && requests <= 65535 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0,
+                   "attention_packed: bad sizes");
+    MLXONE_REQUIRE(page_size >= 16 && (page_size & (page_size - 1)) == 0 && pages > 0 && table_width > 0,
+                   "attention_packed: pages hold a power of two of tokens, 16 or more, not %d", page_size);
+    MLXONE_REQUIRE(splits >= 1 && splits <= 65535 && (partial != nullptr || splits <= 8),
+                   "attention_packed: %d splits need scratch", splits);
+    MLXONE_REQUIRE(kv_heads * (long long)ceil_div_host(heads / kv_heads, HEADS) <= 65535,
+                   "attention_packed: too many heads");
+    MLXONE_REQUIRE((((size_t)cache | (size_t)q) & 15) == 0,
+                   "attention_packed: cache and queries start at multiples of 16 bytes");
+    const int page_shift = 31 - __builtin_clz((unsigned)page_size);
+#define CALL(HD)                                                                                               \
+    if (dtype == MLXONE_BF16)                                                                                  \
+        return launch_packed<bf16, HD>(q, cache, block_table, table_width, page_shift, pages, positions, out,  \
+                                       partial, requests, heads, kv_heads, splits, scale, window, sinks,       \
+                                       error_flag, stream);                                                    \
+    else                                                                                                       \
+        return launch_packed<float, HD>(q, cache, block_table, table_width, page_shift, pages, positions, out, \
+                                        partial, requests, heads, kv_heads, splits, scale, window, sinks,      \
+                                        error_flag, stream)
+    MLXONE_PACKED_DIMS(CALL)
+#undef CALL
+    return 0;
+}

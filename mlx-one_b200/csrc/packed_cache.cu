@@ -1,0 +1,400 @@
+// Keys and values of a step's tokens written to pages of 4-bit codes (packed_cache.cuh has the format),
+// read back, and whole requests opened into pages of plain values.
+//
+// Writing. For a group of a token's values: lowest = bfloat16(min), step = bfloat16(max(max - lowest, 0) / 15,
+// difference and quotient in 32 bits), code = (x - lowest) / step to the nearest whole number, ties to
+// even, cut to 0..15. The codes are those of exact arithmetic on the stored lowest and step: the 32-bit quotient
+// decides, and where it lies within a thousandth of a tie the comparison is made in 64 bits. A group with a
+// value that is not finite, or whose range is none, gets NaN as step and lowest: it stays visible.
+#include "packed_cache.cuh"
+
+namespace {
+
+using bf16 = __nv_bfloat16;
+constexpr int ERROR_WRITE = 2;        // a key written to a position that has no page
+constexpr int ERROR_READ = 3;         // a key read from a position that has no page
+constexpr int TOKENS = 16;            // of a block
+
+template <typename T>
+__device__ __forceinline__ void load_eight(const T* src, bool wide, float (&x)[8]) {
+    if (wide) {
+        if constexpr (sizeof(T) == 2) {
+            const uint4 raw = *reinterpret_cast<const uint4*>(src);
+            const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[2 * i] = __uint_as_float(words[i] << 16);
+                x[2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u);
+            }
+        } else {
+            const float4 a = *reinterpret_cast<const float4*>(src);
+            const float4 b = *reinterpret_cast<const float4*>(src + 4);
+            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+            x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_float<T>(src[i]);
+    }
+}
+
+// The code of x: (x - lowest) / step, about `ratio`, to the nearest whole number in exact arithmetic.
+__device__ __forceinline__ uint32_t code_of(float x, float lowest, float step, float ratio) {
+    float code = rintf(ratio);
+    if (fabsf(ratio - code) > 0.499f) {
+        const float below = floorf(ratio);
+        const double rest = ((double)x - (double)lowest) - ((double)below + 0.5) * (double)step;
+        const bool up = rest > 0.0 || (rest == 0.0 && ((int)fminf(fmaxf(below, -2.f), 32.f) & 1));
+        code = below + (up ? 1.f : 0.f);
+    }
+    return (uint32_t)fminf(fmaxf(code, 0.f), 15.f);
+}
+
+// One block: the runs of tokens that begin among 16 tokens of the step and share a unit (a run ends with its
+// unit or its request), for one key head. HD / 8 lanes take a token's row, eight neighbouring values each: the
+// group's extremes by shuffles, and one exchange of codes with the neighbour that holds the run's other
+// eight dimensions, whose codes share its bytes. The 16 tokens of a whole unit (at most one begins in a block)
+// are put together in shared memory and leave in 16-byte pieces; tokens of a unit's part write their bytes
+// one by one, since the others' stay as they are.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256)
+pack_kernel(const T* keys, long long key_stride, const T* values,
+            long long value_stride, int wide, const int* positions,
+            const int* token_request, const int* request_start,
+            const int* block_table, int table_width, int page_size, int pages, int kv_heads,
+            int tokens, unsigned char* cache, int* error_flag) {
+    using P = Packed<HD>;
+    constexpr int LANES = HD == 96 ? 16 : HD / 8;            // lanes of a row (four of 16 idle with 96 values)
+    constexpr int GROUP_LANES = P::GROUP / 8;
+    __shared__ __align__(16) unsigned char image[P::UNIT];
+    __shared__ int span[3];                                  // first and last + 1 token, the whole unit's first
+    griddep_launch();
+    griddep_wait();
+    const int head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp == 0) {
+        const int t = blockIdx.x * TOKENS + lane;
+        bool begins = false;
+        int length = 0;
+        if (lane < TOKENS && t < tokens) {
+            const int r = token_request[t], inside = positions[t] & 15;
+            begins = inside == 0 || t == request_start[r];
+            length = min(16 - inside, request_start[r + 1] - t);
+        }
+        const unsigned starts = __ballot_sync(0xffffffffu, begins);
+        const unsigned full = __ballot_sync(0xffffffffu, begins && length == 16);
+        const int last = 31 - __clz((int)(starts | 1u));
+        const int end = __shfl_sync(0xffffffffu, t + length, last);
+        if (lane == 0) {
+            span[0] = blockIdx.x * TOKENS + (starts ? __ffs(starts) - 1 : 0);
+            span[1] = starts ? min(end, tokens) : span[0];
+            span[2] = full ? blockIdx.x * TOKENS + __ffs(full) - 1 : -1;
+        }
+    }
+    __syncthreads();
+    const int first = span[0], count = span[1] - span[0], whole = span[2];
+    const int units = page_size >> 4;
+    auto unit_of = [&](int t) -> unsigned char* {
+        const int position = positions[t], block = position / page_size;
+        const int page = position >= 0 && block < table_width
+                             ? block_table[(size_t)token_request[t] * table_width + block] : -1;
+        if (page < 0 || page >= pages) return nullptr;
+        return cache + (((size_t)page * kv_heads + head) * units + (position % page_size >> 4)) * P::UNIT;
+    };
+    const int sub = threadIdx.x % LANES;                     // this thread's place in its row
+    const bool live_lane = sub * 8 < HD;
+    const int rows = 2 * count;                              // keys' rows, then values'
+    for (int base = 0; base < rows; base += blockDim.x / LANES) {
+        const int row = base + threadIdx.x / LANES;
+        const bool live = row < rows && live_lane;
+        const int part = row >= count ? 1 : 0;
+        const int t = first + (live ? row - part * count : 0);
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = 0.f;
+        if (live) {
+            const T* src = (part ? values + (size_t)t * value_stride : keys + (size_t)t * key_stride) +
+                           head * HD + sub * 8;
+            load_eight<T>(src, wide, x);
+        }
+        float least = x[0], most = x[0];
+        bool fine = true;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            least = fminf(least, x[i]);
+            most = fmaxf(most, x[i]);
+            fine = fine && isfinite(x[i]);
+        }
+#pragma unroll
+        for (int offset = 1; offset < GROUP_LANES; offset <<= 1) {
+            least = fminf(least, __shfl_xor_sync(0xffffffffu, least, offset));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, offset));
+            fine = __shfl_xor_sync(0xffffffffu, (int)fine, offset) && fine;
+        }
+        const bf16 lowest_stored = __float2bfloat16_rn(least);
+        const float lowest = __bfloat162float(lowest_stored);
+        const bf16 step_stored = __float2bfloat16_rn(fmaxf(most - lowest, 0.f) / 15.f);
+        const float step = __bfloat162float(step_stored);
+        fine = fine && isfinite(lowest) && isfinite(step);
+        uint32_t mine = 0;
+        if (fine && step > 0.f) {
+            // (a step so small that its inverse is none: the quotient itself)
+            const float inverse = 1.f / step;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float above = x[i] - lowest;
+                const float ratio = isfinite(inverse) ? above * inverse : above / step;
+                mine |= code_of(x[i], lowest, step, ratio) << (4 * i);
+            }
+        }
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
+        const uint32_t low = sub & 1 ? other : mine, high = sub & 1 ? mine : other;   // dimensions e, e + 8
+        if (live) {
+            const bool imaged = whole >= 0 && t >= whole && t < whole + 16;
+            unsigned char* unit = imaged ? image : unit_of(t);
+            if (unit == nullptr) {
+                atomicExch(error_flag, ERROR_WRITE);
+            } else {
+                unit += part * P::PART;
+                const int key = positions[t] & 15, run = sub >> 1;
+                const uint32_t words = fine ? (uint32_t)__bfloat16_as_ushort(step_stored) |
+                                                  (uint32_t)__bfloat16_as_ushort(lowest_stored) << 16
+                                            : 0x7fc07fc0u;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = 4 * (sub & 1) + i;
+                    const unsigned char both = (unsigned char)((low >> (4 * e) & 15u) | (high >> (4 * e) & 15u) << 4);
+                    unit[part ? P::value_byte(key, run, e) : P::key_byte(key, run, e)] = both;
+                }
+                if (sub % GROUP_LANES == 0)
+                    *reinterpret_cast<uint32_t*>(unit + P::scale_at(key, sub / GROUP_LANES)) = words;
+            }
+        }
+    }
+    if (whole >= 0) {
+        __syncthreads();
+        unsigned char* unit = unit_of(whole);
+        if (unit == nullptr) {
+            if (threadIdx.x == 0) atomicExch(error_flag, ERROR_WRITE);
+        } else {
+            for (int i = threadIdx.x; i < P::UNIT / 16; i += blockDim.x)
+                reinterpret_cast<uint4*>(unit)[i] = reinterpret_cast<const uint4*>(image)[i];
+        }
+    }
+}
+
+// Sixteen neighbouring values (run s of a key) from a part's codes, as one thread reads them. `first` and
+// `second`: where the byte of e = 0 lies and how far the next ones are: keys' bytes go by pairs of e.
+template <int HD>
+__device__ __forceinline__ void read_run(const unsigned char* part, int which, int key, int s, float (&x)[16]) {
+    using P = Packed<HD>;
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(part + P::scale_at(key, s * 16 / P::GROUP));
+    const float step = packed_step(word), lowest = packed_lowest(word);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t both = part[which ? P::value_byte(key, s, e) : P::key_byte(key, s, e)];
+        x[e] = fmaf(step, (float)(both & 15u), lowest);
+        x[e + 8] = fmaf(step, (float)(both >> 4), lowest);
+    }
+}
+
+__device__ __forceinline__ void store_run(float* dst, const float (&x)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+}
+__device__ __forceinline__ void store_run(bf16* dst, const float (&x)[16]) {
+    uint32_t words[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const __nv_bfloat162 pair = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        words[i] = *reinterpret_cast<const uint32_t*>(&pair);
+    }
+    *reinterpret_cast<uint4*>(dst) = make_uint4(words[0], words[1], words[2], words[3]);
+    *reinterpret_cast<uint4*>(dst + 8) = make_uint4(words[4], words[5], words[6], words[7]);
+}
+
+// The values that the step's tokens find at their places: keys and values [tokens, kv_heads, HD]. A block
+// takes 16 tokens of one head (neighbours share units, which the first reader brings into the cache), a
+// thread a run of 16 values.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256)
+read_kernel(const unsigned char* cache, const int* positions,
+            const int* token_request, const int* block_table, int table_width,
+            int page_size, int pages, int kv_heads, int tokens, T* keys, T* values,
+            int* error_flag) {
+    using P = Packed<HD>;
+    griddep_launch();
+    griddep_wait();
+    const int head = blockIdx.y, units = page_size >> 4;
+    const unsigned char* from = settled(cache);
+    for (int i = threadIdx.x; i < TOKENS * 2 * P::RUNS; i += blockDim.x) {
+        const int s = i % P::RUNS, which = i / P::RUNS & 1, t = blockIdx.x * TOKENS + i / (2 * P::RUNS);
+        if (t >= tokens) continue;
+        const int position = positions[t], block = position / page_size;
+        const int page = position >= 0 && block < table_width
+                             ? block_table[(size_t)token_request[t] * table_width + block] : -1;
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = 0.f;
+        if (page < 0 || page >= pages) {
+            atomicExch(error_flag, ERROR_READ);
+        } else {
+            const unsigned char* unit =
+                from + (((size_t)page * kv_heads + head) * units + (position % page_size >> 4)) * P::UNIT;
+            read_run<HD>(unit + which * P::PART, which, position & 15, s, x);
+        }
+        store_run((which ? values : keys) + ((size_t)t * kv_heads + head) * HD + s * 16, x);
+    }
+}
+
+// Requests opened: every unit that the requests' tables name, up to their last token, as plain values in
+// pages [2, requests * blocks, open_heads, open_size, HD] of their own, request r's block b in page r * blocks
+// + b, of the key heads from first_head on; rows behind the last token, and of units without a page, are zeros,
+// so that no reader meets a number that is none. `table` gets those page numbers. A thread takes a run of two keys.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256)
+open_kernel(const unsigned char* cache, const int* block_table, int table_width,
+            int page_size, int pages, const int* request_start, const int* history,
+            int span, int first_request, int first_head, int kv_heads, int blocks, int open_size, long long half,
+            T* opened, int* table) {
+    using P = Packed<HD>;
+    griddep_launch();
+    griddep_wait();
+    const unsigned char* from = settled(cache);
+    const int r = blockIdx.z, open_head = blockIdx.y, head = first_head + open_head;
+    const int request = first_request + r;
+    const int held = history[request];
+    const int length = held + request_start[request + 1] - request_start[request];
+    const int per_block = open_size / 16;
+    const int unit = blockIdx.x * (256 / (P::RUNS * 16)) + threadIdx.x / (P::RUNS * 16);
+    if (open_head == 0 && threadIdx.x % (P::RUNS * 16) == 0 && unit < blocks * per_block && unit % per_block == 0)
+        table[(size_t)r * blocks + unit / per_block] = r * blocks + unit / per_block;
+    if (unit >= blocks * per_block || unit / per_block * open_size >= length) return;
+    const int inside = threadIdx.x % (P::RUNS * 16);
+    const int s = inside % P::RUNS, which = inside / P::RUNS & 1, pair = inside / (2 * P::RUNS);   // pair < 8
+    const int first = unit * 16;
+    const bool seen = first < length && first + 15 >= first_visible_key(held, span);
+    const int block = first / page_size;
+    int page = seen && block < table_width ? block_table[(size_t)request * table_width + block] : -1;
+    if (page >= pages) page = -1;
+    const unsigned char* part = page < 0 ? nullptr
+        : from + (((size_t)page * kv_heads + head) * (page_size >> 4) + (first % page_size >> 4)) * P::UNIT +
+              which * P::PART;
+    T* to = opened + which * half +
+            (((size_t)r * blocks + unit / per_block) * gridDim.y + open_head) * open_size * HD +
+            (size_t)(unit % per_block) * 16 * HD;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int key = pair * 2 + i;
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = 0.f;
+        if (part != nullptr && first + key < length) read_run<HD>(part, which, key, s, x);
+        store_run(to + key * HD + s * 16, x);
+    }
+}
+
+int check_geometry(const char* name, int head_dim, int page_size, int pages, int kv_heads, int table_width,
+                   const void* cache) {
+    MLXONE_REQUIRE(page_size >= 16 && page_size % 16 == 0, "%s: pages of 4 bits hold a multiple of 16 tokens, not %d",
+                   name, page_size);
+    MLXONE_REQUIRE(pages > 0 && table_width > 0 && kv_heads > 0 && kv_heads <= 65535, "%s: bad page geometry", name);
+    MLXONE_REQUIRE(((size_t)cache & 15) == 0, "%s: the cache starts at a multiple of 16 bytes", name);
+    MLXONE_REQUIRE(head_dim % 32 == 0 && head_dim >= 32 && head_dim <= 128,
+                   "%s: a cache of 4 bits takes heads of 32, 64, 96 or 128 values, not %d", name, head_dim);
+    return 0;
+}
+
+}  // namespace
+
+// Bytes of 16 tokens of one key head, keys and values; 0 for a head size that the format does not have.
+MLXONE_API int mlxone_packed_unit_bytes(int head_dim) {
+    if (head_dim % 32 != 0 || head_dim < 32 || head_dim > 128) return 0;
+    return 2 * (8 * head_dim + 64 * (head_dim % 64 == 0 ? head_dim / 64 : head_dim / 32));
+}
+
+// keys, values: rows of kv_heads * head_dim values, `*_stride` values apart.
+MLXONE_API int mlxone_pack_key_values(const void* keys, long long key_stride, const void* values,
+                                      long long value_stride, const int* positions, const int* token_request,
+                                      const int* request_start, const int* block_table, int table_width,
+                                      int page_size, int pages, int kv_heads, int head_dim, int tokens,
+                                      void* cache, int dtype, int* error_flag, cudaStream_t stream) {
+    if (tokens == 0) return 0;
+    if (check_geometry("pack_key_values", head_dim, page_size, pages, kv_heads, table_width, cache)) return 1;
+    MLXONE_REQUIRE(tokens > 0, "pack_key_values: bad token count");
+    const int size = dtype == MLXONE_BF16 ? 2 : 4;
+    const int wide = ((size_t)keys & 15) == 0 && ((size_t)values & 15) == 0 && key_stride * size % 16 == 0 &&
+                     value_stride * size % 16 == 0;
+    const dim3 grid(ceil_div_host(tokens, TOKENS), kv_heads);
+#define CALL(HD)                                                                                          \
+    if (dtype == MLXONE_BF16)                                                                             \
+        launch_kernel(pack_kernel<bf16, HD>, grid, dim3(256), 0, stream, true, (const bf16*)keys,         \
+                      key_stride, (const bf16*)values, value_stride, wide, positions, token_request,      \
+                      request_start, block_table, table_width, page_size, pages, kv_heads, tokens,        \
+                      (unsigned char*)cache, error_flag);                                                 \
+    else                                                                                                  \
+        launch_kernel(pack_kernel<float, HD>, grid, dim3(256), 0, stream, true, (const float*)keys,       \
+                      key_stride, (const float*)values, value_stride, wide, positions, token_request,     \
+                      request_start, block_table, table_width, page_size, pages, kv_heads, tokens,        \
+                      (unsigned char*)cache, error_flag)
+    MLXONE_PACKED_DIMS(CALL)
+#undef CALL
+    MLXONE_LAUNCH_CHECK("pack_key_values");
+    return 0;
+}
+
+MLXONE_API int mlxone_read_key_values(const void* cache, const int* positions, const int* token_request,
+                                      const int* block_table, int table_width, int page_size, int pages,
+                                      int kv_heads, int head_dim, int tokens, void* keys, void* values,
+                                      int dtype, int* error_flag, cudaStream_t stream) {
+    if (tokens == 0) return 0;
+    if (check_geometry("read_key_values", head_dim, page_size, pages, kv_heads, table_width, cache)) return 1;
+    MLXONE_REQUIRE(tokens > 0, "read_key_values: bad token count");
+    const dim3 grid(ceil_div_host(tokens, TOKENS), kv_heads);
+#define CALL(HD)                                                                                          \
+    if (dtype == MLXONE_BF16)                                                                             \
+        launch_kernel(read_kernel<bf16, HD>, grid, dim3(256), 0, stream, true, (const unsigned char*)cache, \
+                      positions, token_request, block_table, table_width, page_size, pages, kv_heads,     \
+                      tokens, (bf16*)keys, (bf16*)values, error_flag);                                    \
+    else                                                                                                  \
+        launch_kernel(read_kernel<float, HD>, grid, dim3(256), 0, stream, true, (const unsigned char*)cache, \
+                      positions, token_request, block_table, table_width, page_size, pages, kv_heads,     \
+                      tokens, (float*)keys, (float*)values, error_flag)
+    MLXONE_PACKED_DIMS(CALL)
+#undef CALL
+    MLXONE_LAUNCH_CHECK("read_key_values");
+    return 0;
+}
+
+// Requests first_request.. (`requests` of them) and key heads first_head.. (`open_heads` of kv_heads), `blocks`
+// pages of `open_size` tokens (a multiple of 16) for each request: opened [2, requests * blocks, open_heads,
+// open_size, head_dim], table int32 [requests, blocks]. `span`: see first_visible_key; units that no token of the
+// step sees are zeros.
+MLXONE_API int mlxone_open_key_values(const void* cache, const int* block_table, int table_width, int page_size,
+                                      int pages, const int* request_start, const int* history, int span,
+                                      int first_request, int requests, int kv_heads, int first_head,
+                                      int open_heads, int head_dim, int blocks, int open_size, void* opened, int* table, int dtype, cudaStream_t stream) {
+    if (requests == 0) return 0;
+    if (check_geometry("open_key_values", head_dim, page_size, pages, kv_heads, table_width, cache)) return 1;
+    MLXONE_REQUIRE(requests > 0 && requests <= 65535 && first_request >= 0 && blocks > 0 && open_size >= 16 &&
+                       open_size % 16 == 0 && first_head >= 0 && open_heads > 0 &&
+                       first_head + open_heads <= kv_heads, "open_key_values: bad sizes");
+    const long long half = (long long)requests * blocks * open_heads * open_size * head_dim;
+    const int per = 256 / head_dim;               // units of a block (RUNS * 16 = head_dim threads a unit)
+    MLXONE_REQUIRE(((size_t)opened & 15) == 0, "open_key_values: the output starts at a multiple of 16 bytes");
+    const dim3 grid(ceil_div_host((long long)blocks * (open_size / 16), per), open_heads, requests);
+#define CALL(HD)                                                                                          \
+    if (dtype == MLXONE_BF16)                                                                             \
+        launch_kernel(open_kernel<bf16, HD>, grid, dim3(per * HD), 0, stream, true,                       \
+                      (const unsigned char*)cache, block_table, table_width, page_size, pages,            \
+                      request_start, history, span, first_request, first_head, kv_heads, blocks, open_size, half,     \
+                      (bf16*)opened, table);                                                              \
+    else                                                                                                  \
+        launch_kernel(open_kernel<float, HD>, grid, dim3(per * HD), 0, stream, true,                      \
+                      (const unsigned char*)cache, block_table, table_width, page_size, pages,            \
+                      request_start, history, span, first_request, first_head, kv_heads, blocks, open_size, half,     \
+                      (float*)opened, table)
+    MLXONE_PACKED_DIMS(CALL)
+#undef CALL
+    MLXONE_LAUNCH_CHECK("open_key_values");
+    return 0;
+}

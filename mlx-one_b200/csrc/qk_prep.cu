@@ -16,6 +16,14 @@ namespace {
 constexpr int WARPS = 8;
 constexpr int MAX_HEAD_DIM = 512;
 
+// The page of a token's block of positions; -1: none. Without a table the tokens have pages of one row each, in
+// their own order: keys and values for a cache of another format (packed_cache.cu), which takes them from there.
+__device__ __forceinline__ int page_of(const int* block_table, int table_width, const int* token_request, int t,
+                                       int block) {
+    if (block_table == nullptr) return t;
+    return block < table_width ? block_table[(size_t)token_request[t] * table_width + block] : -1;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(WARPS * 32)
 qk_prep_kernel(const T* __restrict__ qkv, const float* __restrict__ q_weight,
@@ -75,9 +83,7 @@ qk_prep_kernel(const T* __restrict__ qkv, const float* __restrict__ q_weight,
         dst = q_out + ((size_t)t * heads + slot) * head_dim;
     } else {
         const int kv_head = is_k ? slot - heads : slot - heads - kv_heads;
-        const int r = token_request[t];
-        const int block = position / page_size;
-        const int page = block < table_width ? block_table[(size_t)r * table_width + block] : -1;
+        const int page = page_of(block_table, table_width, token_request, t, position / page_size);
         if (page < 0) {
             if (lane == 0) atomicExch(error_flag, 2);
             return;
@@ -150,9 +156,7 @@ qk_prep_wide_kernel(const __nv_bfloat16* __restrict__ qkv, const float* __restri
     // where this token's keys and values go
     T* page_base = nullptr;
     if (write_kv) {
-        const int r = token_request[t];
-        const int block = position / page_size;
-        const int page = block < table_width ? block_table[(size_t)r * table_width + block] : -1;
+        const int page = page_of(block_table, table_width, token_request, t, position / page_size);
         if (page < 0) {
             if (threadIdx.x == 0) atomicExch(error_flag, 2);
         } else {
@@ -279,9 +283,7 @@ qk_prep_general_kernel(const T* __restrict__ qkv, const float* __restrict__ q_we
     // where this token's keys and values go
     T* page_base = nullptr;
     if (write_kv) {
-        const int r = token_request[t];
-        const int block = position / page_size;
-        const int page = block < table_width ? block_table[(size_t)r * table_width + block] : -1;
+        const int page = page_of(block_table, table_width, token_request, t, position / page_size);
         if (page < 0) {
             if (threadIdx.x == 0) atomicExch(error_flag, 2);
         } else {
@@ -387,10 +389,10 @@ qk_prep_eights_kernel(const __nv_bfloat16* qkv, const float* __restrict__ q_weig
         }
     }
     if (threadIdx.x < TOKENS && t0 + (int)threadIdx.x < tokens) {
-        const int t = t0 + threadIdx.x, position = positions[t], block = position / page_size;
+        const int t = t0 + threadIdx.x, position = positions[t];
         long long at = -1;
         if (write_kv) {
-            const int page = block < table_width ? block_table[(size_t)token_request[t] * table_width + block] : -1;
+            const int page = page_of(block_table, table_width, token_request, t, position / page_size);
             if (page < 0) atomicExch(error_flag, 2);
             else at = ((long long)page * kv_heads * page_size + position % page_size) * row_dim;
         }
@@ -500,9 +502,7 @@ qk_prep_rows_kernel(const __nv_bfloat16* __restrict__ qkv, const float* __restri
     const int position = positions[t];
     T* page_base = nullptr;
     if (write_kv) {
-        const int block = position / page_size;
-        const int page = block < table_width
-                             ? block_table[(size_t)token_request[t] * table_width + block] : -1;
+        const int page = page_of(block_table, table_width, token_request, t, position / page_size);
         if (page >= 0)
             page_base = kv + ((size_t)page * kv_heads * page_size + position % page_size) * row_dim;
         else if (threadIdx.x == 0)

@@ -13,11 +13,12 @@ products of the values' parts (24 bits of every value, sums in 32 bits).
 from __future__ import annotations
 
 import ctypes
+from dataclasses import replace
 from typing import Any
 
 import torch
 
-from ..parts.base import NormedInput, NormedUpdate
+from ..parts.base import NormedInput, NormedUpdate, PackedView, PagedView
 from .build import KernelBuildError, library_path
 
 _F32, _BF16 = 0, 1
@@ -135,6 +136,11 @@ class CudaOps:
         # 100; four of 64 tokens 54 / 50; 16 of 32 / 48 / 64 tokens 93 / 88, 139 / 121, 145 / 155. 8 heads:
         # 64 portions of 32 tokens 183 / 166; 16 of 64 82 / 87.
         self.delta_chunk_from = 64
+        # packed pages opened for a step's portions: tokens of an opened page, and bytes of scratch (a call
+        # that needs more takes some key heads after the others)
+        self.open_page = 64
+        self.open_bytes = 1 << 29
+        self._packed_cluster = self.lib.mlxone_attention_packed_cluster()
         # the gated recurrence of few single tokens: the gates' product in the recurrence's kernel
         self.fused_recurrence = True
         self._sample_scratch: torch.Tensor | None = None
@@ -176,7 +182,8 @@ class CudaOps:
     ERRORS = {1: "a token id outside the vocabulary",
               2: "a key written to a position that has no page",
               3: "a key read from a position that has no page",
-              9: "a wait inside a tcgen05 kernel that gave up"}
+              9: "a wait inside a kernel that gave up",
+              10: "a hypothesis, slot or page outside its range"}
 
     def describe_error(self, code: int) -> KernelError:
         return KernelError(f"a kernel reported {self.ERRORS.get(code, f'code {code}')}")
@@ -1526,7 +1533,16 @@ class CudaOps:
         values (1 - m) v + m first, ``first`` [tokens, kv_heads * value_dim])."""
         tokens = qkv.shape[0]
         inv_freq, rotary_dim = (None, 0) if rotary is None else rotary
+        if isinstance(view, PackedView):
+            # (keys and values ready, a row a token, then packed into the pages)
+            return self._prepare_packed(qkv, heads=heads, kv_heads=kv_heads, head_dim=head_dim,
+                                        q_weight=q_weight, k_weight=k_weight, eps=eps, rotary=rotary,
+                                        ctx=ctx, view=view, write=write, value_dim=value_dim,
+                                        amplitude=amplitude, norm_after=norm_after,
+                                        norm_rows=norm_rows, temperature=temperature,
+                                        value_mix=value_mix)
         row_dim = view.kv.shape[-1]
+        width = 1 if view.block_table is None else view.block_table.shape[1]
         value_dim = value_dim or head_dim
         general = (value_dim != head_dim or row_dim != head_dim or amplitude != 1.0 or norm_after
                    or norm_rows or temperature is not None or value_mix is not None)
@@ -1563,7 +1579,7 @@ class CudaOps:
                        _c_int(mode), *mixed, _c_void_p(_ptr(ctx.positions)),
                        _c_void_p(_ptr(ctx.token_request)), _c_void_p(_ptr(q)),
                        _c_void_p(_ptr(view.kv)), _c_void_p(_ptr(view.block_table)),
-                       _c_int(view.block_table.shape[1]), _c_int(view.page_size),
+                       _c_int(width), _c_int(view.page_size),
                        _c_int(view.kv.shape[1]), _c_int(tokens), _c_int(heads), _c_int(kv_heads),
                        _c_int(head_dim), _c_int(value_dim), _c_int(row_dim),
                        _c_int(1 if write else 0), _c_int(qkv.stride(0)),
@@ -1579,7 +1595,7 @@ class CudaOps:
                    _c_void_p(_ptr(inv_freq)), _c_int(rotary_dim), _c_void_p(_ptr(ctx.positions)),
                    _c_void_p(_ptr(ctx.token_request)), _c_void_p(_ptr(q)),
                    _c_void_p(_ptr(view.kv)), _c_void_p(_ptr(view.block_table)),
-                   _c_int(view.block_table.shape[1]), _c_int(view.page_size), _c_int(pages),
+                   _c_int(width), _c_int(view.page_size), _c_int(pages),
                    _c_int(tokens), _c_int(heads), _c_int(kv_heads), _c_int(head_dim),
                    _c_int(1 if write else 0), _c_int(_dtype_code(qkv.dtype)),
                    _c_void_p(_ptr(self.error_flag)))
@@ -1616,10 +1632,11 @@ class CudaOps:
                                         q_weight=q_weight, k_weight=k_weight, eps=eps,
                                         rotary=rotary, ctx=ctx, view=view, write=write, **extra)
             return self.paged_attention(q, heads=heads, kv_heads=kv_heads,
-                                        head_dim=view.kv.shape[-1], scale=scale, window=window,
+                                        head_dim=q.shape[-1], scale=scale, window=window,
                                         ctx=ctx, view=view, sinks=sinks, keep_first=keep_first,
                                         **shaped)
         if (not shaped and self.fused_decode_attention and qkv.dtype == torch.bfloat16
+                and not isinstance(view, PackedView)
                 and ctx.max_portion == 1 and tokens == ctx.requests
                 and self.tensor_core_attention and not keep_first
                 and self.lib.mlxone_attention_decode_fused_supports(_c_int(head_dim))
@@ -1654,7 +1671,7 @@ class CudaOps:
 
     def paged_attention(self, q, *, heads, kv_heads, head_dim, scale, window, ctx, view,
                         sinks=None, chunk=None, keep_first=0, score_cap=0.0, slopes=None,
-                        least_slope=0.0):
+                        least_slope=0.0, out=None):
         """Attention of every token over its request's pages. ``keep_first``: behind a window the
         first ``keep_first`` positions of a sequence stay visible. bfloat16 with a head size that
         is a multiple of 16 up to 128 runs on tensor cores: the split-key decode kernel when
@@ -1662,14 +1679,22 @@ class CudaOps:
         128 values and every earlier key visible runs the 32-bit kernel (``_attention_f32``),
         everything else the general one. ``score_cap`` c (0: none): scores s become c
         tanh(s / c); ``slopes`` (float32 [heads] or None): then they lose slope * (query's position
-        - key's); ``least_slope`` is their minimum on the host."""
+        - key's); ``least_slope`` is their minimum on the host. ``view`` may be a ``PackedView``: keys
+        and values held in 4 bits (``_packed_attention``). ``out``: where the result goes, if not into a
+        tensor of its own."""
+        if isinstance(view, PackedView):
+            return self._packed_attention(q, heads, kv_heads, head_dim, scale, window, ctx, view,
+                                          sinks=sinks, chunk=chunk, keep_first=keep_first,
+                                          score_cap=score_cap, slopes=slopes,
+                                          least_slope=least_slope, out=out)
         if score_cap or slopes is not None:
             if window or chunk or keep_first or sinks is not None:
                 raise KernelError("shaped scores go without windows, chunks and sinks")
             return self._shaped_attention(q, heads, kv_heads, head_dim, scale, ctx, view,
-                                          float(score_cap), slopes, float(least_slope))
+                                          float(score_cap), slopes, float(least_slope), out)
         tokens = q.shape[0]
-        out = torch.empty((tokens, heads * head_dim), dtype=q.dtype, device=self.device)
+        if out is None:
+            out = torch.empty((tokens, heads * head_dim), dtype=q.dtype, device=self.device)
         width = view.block_table.shape[1]
         pages = view.kv.shape[1]
         code = _dtype_code(q.dtype)
@@ -1808,7 +1833,8 @@ class CudaOps:
                 if partial is not None:
                     self.launches += 1          # the merge kernel
 
-    def _shaped_attention(self, q, heads, kv_heads, head_dim, scale, ctx, view, cap, slopes, least_slope):
+    def _shaped_attention(self, q, heads, kv_heads, head_dim, scale, ctx, view, cap, slopes, least_slope,
+                          out=None):
         """paged_attention with capped or distance-biased scores, on the same kernels built with the
         shaping of scores. With both, a key so far back that its weight underflows beside the
         query's own is not read (the kernels find the bound per head): the host bounds the splits of
@@ -1818,7 +1844,8 @@ class CudaOps:
             self._need(slopes, torch.float32, "slopes")
             if slopes.numel() != heads:
                 raise KernelError("one slope per query head")
-        out = torch.empty((tokens, heads * head_dim), dtype=q.dtype, device=self.device)
+        if out is None:
+            out = torch.empty((tokens, heads * head_dim), dtype=q.dtype, device=self.device)
         width, pages = view.block_table.shape[1], view.kv.shape[1]
         code = _dtype_code(q.dtype)
         shape = (_c_float(scale), _c_float(cap), _c_void_p(_ptr(slopes)))
@@ -1946,6 +1973,273 @@ class CudaOps:
             elif wanted == 4 and head_dim <= 64:
                 wanted = 3
         return max(min(wanted, tiles // 4), 1)
+
+    # ---- keys and values held in 4 bits
+
+    def _need_packed(self, view) -> int:
+        """Checks a view of packed pages; returns how many pages there are."""
+        kv, need, size = view.kv, view.need, view.page_size
+        if size < 16 or size & (size - 1):
+            raise KernelError(f"pages of 4 bits hold a power of two of tokens, 16 or more, not {size}")
+        unit = self.lib.mlxone_packed_unit_bytes(need.head_dim)
+        if not unit or need.planes != 2:
+            raise KernelError(f"a cache of 4 bits takes keys and values of 32, 64, 96 or 128 values a "
+                              f"head, not {need.head_dim} in {need.planes} planes")
+        if (kv.dtype != torch.uint8 or not kv.is_contiguous() or kv.device != self.device
+                or kv.dim() != 5 or kv.shape[1:] != (need.kv_heads, size // 16, 2, unit // 2)):
+            raise KernelError(f"packed pages must be contiguous uint8 [pages, {need.kv_heads}, {size // 16}, "
+                              f"2, {unit // 2}] on {self.device}, got {kv.dtype} {tuple(kv.shape)} on "
+                              f"{kv.device}")
+        self._need(view.block_table, torch.int32, "block table")
+        return kv.shape[0]
+
+    def pack_key_values(self, keys, values, *, ctx, view):
+        """Writes the step's keys and values (rows [tokens, kv_heads * head_dim], which may be slices of
+        wider rows, ready as attention reads them) to their tokens' places in the packed pages of
+        ``view``. Every group of a token's values (64; 32 where 64 do not divide the head) is held as its
+        lowest value and a step in bfloat16 and a code of 0 to 15 a value, the nearest; a group with a
+        value that is not finite reads as NaN. Other tokens' bytes stay as they are."""
+        pages = self._need_packed(view)
+        kv_heads, head_dim = view.need.kv_heads, view.need.head_dim
+        tokens = keys.shape[0]
+        for rows, what in ((keys, "keys"), (values, "values")):
+            self._need_rows(rows, keys.dtype, what)
+            if rows.shape != (tokens, kv_heads * head_dim):
+                raise KernelError(f"{what} must be [{tokens}, {kv_heads} * {head_dim}], got {tuple(rows.shape)}")
+        if tokens != ctx.tokens:
+            raise KernelError(f"the step has {ctx.tokens} tokens, {tokens} rows were given")
+        self._call("mlxone_pack_key_values", _c_void_p(_ptr(keys)), _c_ll(keys.stride(0)),
+                   _c_void_p(_ptr(values)), _c_ll(values.stride(0)), _c_void_p(_ptr(ctx.positions)),
+                   _c_void_p(_ptr(ctx.token_request)), _c_void_p(_ptr(ctx.request_start)),
+                   _c_void_p(_ptr(view.block_table)), _c_int(view.block_table.shape[1]),
+                   _c_int(view.page_size), _c_int(pages), _c_int(kv_heads), _c_int(head_dim),
+                   _c_int(tokens), _c_void_p(_ptr(view.kv)), _c_int(_dtype_code(keys.dtype)),
+                   _c_void_p(_ptr(self.error_flag)))
+
+    def read_key_values(self, *, ctx, view, dtype=torch.bfloat16):
+        """What attention finds at the step's tokens' places in packed pages: (keys, values), each
+        [tokens, kv_heads, head_dim] in ``dtype``."""
+        pages = self._need_packed(view)
+        kv_heads, head_dim = view.need.kv_heads, view.need.head_dim
+        keys = torch.empty((ctx.tokens, kv_heads, head_dim), dtype=dtype, device=self.device)
+        values = torch.empty_like(keys)
+        self._call("mlxone_read_key_values", _c_void_p(_ptr(view.kv)), _c_void_p(_ptr(ctx.positions)),
+                   _c_void_p(_ptr(ctx.token_request)), _c_void_p(_ptr(view.block_table)),
+                   _c_int(view.block_table.shape[1]), _c_int(view.page_size), _c_int(pages),
+                   _c_int(kv_heads), _c_int(head_dim), _c_int(ctx.tokens), _c_void_p(_ptr(keys)),
+                   _c_void_p(_ptr(values)), _c_int(_dtype_code(dtype)),
+                   _c_void_p(_ptr(self.error_flag)))
+        return keys, values
+
+    def _prepare_packed(self, qkv, *, kv_heads, ctx, view, write, **how):
+        """qk_norm_rope_store for packed pages: the same kernels write keys and values in the compute
+        dtype, one row a token, and a second one packs them."""
+        self._need_packed(view)
+        tokens, row = qkv.shape[0], view.need.head_dim
+        ready = torch.empty((2, max(tokens, 1), kv_heads, 1, row), dtype=qkv.dtype, device=self.device)
+        # (without a table a token's row is its own page)
+        rows = PagedView(ready, None, 1, view.need)
+        q = self.qk_norm_rope_store(qkv, kv_heads=kv_heads, ctx=ctx, view=rows, write=write, **how)
+        if write and tokens:
+            self.pack_key_values(ready[0].view(tokens, -1), ready[1].view(tokens, -1), ctx=ctx, view=view)
+        return q
+
+    def _packed_attention(self, q, heads, kv_heads, head_dim, scale, window, ctx, view, *, sinks=None,
+                          chunk=None, keep_first=0, score_cap=0.0, slopes=None, least_slope=0.0, out=None):
+        """paged_attention over packed pages. The requests at the head of the step that bring one token
+        each (all of a step of single tokens) go to the kernel that reads the codes themselves; the
+        others are opened into pages of the compute dtype, a scratch of this call, which the prefill
+        kernels read: a portion has many queries for every key that is opened. So do single tokens whose
+        scores are shaped or that see first positions behind a window."""
+        pages = self._need_packed(view)
+        self._need(q, q.dtype, "q")
+        tokens, requests, width = q.shape[0], ctx.requests, view.block_table.shape[1]
+        if q.numel() != tokens * heads * head_dim or heads % kv_heads or \
+                (kv_heads, head_dim) != (view.need.kv_heads, view.need.head_dim):
+            raise KernelError(f"queries {tuple(q.shape)} of {heads} heads of {head_dim} do not fit packed pages "
+                              f"of {view.need.kv_heads} heads of {view.need.head_dim}")
+        if view.block_table.shape[0] < requests:
+            raise KernelError("a block table needs a row for every request")
+        if chunk:
+            window = self._span(window, chunk)
+        window = int(window or 0)
+        if sinks is not None:
+            self._need(sinks, torch.float32, "sinks")
+            if sinks.numel() != heads:
+                raise KernelError("one sink per query head")
+        if out is None:
+            out = torch.empty((tokens, heads * head_dim), dtype=q.dtype, device=self.device)
+        shaped = bool(score_cap) or slopes is not None or (bool(keep_first) and window > 0)
+        singles = requests if ctx.max_portion == 1 and tokens == requests else min(ctx.leading_single, requests)
+        if shaped:
+            singles = 0
+        bound = min(ctx.max_context, width * view.page_size)
+        if singles:
+            splits = self.packed_splits(singles, heads, kv_heads, head_dim, bound, window)
+            partial = None
+            if splits > self._packed_cluster:
+                partial = torch.empty(singles * heads * splits * (head_dim + 2), dtype=torch.float32,
+                                      device=self.device)
+                self.launches += 1          # the merge kernel
+            self._call("mlxone_attention_packed", _c_void_p(_ptr(q)), _c_void_p(_ptr(view.kv)),
+                       _c_void_p(_ptr(view.block_table)), _c_int(width), _c_int(view.page_size),
+                       _c_int(pages), _c_void_p(_ptr(ctx.positions)), _c_void_p(_ptr(out)),
+                       _c_void_p(_ptr(partial)), _c_int(singles), _c_int(heads), _c_int(kv_heads),
+                       _c_int(head_dim), _c_int(splits), _c_float(scale), _c_int(window),
+                       _c_void_p(_ptr(sinks)), _c_int(_dtype_code(q.dtype)),
+                       _c_void_p(_ptr(self.error_flag)))
+        rest = requests - singles
+        if not rest or tokens == singles:
+            return out
+        # (never as a step of single tokens: their kernels read pages ahead of the wait for the kernel before
+        # them, which here is the one that fills the pages)
+        step = replace(ctx, leading_single=0, max_portion=max(ctx.max_portion, 2))
+        if singles:
+            step = replace(step, tokens=tokens - singles, requests=rest, token_ids=ctx.token_ids[singles:],
+                           positions=ctx.positions[singles:],
+                           token_request=ctx.token_request[singles:tokens] - singles,
+                           request_start=ctx.request_start[singles:] - singles,
+                           history=ctx.history[singles:])
+        blocks = max(-(-bound // self.open_page), 1)
+        group = heads // kv_heads
+        each = 2 * rest * blocks * self.open_page * head_dim * q.element_size()      # bytes a key head
+        at_once = max(min(self.open_bytes // each, kv_heads), 1)
+        queries = q.view(tokens, heads, head_dim)[singles:]
+        opened = torch.empty((2, rest * blocks, at_once, self.open_page, head_dim), dtype=q.dtype,
+                             device=self.device)
+        table = torch.empty((rest, blocks), dtype=torch.int32, device=self.device)
+        for first in range(0, kv_heads, at_once):
+            count = min(at_once, kv_heads - first)
+            here = opened if count == at_once else opened.view(-1)[:opened.numel() // at_once * count].view(
+                2, rest * blocks, count, self.open_page, head_dim)
+            # (chunks, and windows with first positions that stay, open everything)
+            self._call("mlxone_open_key_values", _c_void_p(_ptr(view.kv)), _c_void_p(_ptr(view.block_table)),
+                       _c_int(width), _c_int(view.page_size), _c_int(pages),
+                       _c_void_p(_ptr(ctx.request_start)), _c_void_p(_ptr(ctx.history)),
+                       _c_int(0 if keep_first else window), _c_int(singles), _c_int(rest), _c_int(kv_heads),
+                       _c_int(first), _c_int(count), _c_int(head_dim), _c_int(blocks),
+                       _c_int(self.open_page), _c_void_p(_ptr(here)), _c_void_p(_ptr(table)),
+                       _c_int(_dtype_code(q.dtype)))
+            plain = PagedView(here, table, self.open_page, view.need)
+            own = slice(first * group, (first + count) * group)
+            common = dict(heads=count * group, kv_heads=count, head_dim=head_dim, scale=scale, window=window,
+                          ctx=step, view=plain, sinks=None if sinks is None else sinks[own],
+                          keep_first=keep_first, score_cap=score_cap,
+                          slopes=None if slopes is None else slopes[own], least_slope=least_slope)
+            if count == kv_heads:
+                self.paged_attention(queries, out=out[singles:], **common)
+            else:
+                # (more than the scratch holds: some key heads after the others)
+                part = self.paged_attention(queries[:, own].contiguous(), **common)
+                out.view(tokens, heads, head_dim)[singles:, own] = part.view(-1, count * group, head_dim)
+        return out
+
+    def packed_splits(self, requests: int, heads: int, kv_heads: int, head_dim: int, context_bound: int,
+                      window: int) -> int:
+        """Into how many parts the kernel over packed pages cuts a request's keys: as many blocks as the
+        GPU holds at once, each warp of a block with a tile of 32 keys at least."""
+        if window:
+            context_bound = min(context_bound, abs(window) + 31)
+        blocks = requests * kv_heads * -(-(heads // kv_heads) // 8)
+        resident = self._sm_count * self.lib.mlxone_attention_packed_resident(head_dim)
+        tiles = max(-(-context_bound // 32), 1)
+        return max(min(resident // blocks, -(-tiles // 8)), 1)
+
+    # ---- several hypotheses of a request
+
+    def beam_select(self, logits, scores, *, ended=None, end_tokens=None):
+        """The best continuations of every request's hypotheses. ``logits`` float32 [requests * beams, vocab]
+        (rows may be slices of wider ones), ``scores`` float32 [requests, beams]: the hypotheses' sums of
+        logarithms (minus infinity: not one yet); ``ended`` uint8 or bool [requests, beams]: those that
+        have ended and only compete as they are, with the token ``end_tokens[0]`` again; ``end_tokens``
+        int32: tokens that end a hypothesis. Of all score + log_softmax(logits) the ``beams`` largest,
+        largest first, ties to the lower hypothesis, then the lower token. Returns (scores float32,
+        parents int32: the hypothesis continued, tokens int32, ended uint8), each [requests, beams].
+        A logit that is no number counts as minus infinity; a row whose score or sum of exponentials is
+        not finite continues with minus infinity."""
+        self._need_rows(logits, torch.float32, "logits")
+        self._need(scores, torch.float32, "scores")
+        if scores.dim() != 2 or scores.numel() != logits.shape[0]:
+            raise KernelError(f"scores {tuple(scores.shape)} need a row of logits each, got {logits.shape[0]}")
+        requests, beams = scores.shape
+        vocab = logits.shape[1]
+        if not 1 <= beams <= 32 or vocab < beams:
+            raise KernelError(f"1 to 32 hypotheses, no more than tokens, not {beams} of {vocab} tokens")
+        if ended is not None:
+            if ended.dtype == torch.bool:
+                ended = ended.view(torch.uint8)
+            self._need(ended, torch.uint8, "ended")
+            if ended.shape != scores.shape or end_tokens is None or not end_tokens.numel():
+                raise KernelError("ended needs an entry per hypothesis, and a token that ends one")
+        if end_tokens is not None:
+            self._need(end_tokens, torch.int32, "end tokens")
+        chosen = torch.empty((requests, beams), dtype=torch.float32, device=self.device)
+        parents = torch.empty((requests, beams), dtype=torch.int32, device=self.device)
+        tokens = torch.empty((requests, beams), dtype=torch.int32, device=self.device)
+        over = torch.empty((requests, beams), dtype=torch.uint8, device=self.device)
+        rows = requests * beams
+        if rows:
+            parts = self.lib.mlxone_beam_parts(rows, vocab)
+            scratch = torch.empty(rows * parts * (beams + 1), dtype=torch.int64, device=self.device)
+            sums = scratch.data_ptr() + 8 * rows * parts * beams
+            self._call("mlxone_beam_select", _c_void_p(_ptr(logits)), _c_ll(logits.stride(0)),
+                       _c_int(requests), _c_int(beams), _c_int(vocab), _c_void_p(_ptr(scores)),
+                       _c_void_p(_ptr(ended)), _c_void_p(_ptr(end_tokens)),
+                       _c_int(0 if end_tokens is None else end_tokens.numel()), _c_int(parts),
+                       _c_void_p(sums), _c_void_p(_ptr(scratch)), _c_void_p(_ptr(chosen)),
+                       _c_void_p(_ptr(parents)), _c_void_p(_ptr(tokens)), _c_void_p(_ptr(over)))
+            self.launches += 1              # the parts, then the choice
+        return chosen, parents, tokens, over
+
+    def _need_parents(self, parents) -> None:
+        self._need(parents, torch.int32, "parents")
+        if parents.dim() != 2 or not 1 <= parents.shape[1] <= 32:
+            raise KernelError(f"parents are [requests, 1 to 32 hypotheses], got {tuple(parents.shape)}")
+
+    def reorder_slots(self, state, slots, parents) -> None:
+        """In place: of every entry of ``state`` [entries, slots, ...] (any type, contiguous), slot
+        ``slots[r * beams + b]`` gets what slot ``slots[r * beams + parents[r, b]]`` held. ``slots`` int32
+        [requests * beams], no slot twice; ``parents`` int32 [requests, beams]."""
+        self._need_parents(parents)
+        self._need(slots, torch.int32, "slots")
+        requests, beams = parents.shape
+        if not state.is_contiguous() or state.device != self.device or state.dim() < 2:
+            raise KernelError("state must be a contiguous tensor [entries, slots, ...] on the device")
+        if slots.numel() != requests * beams:
+            raise KernelError("one slot per hypothesis")
+        if requests == 0 or state.numel() == 0:
+            return
+        entries, count = state.shape[:2]
+        self._call("mlxone_reorder_slots", _c_void_p(_ptr(state)), _c_ll(entries), _c_ll(count),
+                   _c_ll(state.numel() // (entries * count) * state.element_size()), _c_void_p(_ptr(slots)),
+                   _c_void_p(_ptr(parents)), _c_int(requests), _c_int(beams),
+                   _c_void_p(_ptr(self.error_flag)))
+
+    def reorder_pages(self, storage, block_table, parents, starts, lengths, *, page_size) -> None:
+        """In place: in every entry of ``storage`` [entries, pages, ...] (any type, contiguous; planes are
+        entries of their own), the pages of request r's hypothesis b get what the same blocks' pages
+        of its hypothesis ``parents[r, b]`` held, for the blocks that hold positions ``starts[r]`` to
+        ``lengths[r] - 1``. ``block_table`` int32 [requests * beams, width], a row a hypothesis, -1 where
+        there is no page; a page that moves belongs to one hypothesis. ``starts``, ``lengths`` int32
+        [requests]."""
+        self._need_parents(parents)
+        requests, beams = parents.shape
+        self._need(block_table, torch.int32, "block table")
+        self._need(starts, torch.int32, "starts")
+        self._need(lengths, torch.int32, "lengths")
+        if not storage.is_contiguous() or storage.device != self.device or storage.dim() < 3:
+            raise KernelError("storage must be a contiguous tensor [entries, pages, ...] on the device")
+        if block_table.dim() != 2 or block_table.shape[0] != requests * beams or \
+                starts.numel() != requests or lengths.numel() != requests or page_size < 1:
+            raise KernelError("a row of the block table per hypothesis, a start and a length per request")
+        if requests == 0 or storage.numel() == 0 or block_table.shape[1] == 0:
+            return
+        outer, pages = storage.shape[:2]
+        self._call("mlxone_reorder_pages", _c_void_p(_ptr(storage)), _c_ll(outer), _c_ll(pages),
+                   _c_ll(storage.numel() // (outer * pages) * storage.element_size()),
+                   _c_void_p(_ptr(block_table)), _c_int(block_table.shape[1]), _c_void_p(_ptr(parents)),
+                   _c_void_p(_ptr(starts)), _c_void_p(_ptr(lengths)), _c_int(page_size), _c_int(requests),
+                   _c_int(beams), _c_void_p(_ptr(self.error_flag)))
 
     def argmax(self, logits):
         self._need(logits, torch.float32, "logits")

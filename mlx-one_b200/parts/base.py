@@ -66,6 +66,27 @@ class PagedView:
 
 
 @dataclass
+class PackedView:
+    """One cache entry of a paged group whose keys and values are held in 4 bits, as a step sees it.
+    ``kv`` is uint8 [pages, kv_heads, page_size / 16, 2, part bytes] (csrc/packed_cache.cuh has the
+    format); ``page_size`` is a power of two of 16 or more, ``need.head_dim`` 32, 64, 96 or 128."""
+
+    kv: torch.Tensor
+    block_table: torch.Tensor
+    page_size: int
+    need: PagedKeyValues
+
+
+def packed_part_bytes(head_dim: int) -> int:
+    """Bytes of the keys (or values) of 16 tokens of one head, held in 4 bits: the codes, and a step
+    and a lowest value in bfloat16 for every 64 values of a token (32 where 64 do not divide the
+    head)."""
+    if head_dim not in (32, 64, 96, 128):
+        raise ValueError(f"a cache of 4 bits takes heads of 32, 64, 96 or 128 values, not {head_dim}")
+    return 8 * head_dim + 64 * (head_dim // (64 if head_dim % 64 == 0 else 32))
+
+
+@dataclass
 class StateView:
     """One cache entry of a fixed-state group: ``state`` is [slots, *shape] and
     ``slots`` int32 [requests] names each request's slot."""
