@@ -3,17 +3,23 @@
 //   s_j = scale q . k_j = scale sum_g (step_jg (q_g . code_jg) + lowest_jg sum(q_g))
 //   o   = sum_j p_j v_j,  v_jg = step_jg code_jg + lowest_jg,  p = softmax of s over the keys seen (and a sink)
 //
-// Codes are whole numbers of 0..15, exact in bfloat16, so they go into the matrix instructions as they are:
-// the steps and lowest values stay outside, in 32 bits, four multiplications and additions a key and pair of
-// heads. Scores are computed transposed (keys are the 16 rows of a product, up to eight query heads that share
-// the key head its 8 columns), so that GQA's few heads waste no rows, and a unit's codes are operand
-// registers after one shift, one AND and one OR a pair: 0x4300 | code is 128 + code in bfloat16. The
-// scores' accumulators start at -128 sum(q); the values' product has sum(128 p) taken off at the end, the sum
-// of the rounded p coming from one more product with a matrix of ones.
+// Codes are whole numbers of 0..15, so they go into the matrix instructions as they are: the steps and lowest
+// values stay outside, in 32 bits. Scores are computed transposed (keys are the 16 rows of a product, up to
+// eight query heads that share the key head its 8 columns), so that GQA's few heads waste no rows, and a unit's
+// codes are operand registers after two shifts' worth of masking: four bits at the bottom of a half-precision
+// number are the subnormal number code * 2^-24, four bits above them 16 times that. So one shift and four ANDs
+// make the eight operands of a word; the factor 16 is in the queries of those dimensions, or taken off those
+// dimensions of the output at the end.
+//
+// Roundings (bfloat16 queries): a query becomes half-precision times a power of two that brings the
+// block's largest to 2^13, exact but for what is 2^-26 of the largest and less. A weight p step becomes
+// half-precision times a power of two that keeps the largest step near 2^9 (11 bits of every weight down to
+// 2^-24 of the largest; as bfloat16 with its 8 bits the result was off by 0.003 to 0.008 of itself, now by
+// 0.0003 and its own rounding). Sums, scores, exponentials and the lowest values' share are in 32 bits.
 //
 // float32 queries: every value cut into three bfloat16 parts, which hold its 24 bits, and so are the weights
-// of the values; the codes are centred (code - 8, exact) and the outputs added up in 32-bit registers, tile by
-// tile, so that no sum is longer or larger than it must be.
+// of the values; the codes are centred (code - 8, exact in bfloat16) and the outputs added up in 32-bit
+// registers, tile by tile, so that no sum is longer or larger than it must be.
 //
 // What bounds it: the bytes of the codes, 72 a key and key head of 64 (keys and values), against about 240
 // instructions of a warp for 32 keys. One block = one (request, key head, up to 8 of its query heads,
@@ -21,9 +27,11 @@
 // copies fill (one copy brings the keys and values of 16 tokens). The warps are merged in shared
 // memory, the splits of up to 8 blocks through a cluster's shared memory, more by a second kernel.
 //
-// The running maximum moves only when a score passes it by more than 2^8 (in powers of two): most tiles
-// then need no exchange between lanes and no pass over the output.
+// The running maximum moves only when a score passes it by more than 2^4 (in powers of two), the steps'
+// power of two only when one outgrows it: most tiles need no exchange between lanes and no pass over the
+// output.
 #include <cooperative_groups.h>
+#include <cuda_fp16.h>
 
 #include "packed_cache.cuh"
 
@@ -39,7 +47,7 @@ constexpr int WAIT_LIMIT = 1 << 22;
 constexpr int ERROR_WAIT = 9;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NOTHING = -1e30f;      // a maximum of no scores: finite, so that differences stay numbers
-constexpr float LAZY = 8.f;
+constexpr float LAZY = 4.f;
 
 template <int HD>
 struct Ring {
@@ -86,6 +94,15 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// the same with half-precision operands
+__device__ __forceinline__ void mma_half(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -103,20 +120,36 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
 __device__ __forceinline__ float low_of(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float high_of(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
 
-// The operand pairs of a word's eight codes, in the order of its shifts: 128 + code, or with CENTRED
-// code - 8.
-template <bool CENTRED>
-__device__ __forceinline__ void expand(uint32_t word, uint32_t (&pair)[4]) {
+// The operand pairs of a word's eight codes, in the order of their bits: code - 8 as bfloat16 ...
+__device__ __forceinline__ void expand_centred(uint32_t word, uint32_t (&pair)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        pair[i] = ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-        if (CENTRED) {
-            const uint32_t middle = 0x43084308u;                     // 136
-            const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&pair[i]),
-                                             *reinterpret_cast<const __nv_bfloat162*>(&middle));
-            pair[i] = *reinterpret_cast<const uint32_t*>(&v);
-        }
+        pair[i] = ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;       // 128 + code
+        const uint32_t middle = 0x43084308u;                             // 136
+        const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&pair[i]),
+                                         *reinterpret_cast<const __nv_bfloat162*>(&middle));
+        pair[i] = *reinterpret_cast<const uint32_t*>(&v);
     }
+}
+// ... or in half-precision code * 2^-24, the second and the fourth pair 16 times that.
+__device__ __forceinline__ void expand_small(uint32_t word, uint32_t (&pair)[4]) {
+    pair[0] = word & 0x000f000fu;
+    pair[1] = word & 0x00f000f0u;
+    word >>= 8;
+    pair[2] = word & 0x000f000fu;
+    pair[3] = word & 0x00f000f0u;
+}
+constexpr float CODE_UNIT = 16777216.f;                // 2^24
+
+// 2^(to - floor(log2 x)) for x > 0, and its inverse; x is taken for 2^-113 at least
+__device__ __forceinline__ float power_towards(float x, int to, float& inverse) {
+    const int exponent = max((int)(__float_as_uint(x) >> 23 & 255u), 14);
+    inverse = __uint_as_float((uint32_t)(exponent - to) << 23);
+    return __uint_as_float((uint32_t)(254 - (exponent - to)) << 23);
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 // Cuts a pair of 32-bit values into NP pairs of bfloat16 parts, the largest first: their sum is the value.
@@ -153,7 +186,7 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
     constexpr bool WIDE = sizeof(T) == 4;                  // 32-bit queries
     constexpr int NP = WIDE ? 3 : 1;                       // bfloat16 parts of a value
     constexpr int RUNS = P::RUNS, GROUPS = P::GROUPS, GROUP_RUNS = P::GROUP / 16;
-    constexpr float MIDDLE = WIDE ? 8.f : 128.f;
+    constexpr float MIDDLE = 8.f;                          // of the centred codes
     extern __shared__ unsigned char shared_raw[];
     __shared__ __align__(8) unsigned long long barriers[WARPS * R::STAGES];
     unsigned char* shared = reinterpret_cast<unsigned char*>((reinterpret_cast<size_t>(shared_raw) + 127) &
@@ -245,6 +278,30 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
         sums[g][1] = sum[1] + small[1];
     }
 
+    // bfloat16 queries as half-precision, and what a score's product with the codes is then to be multiplied by
+    float code_scale = scale_log2;
+    if constexpr (!WIDE) {
+        float most = 0.f;
+#pragma unroll
+        for (int s = 0; s < RUNS; ++s)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const float a = fabsf(low_of(qb[s][half][0])), b = fabsf(high_of(qb[s][half][0]));
+                if (a < INFINITY) most = fmaxf(most, a);
+                if (b < INFINITY) most = fmaxf(most, b);
+            }
+        float inverse;
+        const float by = power_towards(warp_max(most), 13, inverse);
+        code_scale = scale_log2 * CODE_UNIT * inverse;
+#pragma unroll
+        for (int s = 0; s < RUNS; ++s)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const float to = half ? by * 0.0625f : by;
+                qb[s][half][0] = pack_half(low_of(qb[s][half][0]) * to, high_of(qb[s][half][0]) * to);
+            }
+    }
+
     float m[2] = {NOTHING, NOTHING}, l[2] = {0.f, 0.f};      // heads 2c, 2c + 1; l: this lane's share
     if (sinks != nullptr && split == 0 && warp == 0) {
 #pragma unroll
@@ -256,17 +313,14 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
                 if (r == 0) l[i] = fast_exp2(sink - m[i]);
             }
     }
-    float o[RUNS][4], lows[GROUPS][2], weights[GROUPS][4];   // outputs, sums of p lowest, sums of p step
+    float o[RUNS][4], lows[GROUPS][2];     // outputs, sums of p lowest
+    float grown = 1.2676506e30f, shrunk = 7.8886091e-31f;    // (not WIDE) the weights' power of two, 2^100 at first
 #pragma unroll
     for (int s = 0; s < RUNS; ++s)
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[s][k] = 0.f;
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
-        lows[g][0] = lows[g][1] = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) weights[g][k] = 0.f;
-    }
+    for (int g = 0; g < GROUPS; ++g) lows[g][0] = lows[g][1] = 0.f;
 
     bool ok = true;
     int stage = 0;
@@ -294,9 +348,7 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
             for (int k = 0; k < 4; ++k) s[u][k] = 0.f;
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
-                float acc[4], small[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) acc[k] = WIDE ? 0.f : -MIDDLE * sums[g][k & 1];
+                float acc[4] = {0.f, 0.f, 0.f, 0.f}, small[4] = {0.f, 0.f, 0.f, 0.f};
                 uint32_t words[GROUP_RUNS];
                 const unsigned char* at = part + P::word_at(lane, g * GROUP_RUNS);
                 if constexpr (GROUP_RUNS == 4) {
@@ -309,14 +361,19 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
 #pragma unroll
                 for (int k = 0; k < GROUP_RUNS; ++k) {
                     uint32_t a[4];
-                    expand<WIDE>(words[k], a);
+                    const auto& b = qb[g * GROUP_RUNS + k];
+                    if constexpr (WIDE) {
+                        expand_centred(words[k], a);
 #pragma unroll
-                    for (int n = NP - 1; n >= 0; --n)
-                        mma_16816(n ? small : acc, a[0], a[2], a[1], a[3], qb[g * GROUP_RUNS + k][0][n],
-                                  qb[g * GROUP_RUNS + k][1][n]);
+                        for (int n = NP - 1; n >= 0; --n)
+                            mma_16816(n ? small : acc, a[0], a[2], a[1], a[3], b[0][n], b[1][n]);
+                    } else {
+                        expand_small(words[k], a);
+                        mma_half(acc, a[0], a[2], a[1], a[3], b[0][0], b[1][0]);
+                    }
                 }
                 const uint2 scale = *reinterpret_cast<const uint2*>(part + P::scale_at(r, g));
-                const float step[2] = {packed_step(scale.x) * scale_log2, packed_step(scale.y) * scale_log2};
+                const float step[2] = {packed_step(scale.x) * code_scale, packed_step(scale.y) * code_scale};
                 float low[2] = {packed_lowest(scale.x) * scale_log2, packed_lowest(scale.y) * scale_log2};
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -346,28 +403,52 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
                 for (int k = 0; k < 4; ++k)
                     if (!(seen >> (4 * u + k) & 1u)) s[u][k] = -INFINITY;
         }
+        // the values' steps and lowest values of this lane's keys (r, r + 8 of either unit); of keys that are not
+        // seen, whatever lies there, zeros
+        float step[GROUPS][2][2], low[GROUPS][2][2], largest = 0.f;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint2 scale = *reinterpret_cast<const uint2*>(held + u * P::UNIT + P::PART + P::scale_at(r, g));
+                step[g][u][0] = packed_step(scale.x); step[g][u][1] = packed_step(scale.y);
+                low[g][u][0] = packed_lowest(scale.x); low[g][u][1] = packed_lowest(scale.y);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (!open && !(seen >> (4 * u + 2 * i) & 1u)) step[g][u][i] = low[g][u][i] = 0.f;
+                    if (WIDE) low[g][u][i] = fmaf(MIDDLE, step[g][u][i], low[g][u][i]);
+                    else largest = fmaxf(largest, step[g][u][i]);
+                }
+            }
         float top[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) top[i] = fmaxf(fmaxf(s[0][i], s[0][i + 2]), fmaxf(s[1][i], s[1][i + 2]));
-        if (__any_sync(0xffffffffu, top[0] > m[0] + LAZY || top[1] > m[1] + LAZY)) {
+        if (__any_sync(0xffffffffu, top[0] > m[0] + LAZY || top[1] > m[1] + LAZY ||
+                                        (!WIDE && largest * grown > 1024.f))) {
+            float resized = 1.f;
+            if constexpr (!WIDE) {
+                largest = warp_max(largest);
+                if (largest * grown > 1024.f) {
+                    const float before = shrunk;
+                    grown = power_towards(largest, 9, shrunk);
+                    resized = grown * before;
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int offset = 4; offset < 32; offset <<= 1)
                     top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], offset));
                 const float raised = fmaxf(m[i], top[i]);
-                const float by = fast_exp2(m[i] - raised);
+                const float by = fast_exp2(m[i] - raised), of_output = by * resized;
                 m[i] = raised;
                 l[i] *= by;
 #pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
-                    lows[g][i] *= by;
-                    weights[g][i] *= by;
-                }
+                for (int g = 0; g < GROUPS; ++g) lows[g][i] *= by;
 #pragma unroll
                 for (int k = 0; k < RUNS; ++k) {
-                    o[k][i] *= by;
-                    o[k][i + 2] *= by;
+                    o[k][i] *= of_output;
+                    o[k][i + 2] *= of_output;
                 }
             }
         }
@@ -384,29 +465,18 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
             // the group's weights p step, transposed: keys 2c, + 1 (and + 8), head r
             uint32_t pb[2][2][NP];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint2 scale = *reinterpret_cast<const uint2*>(held + u * P::UNIT + P::PART + P::scale_at(r, g));
-                const float step[2] = {packed_step(scale.x), packed_step(scale.y)};
-                float low[2] = {packed_lowest(scale.x), packed_lowest(scale.y)};
-                float weight[4];
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (WIDE) low[i] = fmaf(MIDDLE, step[i], low[i]);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    weight[k] = p[u][k] * step[k >> 1];
-                    float taken = p[u][k] * low[k >> 1];
-                    if (!open && !(seen >> (4 * u + k) & 1u)) weight[k] = taken = 0.f;   // whatever lies there
-                    lows[g][k & 1] += taken;
-                }
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    parts_of<NP>(weight[2 * half], weight[2 * half + 1], pb[u][half]);
+                    const float factor = WIDE ? step[g][u][half] : step[g][u][half] * grown;
+                    const float a = p[u][2 * half] * factor, b = p[u][2 * half + 1] * factor;
+                    lows[g][0] = fmaf(p[u][2 * half], low[g][u][half], lows[g][0]);
+                    lows[g][1] = fmaf(p[u][2 * half + 1], low[g][u][half], lows[g][1]);
+                    if constexpr (WIDE) parts_of<NP>(a, b, pb[u][half]);
+                    else pb[u][half][0] = pack_half(a, b);
 #pragma unroll
                     for (int n = 0; n < NP; ++n) pb[u][half][n] = transpose_8x8(pb[u][half][n]);
                 }
-                if (!WIDE) mma_16816(weights[g], ONES, ONES, ONES, ONES, pb[u][0][0], pb[u][1][0]);
-            }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const unsigned char* at = held + u * P::UNIT + P::PART + P::word_at(lane, g * GROUP_RUNS);
@@ -421,16 +491,18 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
 #pragma unroll
                 for (int k = 0; k < GROUP_RUNS; ++k) {
                     uint32_t a[4];
-                    expand<WIDE>(words[k], a);
+                    float (&to)[4] = o[g * GROUP_RUNS + k];
                     if constexpr (WIDE) {
+                        expand_centred(words[k], a);
                         float small[4] = {0.f, 0.f, 0.f, 0.f}, large[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int n = NP - 1; n >= 0; --n)
                             mma_16816(n ? small : large, a[0], a[1], a[2], a[3], pb[u][0][n], pb[u][1][n]);
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) o[g * GROUP_RUNS + k][x] += large[x] + small[x];
+                        for (int x = 0; x < 4; ++x) to[x] += large[x] + small[x];
                     } else {
-                        mma_16816(o[g * GROUP_RUNS + k], a[0], a[1], a[2], a[3], pb[u][0][0], pb[u][1][0]);
+                        expand_small(words[k], a);
+                        mma_half(to, a[0], a[1], a[2], a[3], pb[u][0][0], pb[u][1][0]);
                     }
                 }
             }
@@ -466,9 +538,11 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
 #pragma unroll
             for (int k = 0; k < RUNS; ++k) {
                 const int g = k / GROUP_RUNS;
-                const float base = lows[g][i] - (WIDE ? 0.f : MIDDLE * weights[g][i]);
-                row[16 * k + r] = o[k][i] + base;
-                row[16 * k + r + 8] = o[k][i + 2] + base;
+                // (not WIDE: codes were 2^-24 of themselves, 2^-20 in dimensions r + 8, weights `grown` times)
+                const float a = WIDE ? o[k][i] : o[k][i] * CODE_UNIT * shrunk;
+                const float b = WIDE ? o[k][i + 2] : o[k][i + 2] * (CODE_UNIT / 16.f) * shrunk;
+                row[16 * k + r] = a + lows[g][i];
+                row[16 * k + r + 8] = b + lows[g][i];
             }
             if (r == 0) {
                 row[HD] = m[i];
