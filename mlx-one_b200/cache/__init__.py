@@ -1,6 +1,6 @@
 from .errors import CacheCapacityError, CacheError, CacheOwnershipError
-from .manager import CacheManager, CacheStats, RequestCache
+from .manager import CacheManager, CacheOrder, CacheStats, RequestCache
 from .pools import IndexPool
 
-__all__ = ["CacheCapacityError", "CacheError", "CacheOwnershipError", "CacheManager",
+__all__ = ["CacheCapacityError", "CacheError", "CacheOwnershipError", "CacheManager", "CacheOrder",
            "CacheStats", "RequestCache", "IndexPool"]

@@ -9,6 +9,7 @@ chunks that have ended. A fixed-state group owns a pool of slots; a request has 
 
 Storage (on the device, in place):
   paged group   [entries, planes, pages, kv_heads, page_size, head_dim]
+                with ``bits`` 4: uint8 [entries, pages, kv_heads, page_size / 16, 2, part bytes]
   state group   [entries, slots, *shape]
 
 Requests are opened, grown before a step (``grow``), advanced after it (``advance``) and
@@ -26,7 +27,8 @@ from typing import Any, Mapping
 
 import torch
 
-from ..parts.base import FixedState, PagedKeyValues, PagedView, StateView
+from ..parts.base import (FixedState, PackedView, PagedKeyValues, PagedView, StateView,
+                          packed_part_bytes)
 from .errors import CacheCapacityError, CacheOwnershipError
 from .pools import IndexPool
 
@@ -80,10 +82,16 @@ class CacheStats:
 class CacheManager:
     def __init__(self, needs: Mapping[int, Any], *, page_size: int, capacity_tokens: int,
                  max_requests: int, dtype: torch.dtype, device, max_step_tokens: int = 1 << 30,
-                 allocate: bool = True) -> None:
+                 allocate: bool = True, bits: int | None = None) -> None:
         """``needs``: cache entry -> ``PagedKeyValues`` | ``FixedState``.
         ``capacity_tokens``: tokens that all live requests may hold together; every paged
-        group gets ceil(capacity_tokens / page_size) pages."""
+        group gets ceil(capacity_tokens / page_size) pages. ``bits``: None (keys and values in
+        ``dtype``) or 4."""
+        if bits not in (None, 4):
+            raise ValueError(f"keys and values are held in the compute dtype or in 4 bits, not {bits}")
+        if bits and (page_size < 16 or page_size & (page_size - 1)):
+            raise ValueError(f"a cache of 4 bits has pages of 16, 32, 64 or 128 tokens, not {page_size}")
+        self.bits = bits
         if page_size < 1 or capacity_tokens < 1 or max_requests < 1:
             raise ValueError("page_size, capacity_tokens and max_requests must be positive")
         self.page_size = page_size
@@ -103,7 +111,14 @@ class CacheManager:
         for need, entries in by_need.items():
             if isinstance(need, PagedKeyValues):
                 storage = None
-                if allocate:
+                if bits and need.planes != 2:
+                    raise ValueError(f"cache entry {entries[0]} keeps {need.planes} rows per token, not keys "
+                                     "and values: it cannot be held in 4 bits")
+                part = packed_part_bytes(need.head_dim) if bits else 0
+                if allocate and bits:
+                    storage = torch.zeros((len(entries), pages + 1, need.kv_heads, page_size // 16, 2, part),
+                                          dtype=torch.uint8, device=self.device)
+                elif allocate:
                     # one page beyond the pool's: the scratch page (see ``scratch_page``)
                     storage = torch.zeros((len(entries), need.planes, pages + 1, need.kv_heads, page_size,
                                            need.head_dim), dtype=dtype, device=self.device)
@@ -285,9 +300,14 @@ class CacheManager:
         kind, group, index = self._where[entry]
         if kind == "paged":
             g = self.paged[group]
-            return PagedView(g.storage[index], tables[group], self.page_size, g.need)
+            kind = PackedView if self.bits else PagedView
+            return kind(g.storage[index], tables[group], self.page_size, g.need)
         g = self.states[group]
         return StateView(g.storage[index], slots[group], g.need)
+
+    def order_of(self, request_ids) -> "CacheOrder":
+        """What brings the caches of these requests to new owners among them (see ``CacheOrder``)."""
+        return CacheOrder(self, request_ids)
 
     def requests(self) -> tuple[Any, ...]:
         return tuple(self._requests)
@@ -324,3 +344,40 @@ class CacheManager:
             slots = [c.slots[index] for c in self._requests.values()]
             if len(set(slots)) != len(slots) or set(slots) != group.pool.held():
                 raise CacheOwnershipError("slots and requests disagree")
+
+
+class CacheOrder:
+    """Several requests of one length that take over one another's caches (the hypotheses of a beam
+    search). What their slots and pages are is kept on the device from one call to the next, and
+    brought there again when a request has got or given back a page."""
+
+    def __init__(self, cache: CacheManager, request_ids) -> None:
+        self.cache = cache
+        self.caches = [cache.get(request_id) for request_id in request_ids]
+        self.slots = [self._ints([c.slots[index] for c in self.caches]) for index in range(len(cache.states))]
+        self.start = self._ints([0])
+        self._rows: list[tuple] = [((), None, None) for _ in cache.paged]
+
+    def _ints(self, values) -> torch.Tensor:
+        return torch.tensor(values, dtype=torch.int32, device=self.cache.device)
+
+    def apply(self, ops, parents: torch.Tensor, first: int = 0) -> None:
+        """Request b gets what request ``parents[b]`` holds, for all at once, on the device and in place:
+        fixed-size state, and pages from the one of position ``first`` on (the requests hold the same
+        before it). ``parents``: int32 [requests] on the device."""
+        cache, length = self.cache, self.caches[0].length
+        if any(c.length != length for c in self.caches):
+            raise CacheOwnershipError("requests of different lengths cannot take over one another's caches")
+        parents = parents.view(1, len(self.caches))
+        for group, slots in zip(cache.states, self.slots):
+            ops.reorder_slots(group.storage, slots, parents)
+        begin, end = first // cache.page_size, ceil_div(length, cache.page_size)
+        if begin >= end:
+            return
+        for index, group in enumerate(cache.paged):
+            tables = tuple(tuple(c.tables[index][begin:end]) for c in self.caches)
+            if self._rows[index][0] != tables:
+                self._rows[index] = (tables, self._ints(tables), self._ints([(end - begin) * cache.page_size]))
+            _, rows, held = self._rows[index]
+            storage = group.storage if cache.bits else group.storage.flatten(0, 1)
+            ops.reorder_pages(storage, rows, parents, self.start, held, page_size=cache.page_size)

@@ -34,19 +34,41 @@ def main() -> None:
                    "printed. For model folders without a tokenizer.")
 @click.option("--dtype", type=click.Choice(["bfloat16", "float32"]), default="bfloat16",
               show_default=True, help="Execution dtype.")
+@click.option("--cache-bits", type=click.Choice(["4"]), default=None,
+              help="Hold keys and values in 4 bits instead of the execution dtype.")
+@click.option("--beams", type=click.IntRange(min=1, max=32), default=None,
+              help="Beam search with so many hypotheses; the best one is printed (all as JSON).")
+@click.option("--length-penalty", type=float, default=1.0, show_default=True,
+              help="Hypotheses are ranked by score / length ** penalty.")
 @click.option("--device", default="cuda:0", show_default=True)
 def generate_command(model, prompt, revision, offline, cache_dir, max_tokens, temperature, top_k, top_p, seed, stop, stream,
-                     as_json, token_ids, dtype, device) -> None:
-    from .engine import Engine
+                     as_json, token_ids, dtype, cache_bits, beams, length_penalty, device) -> None:
+    from .engine import CacheConfig, Engine
     from .sampling import TextGenerationOptions
 
     try:
         options = TextGenerationOptions(max_tokens=max_tokens, temperature=temperature,
                                         top_k=top_k, top_p=top_p, seed=seed, stop=stop)
+        more = {}
+        if cache_bits or beams:
+            # (a hypothesis is a request of the cache)
+            more["cache_config"] = CacheConfig(bits=int(cache_bits) if cache_bits else None, max_requests=beams)
         engine = Engine(model, execution_dtype=dtype, device=device, revision=revision,
-                        offline=True, cache_dir=cache_dir)
+                        offline=True, cache_dir=cache_dir, **more)
         ids = ([int(v) for v in prompt.replace(",", " ").split()] if token_ids
                else engine.encode(prompt))
+        if beams:
+            if stream:
+                raise ValueError("a beam search has nothing to stream")
+            results = engine.generate_beams_ids(ids, options, beams=beams, length_penalty=length_penalty,
+                                                prompt_text="" if token_ids else prompt)
+            if as_json:
+                click.echo(json.dumps([r.to_dict() for r in results], sort_keys=True, indent=2))
+            elif token_ids:
+                click.echo(" ".join(str(t) for t in results[0].token_ids))
+            else:
+                click.echo(results[0].text)
+            return
         if stream:
             for chunk in engine.stream_ids(ids, options):
                 if as_json:

@@ -1,3 +1,3 @@
-from .options import GenerationChunk, GenerationResult, TextGenerationOptions
+from .options import BeamResult, GenerationChunk, GenerationResult, TextGenerationOptions
 
-__all__ = ["GenerationChunk", "GenerationResult", "TextGenerationOptions"]
+__all__ = ["BeamResult", "GenerationChunk", "GenerationResult", "TextGenerationOptions"]

@@ -88,3 +88,12 @@ class GenerationResult:
 
     def to_json(self) -> str:
         return json.dumps(self.to_dict(), sort_keys=True, indent=2)
+
+
+@dataclass(frozen=True)
+class BeamResult(GenerationResult):
+    """One hypothesis of a beam search: ``score`` is the sum of its tokens' logarithms (an
+    end-of-sequence token's among them), by which, divided by length to the power of the penalty,
+    hypotheses are ranked."""
+
+    score: float = 0.0
