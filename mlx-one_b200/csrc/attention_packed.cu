@@ -33,6 +33,8 @@
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "packed_cache.cuh"
 
 namespace cg = cooperative_groups;
@@ -40,7 +42,6 @@ namespace cg = cooperative_groups;
 namespace {
 
 using bf16 = __nv_bfloat16;
-constexpr int KEYS = 32;               // keys of a tile: two units
 constexpr int WARPS = 8;
 constexpr int HEADS = 8;               // query heads of a block
 constexpr int WAIT_LIMIT = 1 << 22;
@@ -49,10 +50,15 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NOTHING = -1e30f;      // a maximum of no scores: finite, so that differences stay numbers
 constexpr float LAZY = 4.f;
 
-template <int HD>
+// Keys of a tile, and tiles of a warp's ring. 64 keys with heads of up to 64 values (what a tile costs beside its
+// keys, the look-up of pages, the copies, the wait and the vote, is paid half as often), 32 where registers
+// are short.
+template <typename T, int HD>
 struct Ring {
-    static constexpr int STAGES = HD <= 64 ? 4 : 3;
-    static constexpr int STAGE = 2 * Packed<HD>::UNIT;
+    static constexpr int KEYS = HD <= 64 && sizeof(T) == 2 ? 64 : 32;
+    static constexpr int UNITS = KEYS / 16;
+    static constexpr int STAGES = HD == 32 ? 4 : 3;
+    static constexpr int STAGE = UNITS * Packed<HD>::UNIT;
     static constexpr int BYTES = WARPS * STAGES * STAGE;
     // what the merge needs: a maximum, a sum and an output per head, for every warp and then for the block
     static constexpr int MERGE = (WARPS + 1) * HEADS * (HD + 2) * 4;
@@ -163,6 +169,15 @@ __device__ __forceinline__ void parts_of(float a, float b, uint32_t (&part)[NP])
     }
 }
 
+__device__ __forceinline__ void load_words(const unsigned char* at, uint32_t (&words)[4]) {
+    const uint4 w = *reinterpret_cast<const uint4*>(at);
+    words[0] = w.x; words[1] = w.y; words[2] = w.z; words[3] = w.w;
+}
+__device__ __forceinline__ void load_words(const unsigned char* at, uint32_t (&words)[2]) {
+    const uint2 w = *reinterpret_cast<const uint2*>(at);
+    words[0] = w.x; words[1] = w.y;
+}
+
 template <typename T>
 __device__ __forceinline__ void store_pair(T* dst, float a, float b);
 template <>
@@ -175,14 +190,15 @@ __device__ __forceinline__ void store_pair<bf16>(bf16* dst, float a, float b) {
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(WARPS * 32, HD <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(WARPS * 32, HD <= 64 || sizeof(T) == 2 ? 2 : 1)
 attention_packed_kernel(const T* q, const unsigned char* cache,
                         const int* block_table, int table_width, int page_shift, int pages,
                         const int* positions, T* out, float* partial,
                         int heads, int kv_heads, int splits, float scale_log2, int window,
                         const float* sinks, int* error_flag) {
     using P = Packed<HD>;
-    using R = Ring<HD>;
+    using R = Ring<T, HD>;
+    constexpr int KEYS = R::KEYS, UNITS = R::UNITS;
     constexpr bool WIDE = sizeof(T) == 4;                  // 32-bit queries
     constexpr int NP = WIDE ? 3 : 1;                       // bfloat16 parts of a value
     constexpr int RUNS = P::RUNS, GROUPS = P::GROUPS, GROUP_RUNS = P::GROUP / 16;
@@ -220,30 +236,40 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
     const int units_per_page = 1 << (page_shift - 4);
     unsigned char* ring = shared + warp * R::STAGES * R::STAGE;
     auto barrier = [&](int stage) { return shared_address(&barriers[warp * R::STAGES + stage]); };
-    // lanes 0 and 1 look after the two units of a tile: where it lies, or -1 if no key of it is seen
-    auto look_up = [&](int tile) -> long long {
-        const int key = tile * KEYS + 16 * lane;
-        if (lane > 1 || tile >= to || key > position || key + 15 < lowest_key) return -1;
+    // Where the units of a warp's tiles lie, a lane each for AHEAD tiles at a time (lane = tile of these * UNITS +
+    // unit; -1: no key of it is seen); the next ones are looked up half a turn before the first is wanted.
+    constexpr int AHEAD = 32 / UNITS;
+    auto look_up = [&](int first_tile) -> long long {
+        const int tile = first_tile + lane / UNITS * WARPS;
+        const int key = tile * KEYS + 16 * (lane % UNITS);
+        if (tile >= to || key > position || key + 15 < lowest_key) return -1;
         const int block = key >> page_shift;
         const int page = block < table_width ? table[block] : -1;
         if (page < 0 || page >= pages) return -1;
         return ((long long)page * kv_heads + kv_head) * units_per_page + ((key & ((1 << page_shift) - 1)) >> 4);
     };
-    uint32_t live_units = 0;               // two bits a stage: which units it holds
-    auto fetch = [&](int stage, long long unit) {
-        const unsigned live = __ballot_sync(0xffffffffu, unit >= 0);
-        live_units = (live_units & ~(3u << (2 * stage))) | live << (2 * stage);
+    uint32_t live_units = 0;               // UNITS bits a stage: which units it holds
+    constexpr uint32_t EVERY = (1u << UNITS) - 1;
+    int tile = from + warp, turn = 0;          // turn: of AHEAD, the place of the next tile to be asked for
+    long long units_now = look_up(tile), units_next = -1;
+    auto fetch = [&](int stage, int asked) {
+        const long long unit = __shfl_sync(0xffffffffu, units_now, turn * UNITS + (lane & (UNITS - 1)));
+        const unsigned live = __ballot_sync(0xffffffffu, unit >= 0) & EVERY;
+        live_units = (live_units & ~(EVERY << (UNITS * stage))) | live << (UNITS * stage);
         if (lane == 0) barrier_expect(barrier(stage), (uint32_t)__popc(live) * P::UNIT);
         __syncwarp();
-        if (unit >= 0)
+        if (lane < UNITS && unit >= 0)
             bulk_load(shared_address(ring + stage * R::STAGE + lane * P::UNIT), codes + (size_t)unit * P::UNIT,
                       P::UNIT, barrier(stage));
+        if (turn == AHEAD / 2) units_next = look_up(asked + (AHEAD - AHEAD / 2) * WARPS);
+        if (++turn == AHEAD) {
+            turn = 0;
+            units_now = units_next;
+        }
     };
-    int tile = from + warp;
 #pragma unroll
     for (int ahead = 0; ahead < R::STAGES - 1; ++ahead)
-        if (tile + ahead * WARPS < to) fetch(ahead, look_up(tile + ahead * WARPS));
-    long long coming = look_up(tile + (R::STAGES - 1) * WARPS);
+        if (tile + ahead * WARPS < to) fetch(ahead, tile + ahead * WARPS);
 
     // q^T as the 8-column operand (head r, dims 16 s + 2c, + 1 and + 8), in NP parts
     uint32_t qb[RUNS][2][NP];
@@ -263,7 +289,7 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
                 }
             }
     }
-    // sum(q) of every group for heads 2c and 2c + 1, by a product with ones
+    // scale sum(q) of every group for heads 2c and 2c + 1, by a product with ones
     constexpr uint32_t ONES = 0x3f803f80u;
     float sums[GROUPS][2];
 #pragma unroll
@@ -274,8 +300,8 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
 #pragma unroll
             for (int n = NP - 1; n >= 0; --n)
                 mma_16816(n ? small : sum, ONES, ONES, ONES, ONES, qb[s][0][n], qb[s][1][n]);
-        sums[g][0] = sum[0] + small[0];
-        sums[g][1] = sum[1] + small[1];
+        sums[g][0] = (sum[0] + small[0]) * scale_log2;
+        sums[g][1] = (sum[1] + small[1]) * scale_log2;
     }
 
     // bfloat16 queries as half-precision, and what a score's product with the codes is then to be multiplied by
@@ -302,15 +328,21 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
             }
     }
 
-    float m[2] = {NOTHING, NOTHING}, l[2] = {0.f, 0.f};      // heads 2c, 2c + 1; l: this lane's share
+    // heads 2c, 2c + 1: what scores are taken against, whether that has come from a score yet, this lane's
+    // share of the sum
+    float m[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
+    bool begun[2] = {false, false};
     if (sinks != nullptr && split == 0 && warp == 0) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
             if (2 * c + i < rows) {
                 // a sink: a term of the denominator with neither key nor value
                 const float sink = sinks[head0 + 2 * c + i] * LOG2E;
-                m[i] = fmaxf(sink, NOTHING);
-                if (r == 0) l[i] = fast_exp2(sink - m[i]);
+                begun[i] = !(sink < NOTHING);
+                if (begun[i]) {
+                    m[i] = sink;
+                    l[i] = r == 0 ? 1.f : 0.f;
+                }
             }
     }
     float o[RUNS][4], lows[GROUPS][2];     // outputs, sums of p lowest
@@ -322,42 +354,30 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) lows[g][0] = lows[g][1] = 0.f;
 
-    bool ok = true;
-    int stage = 0;
-    uint32_t parity = 0;
-    for (; tile < to; tile += WARPS) {
-        {
-            const int next = tile + (R::STAGES - 1) * WARPS;
-            __syncwarp();                  // every lane is done with the stage that is filled now
-            if (next < to) fetch(stage == 0 ? R::STAGES - 1 : stage - 1, coming);
-            coming = look_up(next + WARPS);
-        }
-        for (int i = 0; !barrier_test(barrier(stage), parity); ++i)
-            if (i >= WAIT_LIMIT) { ok = false; break; }
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const unsigned char* held = ring + stage * R::STAGE;
-        const uint32_t live = live_units >> (2 * stage) & 3u;
-        const int first = tile * KEYS;
-
-        float s[2][4];
+    // One tile: `held` its units, of which `live` are there; `first` its first key.
+    auto attend = [&](auto masked, const unsigned char* held, uint32_t live, int first) {
+        constexpr bool MASKED = decltype(masked)::value;
+        // which of this lane's keys are seen: two bits a unit, r and r + 8
+        uint32_t seen = 0;
+        if (MASKED) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+            for (int i = 0; i < 2 * UNITS; ++i) {
+                const int key = first + 8 * i + r;
+                if ((live >> (i >> 1) & 1u) && key >= lowest_key && key <= position) seen |= 1u << i;
+            }
+        }
+        // scores (times log2 e), less what they are taken against
+        float s[UNITS][4];
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
             const unsigned char* part = held + u * P::UNIT;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[u][k] = 0.f;
+            for (int k = 0; k < 4; ++k) s[u][k] = -m[k & 1];
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
                 float acc[4] = {0.f, 0.f, 0.f, 0.f}, small[4] = {0.f, 0.f, 0.f, 0.f};
                 uint32_t words[GROUP_RUNS];
-                const unsigned char* at = part + P::word_at(lane, g * GROUP_RUNS);
-                if constexpr (GROUP_RUNS == 4) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(at);
-                    words[0] = w.x; words[1] = w.y; words[2] = w.z; words[3] = w.w;
-                } else {
-                    const uint2 w = *reinterpret_cast<const uint2*>(at);
-                    words[0] = w.x; words[1] = w.y;
-                }
+                load_words(part + P::word_at(lane, g * GROUP_RUNS), words);
 #pragma unroll
                 for (int k = 0; k < GROUP_RUNS; ++k) {
                     uint32_t a[4];
@@ -374,56 +394,46 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
                 }
                 const uint2 scale = *reinterpret_cast<const uint2*>(part + P::scale_at(r, g));
                 const float step[2] = {packed_step(scale.x) * code_scale, packed_step(scale.y) * code_scale};
-                float low[2] = {packed_lowest(scale.x) * scale_log2, packed_lowest(scale.y) * scale_log2};
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (WIDE) low[i] = fmaf(MIDDLE, step[i], low[i]);
+                float low[2] = {packed_lowest(scale.x), packed_lowest(scale.y)};
+                if (WIDE) {
+                    low[0] = fmaf(MIDDLE, packed_step(scale.x), low[0]);
+                    low[1] = fmaf(MIDDLE, packed_step(scale.y), low[1]);
+                }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     s[u][k] = fmaf(low[k >> 1], sums[g][k & 1], s[u][k]);
                     s[u][k] = fmaf(step[k >> 1], NP > 1 ? acc[k] + small[k] : acc[k], s[u][k]);
                 }
             }
-        }
-        // (a tile whose keys are all seen needs no mask)
-        const bool open = live == 3u && first >= lowest_key && first + KEYS - 1 <= position;
-        uint32_t seen = 0xffu;
-        if (!open) {
-            seen = 0;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int key = first + 16 * u + 8 * half + r;
-                    if ((live >> u & 1u) && key >= lowest_key && key <= position) seen |= 3u << (4 * u + 2 * half);
-                }
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
+            if (MASKED) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (!(seen >> (4 * u + k) & 1u)) s[u][k] = -INFINITY;
+                    if (!(seen >> (2 * u + (k >> 1)) & 1u)) s[u][k] = -INFINITY;
+            }
         }
-        // the values' steps and lowest values of this lane's keys (r, r + 8 of either unit); of keys that are not
-        // seen, whatever lies there, zeros
-        float step[GROUPS][2][2], low[GROUPS][2][2], largest = 0.f;
+        // the values' steps and lowest values of this lane's keys; of keys that are not seen, whatever lies
+        // there, zeros
+        float step[GROUPS][UNITS][2], low[GROUPS][UNITS][2], largest = 0.f;
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < UNITS; ++u) {
                 const uint2 scale = *reinterpret_cast<const uint2*>(held + u * P::UNIT + P::PART + P::scale_at(r, g));
                 step[g][u][0] = packed_step(scale.x); step[g][u][1] = packed_step(scale.y);
                 low[g][u][0] = packed_lowest(scale.x); low[g][u][1] = packed_lowest(scale.y);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    if (!open && !(seen >> (4 * u + 2 * i) & 1u)) step[g][u][i] = low[g][u][i] = 0.f;
+                    if (MASKED && !(seen >> (2 * u + i) & 1u)) step[g][u][i] = low[g][u][i] = 0.f;
                     if (WIDE) low[g][u][i] = fmaf(MIDDLE, step[g][u][i], low[g][u][i]);
                     else largest = fmaxf(largest, step[g][u][i]);
                 }
             }
-        float top[2];
+        float top[2] = {s[0][0], s[0][1]};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) top[i] = fmaxf(fmaxf(s[0][i], s[0][i + 2]), fmaxf(s[1][i], s[1][i + 2]));
-        if (__any_sync(0xffffffffu, top[0] > m[0] + LAZY || top[1] > m[1] + LAZY ||
+        for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) top[k & 1] = fmaxf(top[k & 1], s[u][k]);
+        if (__any_sync(0xffffffffu, fmaxf(top[0], top[1]) > LAZY || !(begun[0] && begun[1]) ||
                                         (!WIDE && largest * grown > 1024.f))) {
             float resized = 1.f;
             if constexpr (!WIDE) {
@@ -439,10 +449,18 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
 #pragma unroll
                 for (int offset = 4; offset < 32; offset <<= 1)
                     top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], offset));
-                const float raised = fmaxf(m[i], top[i]);
-                const float by = fast_exp2(m[i] - raised), of_output = by * resized;
-                m[i] = raised;
+                // (the first score of a head may lie anywhere; from then on the maximum only rises)
+                const bool any = top[i] > -INFINITY;
+                const float rise = begun[i] ? fmaxf(top[i], 0.f) : any ? top[i] : 0.f;
+                const float by = begun[i] ? fast_exp2(-rise) : 1.f, of_output = by * resized;
+                begun[i] = begun[i] || any;
+                m[i] += rise;
                 l[i] *= by;
+#pragma unroll
+                for (int u = 0; u < UNITS; ++u) {
+                    s[u][i] -= rise;
+                    s[u][i + 2] -= rise;
+                }
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) lows[g][i] *= by;
 #pragma unroll
@@ -452,42 +470,32 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
                 }
             }
         }
-        float p[2][4];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < UNITS; ++u)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                p[u][k] = fast_exp2(s[u][k] - m[k & 1]);
-                l[k & 1] += p[u][k];
+                s[u][k] = fast_exp2(s[u][k]);                // from here on p
+                l[k & 1] += s[u][k];
             }
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-            // the group's weights p step, transposed: keys 2c, + 1 (and + 8), head r
-            uint32_t pb[2][2][NP];
+        for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < UNITS; ++u) {
+                // the group's weights p step, transposed: keys 2c, + 1 (and + 8), head r
+                uint32_t pb[2][NP];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const float factor = WIDE ? step[g][u][half] : step[g][u][half] * grown;
-                    const float a = p[u][2 * half] * factor, b = p[u][2 * half + 1] * factor;
-                    lows[g][0] = fmaf(p[u][2 * half], low[g][u][half], lows[g][0]);
-                    lows[g][1] = fmaf(p[u][2 * half + 1], low[g][u][half], lows[g][1]);
-                    if constexpr (WIDE) parts_of<NP>(a, b, pb[u][half]);
-                    else pb[u][half][0] = pack_half(a, b);
+                    lows[g][0] = fmaf(s[u][2 * half], low[g][u][half], lows[g][0]);
+                    lows[g][1] = fmaf(s[u][2 * half + 1], low[g][u][half], lows[g][1]);
+                    const float a = s[u][2 * half] * factor, b = s[u][2 * half + 1] * factor;
+                    if constexpr (WIDE) parts_of<NP>(a, b, pb[half]);
+                    else pb[half][0] = pack_half(a, b);
 #pragma unroll
-                    for (int n = 0; n < NP; ++n) pb[u][half][n] = transpose_8x8(pb[u][half][n]);
+                    for (int n = 0; n < NP; ++n) pb[half][n] = transpose_8x8(pb[half][n]);
                 }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const unsigned char* at = held + u * P::UNIT + P::PART + P::word_at(lane, g * GROUP_RUNS);
                 uint32_t words[GROUP_RUNS];
-                if constexpr (GROUP_RUNS == 4) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(at);
-                    words[0] = w.x; words[1] = w.y; words[2] = w.z; words[3] = w.w;
-                } else {
-                    const uint2 w = *reinterpret_cast<const uint2*>(at);
-                    words[0] = w.x; words[1] = w.y;
-                }
+                load_words(held + u * P::UNIT + P::PART + P::word_at(lane, g * GROUP_RUNS), words);
 #pragma unroll
                 for (int k = 0; k < GROUP_RUNS; ++k) {
                     uint32_t a[4];
@@ -497,16 +505,39 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
                         float small[4] = {0.f, 0.f, 0.f, 0.f}, large[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int n = NP - 1; n >= 0; --n)
-                            mma_16816(n ? small : large, a[0], a[1], a[2], a[3], pb[u][0][n], pb[u][1][n]);
+                            mma_16816(n ? small : large, a[0], a[1], a[2], a[3], pb[0][n], pb[1][n]);
 #pragma unroll
                         for (int x = 0; x < 4; ++x) to[x] += large[x] + small[x];
                     } else {
                         expand_small(words[k], a);
-                        mma_half(to, a[0], a[1], a[2], a[3], pb[u][0][0], pb[u][1][0]);
+                        mma_half(to, a[0], a[1], a[2], a[3], pb[0][0], pb[1][0]);
                     }
                 }
             }
+    };
+
+    bool ok = true;
+    int stage = 0;
+    uint32_t parity = 0;
+    for (; tile < to; tile += WARPS) {
+        {
+            const int next = tile + (R::STAGES - 1) * WARPS;
+            __syncwarp();                  // every lane is done with the stage that is filled now
+            if (next < to) fetch(stage == 0 ? R::STAGES - 1 : stage - 1, next);
         }
+        for (int i = 0; !barrier_test(barrier(stage), parity); ++i)
+            if (i >= WAIT_LIMIT) { ok = false; break; }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const unsigned char* held = ring + stage * R::STAGE;
+        const uint32_t live = live_units >> (UNITS * stage) & EVERY;
+        const int first = tile * KEYS;
+
+        // (a tile whose keys are all seen needs no mask)
+        if (live == EVERY && first >= lowest_key && first + KEYS - 1 <= position)
+            attend(std::false_type{}, held, live, first);
+        else
+            attend(std::true_type{}, held, live, first);
         stage = stage + 1 == R::STAGES ? 0 : stage + 1;
         if (stage == 0) parity ^= 1;
     }
@@ -545,7 +576,7 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
                 row[16 * k + r + 8] = b + lows[g][i];
             }
             if (r == 0) {
-                row[HD] = m[i];
+                row[HD] = begun[i] ? m[i] : NOTHING;
                 row[HD + 1] = l[i];
             }
         }
@@ -639,7 +670,7 @@ int launch_packed(const void* q, const void* cache, const int* block_table, int 
     cudaGetDevice(&device);
     if (prepared != device) {
         const cudaError_t error =
-            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<HD>::SHARED);
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring<T, HD>::SHARED);
         MLXONE_REQUIRE(error == cudaSuccess, "attention_packed: %s", cudaGetErrorString(error));
         prepared = device;
     }
@@ -647,7 +678,7 @@ int launch_packed(const void* q, const void* cache, const int* block_table, int 
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(splits, groups, requests);
     config.blockDim = dim3(WARPS * 32);
-    config.dynamicSmemBytes = Ring<HD>::SHARED;
+    config.dynamicSmemBytes = Ring<T, HD>::SHARED;
     config.stream = stream;
     cudaLaunchAttribute attributes[2];
     int count = 0;
@@ -684,7 +715,9 @@ int launch_packed(const void* q, const void* cache, const int* block_table, int 
 MLXONE_API int mlxone_attention_packed_cluster() { return 8; }
 
 // Blocks of the kernel that an SM holds at once.
-MLXONE_API int mlxone_attention_packed_resident(int head_dim) { return head_dim <= 64 ? 2 : 1; }
+MLXONE_API int mlxone_attention_packed_resident(int head_dim, int dtype) {
+    return head_dim <= 64 || dtype == MLXONE_BF16 ? 2 : 1;
+}
 
 // One token a request: q [requests, heads, head_dim], positions [requests] (each token's own position: the last key
 // that it sees; below 0: none). window: as first_visible_key's span. sinks: float32 [heads] or null. partial:

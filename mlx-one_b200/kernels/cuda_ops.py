@@ -2075,7 +2075,7 @@ class CudaOps:
             singles = 0
         bound = min(ctx.max_context, width * view.page_size)
         if singles:
-            splits = self.packed_splits(singles, heads, kv_heads, head_dim, bound, window)
+            splits = self.packed_splits(singles, heads, kv_heads, head_dim, bound, window, q.dtype)
             partial = None
             if splits > self._packed_cluster:
                 partial = torch.empty(singles * heads * splits * (head_dim + 2), dtype=torch.float32,
@@ -2135,13 +2135,13 @@ class CudaOps:
         return out
 
     def packed_splits(self, requests: int, heads: int, kv_heads: int, head_dim: int, context_bound: int,
-                      window: int) -> int:
+                      window: int, dtype=torch.bfloat16) -> int:
         """Into how many parts the kernel over packed pages cuts a request's keys: as many blocks as the
         GPU holds at once, each warp of a block with a tile of 32 keys at least."""
         if window:
             context_bound = min(context_bound, abs(window) + 31)
         blocks = requests * kv_heads * -(-(heads // kv_heads) // 8)
-        resident = self._sm_count * self.lib.mlxone_attention_packed_resident(head_dim)
+        resident = self._sm_count * self.lib.mlxone_attention_packed_resident(head_dim, _dtype_code(dtype))
         tiles = max(-(-context_bound // 32), 1)
         return max(min(resident // blocks, -(-tiles // 8)), 1)
 

@@ -14,7 +14,7 @@ class Library:
     def mlxone_packed_unit_bytes(self, dim):
         return 2 * packed_part_bytes(dim) if dim in (32, 64, 96, 128) else 0
 
-    def mlxone_attention_packed_resident(self, dim):
+    def mlxone_attention_packed_resident(self, dim, dtype):
         return 2
 
     def __getattr__(self, name):
