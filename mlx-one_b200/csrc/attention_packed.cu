@@ -44,6 +44,7 @@ namespace {
 using bf16 = __nv_bfloat16;
 constexpr int WARPS = 8;
 constexpr int HEADS = 8;               // query heads of a block
+constexpr int CLUSTER = 8;             // splits that a cluster merges
 constexpr int WAIT_LIMIT = 1 << 22;
 constexpr int ERROR_WAIT = 9;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -109,6 +110,15 @@ __device__ __forceinline__ void mma_half(float (&d)[4], uint32_t a0, uint32_t a1
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// ... and nothing to add to
+__device__ __forceinline__ void mma_half_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -122,6 +132,11 @@ __device__ __forceinline__ float fast_exp2(float x) {
 __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float max_of_three(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 __device__ __forceinline__ float low_of(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float high_of(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
@@ -217,9 +232,13 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
     const int r = lane >> 2, c = lane & 3;
 
     griddep_launch();
-    if (threadIdx.x < WARPS * R::STAGES) barrier_init(shared_address(&barriers[threadIdx.x]));
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    __syncthreads();
+    // (a warp's barriers are its own: nobody else waits for them or for their making)
+    if (lane == 0) {
+#pragma unroll
+        for (int k = 0; k < R::STAGES; ++k) barrier_init(shared_address(&barriers[warp * R::STAGES + k]));
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
     // Queries, and pages: the kernel before this one may have written this step's tokens there.
     griddep_wait();
     const T* queries = settled(q);
@@ -372,10 +391,12 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
         for (int u = 0; u < UNITS; ++u) {
             const unsigned char* part = held + u * P::UNIT;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[u][k] = -m[k & 1];
-#pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
-                float acc[4] = {0.f, 0.f, 0.f, 0.f}, small[4] = {0.f, 0.f, 0.f, 0.f};
+                float acc[4], small[4];
+                if constexpr (WIDE) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[k] = small[k] = 0.f;
+                }
                 uint32_t words[GROUP_RUNS];
                 load_words(part + P::word_at(lane, g * GROUP_RUNS), words);
 #pragma unroll
@@ -389,7 +410,8 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
                             mma_16816(n ? small : acc, a[0], a[2], a[1], a[3], b[0][n], b[1][n]);
                     } else {
                         expand_small(words[k], a);
-                        mma_half(acc, a[0], a[2], a[1], a[3], b[0][0], b[1][0]);
+                        if (k == 0) mma_half_first(acc, a[0], a[2], a[1], a[3], b[0][0], b[1][0]);
+                        else mma_half(acc, a[0], a[2], a[1], a[3], b[0][0], b[1][0]);
                     }
                 }
                 const uint2 scale = *reinterpret_cast<const uint2*>(part + P::scale_at(r, g));
@@ -401,7 +423,7 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    s[u][k] = fmaf(low[k >> 1], sums[g][k & 1], s[u][k]);
+                    s[u][k] = fmaf(low[k >> 1], sums[g][k & 1], g ? s[u][k] : -m[k & 1]);
                     s[u][k] = fmaf(step[k >> 1], NP > 1 ? acc[k] + small[k] : acc[k], s[u][k]);
                 }
             }
@@ -425,14 +447,16 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
                 for (int i = 0; i < 2; ++i) {
                     if (MASKED && !(seen >> (2 * u + i) & 1u)) step[g][u][i] = low[g][u][i] = 0.f;
                     if (WIDE) low[g][u][i] = fmaf(MIDDLE, step[g][u][i], low[g][u][i]);
-                    else largest = fmaxf(largest, step[g][u][i]);
                 }
+                if (!WIDE) largest = max_of_three(largest, step[g][u][0], step[g][u][1]);
             }
-        float top[2] = {s[0][0], s[0][1]};
+        float top[2];
 #pragma unroll
-        for (int u = 0; u < UNITS; ++u)
+        for (int i = 0; i < 2; ++i) {
+            top[i] = fmaxf(s[0][i], s[0][i + 2]);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) top[k & 1] = fmaxf(top[k & 1], s[u][k]);
+            for (int u = 1; u < UNITS; ++u) top[i] = max_of_three(top[i], s[u][i], s[u][i + 2]);
+        }
         if (__any_sync(0xffffffffu, fmaxf(top[0], top[1]) > LAZY || !(begun[0] && begun[1]) ||
                                         (!WIDE && largest * grown > 1024.f))) {
             float resized = 1.f;
@@ -582,6 +606,27 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
         }
     }
     __syncthreads();
+    if (splits == 1) {
+        // no key and no sink: zeros; a sum that is no number stays one
+        for (int i = threadIdx.x; i < rows * HD / 2; i += WARPS * 32) {
+            const int head = i / (HD / 2), d = i % (HD / 2) * 2;
+            float top = NOTHING;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) top = fmaxf(top, merge[(w * HEADS + head) * ROW + HD]);
+            float sum = 0.f, a = 0.f, b = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float* row = merge + (w * HEADS + head) * ROW;
+                const float by = fast_exp2(row[HD] - top);
+                sum = fmaf(by, row[HD + 1], sum);
+                a = fmaf(by, row[d], a);
+                b = fmaf(by, row[d + 1], b);
+            }
+            const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+            store_pair(out + ((size_t)request * heads + head0 + head) * HD + d, a * inverse, b * inverse);
+        }
+        return;
+    }
     // the block's result behind the warps' rows
     float* block_row = merge + WARPS * HEADS * ROW;
     for (int i = threadIdx.x; i < HEADS * HD; i += WARPS * 32) {
@@ -624,7 +669,6 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
             a = fmaf(by, row[d], a);
             b = fmaf(by, row[d + 1], b);
         }
-        // (no key and no sink: zeros; a sum that is no number stays one)
         const float inverse = sum == 0.f ? 0.f : 1.f / sum;
         store_pair(out + ((size_t)request * heads + head0 + head) * HD + d, a * inverse, b * inverse);
     }
@@ -682,7 +726,7 @@ int launch_packed(const void* q, const void* cache, const int* block_table, int 
     config.stream = stream;
     cudaLaunchAttribute attributes[2];
     int count = 0;
-    if (partial == nullptr) {
+    if (partial == nullptr && splits > 1) {
         attributes[count].id = cudaLaunchAttributeClusterDimension;
         attributes[count].val.clusterDim.x = splits;
         attributes[count].val.clusterDim.y = 1;
@@ -712,7 +756,7 @@ int launch_packed(const void* q, const void* cache, const int* block_table, int 
 }  // namespace
 
 // Splits that a cluster merges; more need `partial`.
-MLXONE_API int mlxone_attention_packed_cluster() { return 8; }
+MLXONE_API int mlxone_attention_packed_cluster() { return CLUSTER; }
 
 // Blocks of the kernel that an SM holds at once.
 MLXONE_API int mlxone_attention_packed_resident(int head_dim, int dtype) {
@@ -733,7 +777,7 @@ MLXONE_API int mlxone_attention_packed(const void* q, const void* cache, const i
                    "attention_packed: bad sizes");
     MLXONE_REQUIRE(page_size >= 16 && (page_size & (page_size - 1)) == 0 && pages > 0 && table_width > 0,
                    "attention_packed: pages hold a power of two of tokens, 16 or more, not %d", page_size);
-    MLXONE_REQUIRE(splits >= 1 && splits <= 65535 && (partial != nullptr || splits <= 8),
+    MLXONE_REQUIRE(splits >= 1 && splits <= 65535 && (partial != nullptr || splits <= CLUSTER),
                    "attention_packed: %d splits need scratch", splits);
     MLXONE_REQUIRE(kv_heads * (long long)ceil_div_host(heads / kv_heads, HEADS) <= 65535,
                    "attention_packed: too many heads");
