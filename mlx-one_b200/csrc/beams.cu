@@ -3,12 +3,13 @@
 // Choice. A request has B hypotheses with summed logarithms score_b; candidate (b, v) has score_b + logit_bv -
 // log sum_v exp(logit_bv), a hypothesis that has ended one candidate, itself. The B best of a request are
 // wanted, best first, ties to the lowest (b, v). Bound by reading the logits once (4 bytes a candidate):
-//   beam_parts  a block per (row, part of the vocabulary): the part's maximum and sum of exponentials by a running
-//               maximum, and its B best logits. A warp holds its best in its lanes, sorted, and looks at a
-//               vector of values only if one of them passes the worst of the B: few do after the first
-//               hundreds (about B ln(n / B) of n).
-//   beam_choice a block per request: a warp per hypothesis joins the parts (the logarithm in 64 bits), then
-//               every candidate counts those ahead of it.
+//   beam_parts  a block per (row, part of the vocabulary), the part in its registers, 4 to 32 values a thread: the
+//               sum of exponentials against the warp's maximum, and the part's B best. The B-th largest of a
+//               warp's 32 lane maxima bounds its B best from below; the few values above it go to a list in
+//               shared memory, where each counts those ahead of it. A list that runs over (ties) is made again
+//               by insertion, value after value.
+//   beam_choice a block per request: a warp per hypothesis takes the best of its parts' sorted lists B times (the
+//               logarithm in 64 bits), then every candidate counts those ahead of it.
 // Within a row logits are compared as they are, between rows sums in 64 bits: no order is lost to rounding. A
 // logit that is no number counts as minus infinity; a row whose score or sum of exponentials is not finite
 // has no continuation (minus infinity for all of them).
@@ -62,85 +63,125 @@ struct Best {
     }
 };
 
-// -0 counts as 0 and what is no number as minus infinity
-__device__ __forceinline__ float logit_of(float x) { return fmaxf(x, -INFINITY) + 0.f; }
+// what is no number counts as minus infinity
+__device__ __forceinline__ float logit_of(float x) { return fmaxf(x, -INFINITY); }
 
-// parts_out [rows, parts, 2]: maximum (of x log2 e) and sum of 2^(x log2 e - maximum); ranks_out [rows, parts, beams]
+constexpr int LISTED = 1536;           // candidates of a block's list (32 hypotheses leave about 900)
+constexpr int MOST_PARTS = 256;
+
+// parts_out [rows, parts, 2]: maximum (of x log2 e) and sum of 2^(x log2 e - maximum); ranks_out [rows, parts, beams].
+// A part is 1,024 V values: V vectors of four a thread.
+template <int V>
 __global__ void __launch_bounds__(WARPS * 32)
-beam_parts_kernel(const float* logits, long long stride, int vocab, int beams, int part_size,
-                  const float* scores, const unsigned char* ended,
-                  float* parts_out, unsigned long long* ranks_out) {
-    __shared__ unsigned long long lists[WARPS][MAX_BEAMS];
+beam_parts_kernel(const float* logits, long long stride, int vocab, int beams, const float* scores,
+                  const unsigned char* ended, float* parts_out, unsigned long long* ranks_out) {
+    __shared__ unsigned long long list[LISTED];
     __shared__ float tops[WARPS], sums[WARPS];
+    __shared__ int listed;
     griddep_launch();
     griddep_wait();
     const int row = blockIdx.y, part = blockIdx.x, parts = gridDim.x;
     if ((ended != nullptr && ended[row]) || !isfinite(scores[row])) return;     // nothing of the row is wanted
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float* x = logits + (size_t)row * stride;
-    const int begin = part * part_size, end = min(begin + part_size, vocab);
-    Best best;
-    float top = NOTHING, sum = 0.f;
-    auto take = [&](const float (&v)[4], int place, int live) {
-        const float most = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
-        const float scaled = most * LOG2E;
-        if (scaled > top) {
-            sum *= fast_exp2(top - scaled);
-            top = scaled;
-        }
+    const int begin = part * (V * 1024), end = min(begin + V * 1024, vocab);
+    const int first = begin + (int)threadIdx.x * 4;              // of vector v: first + 1024 v
+    float value[V][4];
+    if (((size_t)x & 15) == 0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += fast_exp2(fmaf(v[i], LOG2E, -top));
-        // (equal to the worst still counts here: its place decides)
-        if (__any_sync(0xffffffffu, live > 0 && ranked(most, 0) > best.worst)) {
+        for (int v = 0; v < V; ++v) {
+            const int place = first + v * 1024;
+            if (place + 4 <= end) {
+                const float4 four = __ldcs(reinterpret_cast<const float4*>(x + place));
+                value[v][0] = four.x; value[v][1] = four.y; value[v][2] = four.z; value[v][3] = four.w;
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) best.offer(i < live ? ranked(v[i], place + i) : 0, beams, lane);
-        }
-    };
-    const bool wide = ((size_t)x & 15) == 0 && (begin & 3) == 0;
-    if (wide) {
-        // four vectors a lane at a time, all asked for before the first is looked at
-        constexpr int AHEAD = 4;
-        for (int at = begin + warp * AHEAD * 128; at < end; at += WARPS * AHEAD * 128) {
-            float v[AHEAD][4];
-#pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                const int place = at + a * 128 + lane * 4;
-                if (place + 4 <= end) {
-                    const float4 four = __ldcs(reinterpret_cast<const float4*>(x + place));
-                    v[a][0] = four.x; v[a][1] = four.y; v[a][2] = four.z; v[a][3] = four.w;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[a][i] = place + i < end ? x[place + i] : -INFINITY;
-                }
-            }
-#pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                const int place = at + a * 128 + lane * 4;
-                if (at + a * 128 >= end) break;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[a][i] = logit_of(v[a][i]);
-                take(v[a], place, min(max(end - place, 0), 4));
+                for (int i = 0; i < 4; ++i) value[v][i] = place + i < end ? x[place + i] : -INFINITY;
             }
         }
     } else {
-        for (int at = begin + warp * 32; at < end; at += WARPS * 32) {
-            const int place = at + lane;
-            float v[4] = {place < end ? logit_of(x[place]) : -INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            take(v, place, place < end ? 1 : 0);
-        }
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int place = first + v * 1024 + i;
+                value[v][i] = place < end ? x[place] : -INFINITY;
+            }
     }
-    // lanes, then warps
-    const float warp_top = warp_max(top);
-    sum = warp_sum(sum * fast_exp2(top - warp_top));
+    if (threadIdx.x == 0) listed = 0;
+    float most = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            value[v][i] = logit_of(value[v][i]);
+            most = fmaxf(most, value[v][i]);
+        }
+    // the maximum of the warp, and the B-th largest of its lanes' maxima: no lane's value below that is wanted
+    const uint32_t order = (uint32_t)(ranked(most, 0) >> 32);
+    uint32_t left = order, bound = 0, top_order = 0;
+    for (int k = 0; k < beams; ++k) {
+        bound = __reduce_max_sync(0xffffffffu, left);
+        if (k == 0) top_order = bound;
+        // (one lane of those that have it leaves)
+        const unsigned have = __ballot_sync(0xffffffffu, left == bound);
+        if (lane == __ffs(have) - 1) left = 0;
+    }
+    const float top = fmaxf(value_of((unsigned long long)top_order << 32) * LOG2E, NOTHING);
+    const float least = value_of((unsigned long long)bound << 32);
+    float sum = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += fast_exp2(fmaf(value[v][i], LOG2E, -top));
+    sum = warp_sum(sum);
     if (lane == 0) {
-        tops[warp] = warp_top;
+        tops[warp] = top;
         sums[warp] = sum;
     }
-    lists[warp][lane] = best.mine;
     __syncthreads();
+    if (most >= least) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int place = first + v * 1024 + i;
+                if (value[v][i] >= least && place < end) {
+                    const int at = atomicAdd(&listed, 1);
+                    if (at < LISTED) list[at] = ranked(value[v][i] + 0.f, place);      // (-0 is 0)
+                }
+            }
+    }
+    __syncthreads();
+    const int count = listed;
+    unsigned long long* out = ranks_out + ((size_t)row * parts + part) * beams;
+    if (count <= LISTED) {
+        // (at least B unless the part is shorter; all different, so every rank has one owner)
+        for (int i = threadIdx.x; i < count; i += WARPS * 32) {
+            const unsigned long long mine = list[i];
+            int ahead = 0;
+            for (int k = 0; k < count; ++k) ahead += list[k] > mine;
+            if (ahead < beams) out[ahead] = mine;
+        }
+        if ((int)threadIdx.x >= count && (int)threadIdx.x < beams) out[threadIdx.x] = 0;
+    } else {
+        Best best;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int place = first + v * 1024 + i;
+                best.offer(place < end ? ranked(value[v][i] + 0.f, place) : 0, beams, lane);
+            }
+        __syncthreads();                                         // (the list's room is the warps' now)
+        list[warp * MAX_BEAMS + lane] = best.mine;
+        __syncthreads();
+        if (warp == 0) {
+            for (int w = 1; w < WARPS; ++w) best.offer(lane < beams ? list[w * MAX_BEAMS + lane] : 0, beams, lane);
+            if (lane < beams) out[lane] = best.mine;
+        }
+    }
     if (warp == 0) {
-        for (int w = 1; w < WARPS; ++w) best.offer(lane < beams ? lists[w][lane] : 0, beams, lane);
-        if (lane < beams) ranks_out[((size_t)row * parts + part) * beams + lane] = best.mine;
         const float all = warp_max(lane < WARPS ? tops[lane] : NOTHING);
         const float total = warp_sum(lane < WARPS ? sums[lane] * fast_exp2(tops[lane] - all) : 0.f);
         if (lane == 0) {
@@ -176,7 +217,7 @@ beam_choice_kernel(const float* parts_in, const unsigned long long* ranks_in, in
         }
     } else {
         double whole = (double)NAN;                        // the logarithm of the row's sum, times log2 e
-        Best best;
+        unsigned long long best = 0;
         if (isfinite(score)) {
             float top = NOTHING;
             for (int i = lane; i < parts; i += 32) top = fmaxf(top, part_sums[((size_t)row * parts + i) * 2]);
@@ -188,15 +229,40 @@ beam_choice_kernel(const float* parts_in, const unsigned long long* ranks_in, in
             }
             sum = warp_sum(sum);
             whole = (double)top + log2((double)sum);
+            // the parts' lists are sorted: a lane looks after every 32nd part's, its first and the one after
             const unsigned long long* at = part_ranks + (size_t)row * parts * beams;
-            for (int i = 0; i < parts * beams; i += 32)
-                best.offer(i + lane < parts * beams ? at[i + lane] : 0, beams, lane);
+            constexpr int MINE = MOST_PARTS / 32;
+            unsigned long long head[MINE], next[MINE];
+            int taken[MINE];
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) {
+                const bool there = lane + 32 * i < parts;
+                head[i] = there ? at[(size_t)(lane + 32 * i) * beams] : 0;
+                next[i] = there && beams > 1 ? at[(size_t)(lane + 32 * i) * beams + 1] : 0;
+                taken[i] = 2;
+            }
+            for (int k = 0; k < beams; ++k) {
+                unsigned long long mine = head[0];
+#pragma unroll
+                for (int i = 1; i < MINE; ++i) mine = head[i] > mine ? head[i] : mine;
+                const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(mine >> 32));
+                const uint32_t low = __reduce_max_sync(0xffffffffu, (uint32_t)(mine >> 32) == high ? (uint32_t)mine : 0u);
+                const unsigned long long found = (unsigned long long)high << 32 | low;
+                if (lane == k) best = found;
+#pragma unroll
+                for (int i = 0; i < MINE; ++i)
+                    if (head[i] == found && found != 0) {
+                        head[i] = next[i];
+                        next[i] = taken[i] < beams ? at[(size_t)(lane + 32 * i) * beams + taken[i]] : 0;
+                        ++taken[i];
+                    }
+            }
         }
         if (lane < beams) {
             value = minus;
             if (isfinite(whole)) {
-                const float logit = value_of(best.mine);
-                token = place_of(best.mine);
+                const float logit = value_of(best);
+                token = place_of(best);
                 value = (double)score + ((double)logit - whole * 0.6931471805599453094);
             }
         }
@@ -306,12 +372,18 @@ reorder_pages_kernel(unsigned char* storage, long long pages, long long bytes, c
 
 }  // namespace
 
+// Vectors of four that a thread takes: as many as leave two blocks an SM and more.
+static int beam_vectors(int rows, int vocab) {
+    int v = 8;
+    while (v > 1 && (long long)rows * ceil_div_host(vocab, 1024 * v) < 2 * 148) v >>= 1;
+    while (v < 8 && ceil_div_host(vocab, 1024 * v) > 64) v <<= 1;
+    return v;
+}
+
 // Scratch of mlxone_beam_select: into how many parts a row's vocabulary is cut.
 MLXONE_API int mlxone_beam_parts(int rows, int vocab) {
     if (rows <= 0 || vocab <= 0) return 1;
-    const int wanted = ceil_div_host(148 * 4, rows), most = ceil_div_host(vocab, 1024);
-    const int parts = wanted < most ? wanted : most;
-    return parts < 1 ? 1 : parts > 64 ? 64 : parts;
+    return ceil_div_host(vocab, 1024 * beam_vectors(rows, vocab));
 }
 
 // logits float32 [requests * beams, vocab], rows `stride` values apart; scores float32 [requests, beams]; ended bytes
@@ -327,11 +399,19 @@ MLXONE_API int mlxone_beam_select(const float* logits, long long stride, int req
                    MAX_BEAMS, beams);
     MLXONE_REQUIRE(vocab >= beams, "beam_select: %d tokens are fewer than %d hypotheses", vocab, beams);
     MLXONE_REQUIRE((long long)requests * beams <= 65535, "beam_select: too many rows");
-    MLXONE_REQUIRE(parts >= 1 && parts <= 64 && end_count >= 0 && (ended == nullptr || end_count > 0),
-                   "beam_select: bad sizes");
-    const int part_size = ceil_div_host(ceil_div_host(vocab, parts), 4) * 4;
-    launch_kernel(beam_parts_kernel, dim3(parts, requests * beams), dim3(WARPS * 32), 0, stream, true, logits, stride,
-                  vocab, beams, part_size, scores, ended, partial, ranks);
+    MLXONE_REQUIRE(parts == mlxone_beam_parts(requests * beams, vocab) && end_count >= 0 &&
+                       (ended == nullptr || end_count > 0), "beam_select: bad sizes");
+    MLXONE_REQUIRE(parts <= MOST_PARTS, "beam_select: a vocabulary of %d tokens is too large", vocab);
+#define CALL(V)                                                                                               \
+    launch_kernel(beam_parts_kernel<V>, dim3(parts, requests * beams), dim3(WARPS * 32), 0, stream, true,     \
+                  logits, stride, vocab, beams, scores, ended, partial, ranks)
+    switch (beam_vectors(requests * beams, vocab)) {
+        case 1: CALL(1); break;
+        case 2: CALL(2); break;
+        case 4: CALL(4); break;
+        default: CALL(8); break;
+    }
+#undef CALL
     MLXONE_LAUNCH_CHECK("beam_parts");
     launch_kernel(beam_choice_kernel, dim3(requests), dim3(beams * 32), 0, stream, true, (const float*)partial,
                   (const unsigned long long*)ranks, parts, beams, scores, ended, ends, end_count, scores_out,
