@@ -3,13 +3,14 @@
 // Choice. A request has B hypotheses with summed logarithms score_b; candidate (b, v) has score_b + logit_bv -
 // log sum_v exp(logit_bv), a hypothesis that has ended one candidate, itself. The B best of a request are
 // wanted, best first, ties to the lowest (b, v). Bound by reading the logits once (4 bytes a candidate):
-//   beam_parts  a block per (row, part of the vocabulary), the part in its registers, 4 to 32 values a thread: the
-//               sum of exponentials against the warp's maximum, and the part's B best. The B-th largest of a
-//               warp's 32 lane maxima bounds its B best from below; the few values above it go to a list in
-//               shared memory, where each counts those ahead of it. A list that runs over (ties) is made again
-//               by insertion, value after value.
-//   beam_choice a block per request: a warp per hypothesis takes the best of its parts' sorted lists B times (the
-//               logarithm in 64 bits), then every candidate counts those ahead of it.
+//   beam_sums   reads them: a thread takes 32 (eight vectors, all asked for at once) and leaves their maximum, a block
+//               of 8,192 the sum of their exponentials. About 5 instructions a value, no exchange but at the end.
+//   beam_choice a block per row. With the ceil(B / 8) largest of what each of its 8 warps sees of the row's thread
+//               maxima the B-th largest of those bounds the B best from below (B threads have a value of that
+//               size at least), so only the values of the few threads whose maximum reaches it are read again;
+//               those that reach it are ordered by counting who is ahead. Where ties make them many, the row is
+//               walked value by value instead. The last block of a request to arrive (a counter in the call's own
+//               scratch, set to zero by the kernel before) orders its rows' candidates in the same way.
 // Within a row logits are compared as they are, between rows sums in 64 bits: no order is lost to rounding. A
 // logit that is no number counts as minus infinity; a row whose score or sum of exponentials is not finite
 // has no continuation (minus infinity for all of them).
@@ -66,225 +67,257 @@ struct Best {
 // what is no number counts as minus infinity
 __device__ __forceinline__ float logit_of(float x) { return fmaxf(x, -INFINITY); }
 
-constexpr int LISTED = 1536;           // candidates of a block's list (32 hypotheses leave about 900)
-constexpr int MOST_PARTS = 256;
+constexpr int PART = 8192;             // logits of a block, 32 a thread
+constexpr int CHOSEN = 256, LISTED = 512;       // of a row: threads and values that reach the bound
 
-// parts_out [rows, parts, 2]: maximum (of x log2 e) and sum of 2^(x log2 e - maximum); ranks_out [rows, parts, beams].
-// A part is 1,024 V values: V vectors of four a thread.
-template <int V>
+// Where value e (0..31) of thread t of a row lies.
+__device__ __forceinline__ int place_in_row(int t, int e) {
+    return (t >> 8) * PART + (e >> 2) * 1024 + (t & 255) * 4 + (e & 3);
+}
+
+// maxima [rows, parts * 256]; sums [rows, parts, 2]: maximum (of x log2 e) and sum of 2^(x log2 e - maximum).
 __global__ void __launch_bounds__(WARPS * 32)
-beam_parts_kernel(const float* logits, long long stride, int vocab, int beams, const float* scores,
-                  const unsigned char* ended, float* parts_out, unsigned long long* ranks_out) {
-    __shared__ unsigned long long list[LISTED];
+beam_sums_kernel(const float* logits, long long stride, int vocab, int beams, const float* scores,
+                 const unsigned char* ended, float* maxima, float* sums_out, int* arrived) {
     __shared__ float tops[WARPS], sums[WARPS];
-    __shared__ int listed;
     griddep_launch();
     griddep_wait();
     const int row = blockIdx.y, part = blockIdx.x, parts = gridDim.x;
+    if (part == 0 && row % beams == 0 && threadIdx.x == 0) arrived[row / beams] = 0;
     if ((ended != nullptr && ended[row]) || !isfinite(scores[row])) return;     // nothing of the row is wanted
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const float* x = logits + (size_t)row * stride;
-    const int begin = part * (V * 1024), end = min(begin + V * 1024, vocab);
-    const int first = begin + (int)threadIdx.x * 4;              // of vector v: first + 1024 v
-    float value[V][4];
-    if (((size_t)x & 15) == 0) {
+    const float* x = logits + (size_t)row * stride + (size_t)part * PART;
+    const int left = vocab - part * PART, first = (int)threadIdx.x * 4;
+    float value[8][4];
+    if (left >= PART && ((size_t)x & 15) == 0) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int place = first + v * 1024;
-            if (place + 4 <= end) {
-                const float4 four = __ldcs(reinterpret_cast<const float4*>(x + place));
-                value[v][0] = four.x; value[v][1] = four.y; value[v][2] = four.z; value[v][3] = four.w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) value[v][i] = place + i < end ? x[place + i] : -INFINITY;
-            }
+        for (int v = 0; v < 8; ++v) {
+            const float4 four = __ldcs(reinterpret_cast<const float4*>(x + first + v * 1024));
+            value[v][0] = four.x; value[v][1] = four.y; value[v][2] = four.z; value[v][3] = four.w;
         }
     } else {
 #pragma unroll
-        for (int v = 0; v < V; ++v)
+        for (int v = 0; v < 8; ++v)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int place = first + v * 1024 + i;
-                value[v][i] = place < end ? x[place] : -INFINITY;
+                value[v][i] = place < left ? x[place] : -INFINITY;
             }
     }
-    if (threadIdx.x == 0) listed = 0;
     float most = -INFINITY;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
+    for (int v = 0; v < 8; ++v)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             value[v][i] = logit_of(value[v][i]);
             most = fmaxf(most, value[v][i]);
         }
-    // the maximum of the warp, and the B-th largest of its lanes' maxima: no lane's value below that is wanted
-    const uint32_t order = (uint32_t)(ranked(most, 0) >> 32);
-    uint32_t left = order, bound = 0, top_order = 0;
-    for (int k = 0; k < beams; ++k) {
-        bound = __reduce_max_sync(0xffffffffu, left);
-        if (k == 0) top_order = bound;
-        // (one lane of those that have it leaves)
-        const unsigned have = __ballot_sync(0xffffffffu, left == bound);
-        if (lane == __ffs(have) - 1) left = 0;
-    }
-    const float top = fmaxf(value_of((unsigned long long)top_order << 32) * LOG2E, NOTHING);
-    const float least = value_of((unsigned long long)bound << 32);
-    float sum = 0.f;
+    const float top = fmaxf(most * LOG2E, NOTHING);
+    float sum[2] = {0.f, 0.f};
 #pragma unroll
-    for (int v = 0; v < V; ++v)
+    for (int v = 0; v < 8; ++v)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += fast_exp2(fmaf(value[v][i], LOG2E, -top));
-    sum = warp_sum(sum);
+        for (int i = 0; i < 4; ++i) sum[i & 1] += fast_exp2(fmaf(value[v][i], LOG2E, -top));
+    maxima[((size_t)row * parts + part) * (WARPS * 32) + threadIdx.x] = most;
+    const float warp_top = warp_max(top);
+    const float warp_sum_ = warp_sum((sum[0] + sum[1]) * fast_exp2(top - warp_top));
     if (lane == 0) {
-        tops[warp] = top;
-        sums[warp] = sum;
+        tops[warp] = warp_top;
+        sums[warp] = warp_sum_;
     }
     __syncthreads();
-    if (most >= least) {
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int place = first + v * 1024 + i;
-                if (value[v][i] >= least && place < end) {
-                    const int at = atomicAdd(&listed, 1);
-                    if (at < LISTED) list[at] = ranked(value[v][i] + 0.f, place);      // (-0 is 0)
-                }
-            }
-    }
-    __syncthreads();
-    const int count = listed;
-    unsigned long long* out = ranks_out + ((size_t)row * parts + part) * beams;
-    if (count <= LISTED) {
-        // (at least B unless the part is shorter; all different, so every rank has one owner)
-        for (int i = threadIdx.x; i < count; i += WARPS * 32) {
-            const unsigned long long mine = list[i];
-            int ahead = 0;
-            for (int k = 0; k < count; ++k) ahead += list[k] > mine;
-            if (ahead < beams) out[ahead] = mine;
-        }
-        if ((int)threadIdx.x >= count && (int)threadIdx.x < beams) out[threadIdx.x] = 0;
-    } else {
-        Best best;
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int place = first + v * 1024 + i;
-                best.offer(place < end ? ranked(value[v][i] + 0.f, place) : 0, beams, lane);
-            }
-        __syncthreads();                                         // (the list's room is the warps' now)
-        list[warp * MAX_BEAMS + lane] = best.mine;
-        __syncthreads();
-        if (warp == 0) {
-            for (int w = 1; w < WARPS; ++w) best.offer(lane < beams ? list[w * MAX_BEAMS + lane] : 0, beams, lane);
-            if (lane < beams) out[lane] = best.mine;
-        }
-    }
     if (warp == 0) {
         const float all = warp_max(lane < WARPS ? tops[lane] : NOTHING);
         const float total = warp_sum(lane < WARPS ? sums[lane] * fast_exp2(tops[lane] - all) : 0.f);
         if (lane == 0) {
-            parts_out[((size_t)row * parts + part) * 2] = all;
-            parts_out[((size_t)row * parts + part) * 2 + 1] = total;
+            sums_out[((size_t)row * parts + part) * 2] = all;
+            sums_out[((size_t)row * parts + part) * 2 + 1] = total;
         }
     }
 }
 
-__global__ void __launch_bounds__(MAX_BEAMS * 32)
-beam_choice_kernel(const float* parts_in, const unsigned long long* ranks_in, int parts,
-                   int beams, const float* scores, const unsigned char* ended,
-                   const int* ends, int end_count, float* scores_out,
-                   int* parents_out, int* tokens_out,
-                   unsigned char* ended_out) {
-    __shared__ double values[MAX_BEAMS * MAX_BEAMS];       // (a NaN: no candidate)
-    __shared__ int tokens[MAX_BEAMS * MAX_BEAMS];
+// A number that orders as the value does; 0 for none.
+__device__ __forceinline__ unsigned long long ordered(double value) {
+    const unsigned long long bits = (unsigned long long)__double_as_longlong(value + 0.0);
+    return bits >> 63 ? ~bits : bits | 1ull << 63;
+}
+__device__ __forceinline__ double of_order(unsigned long long order) {
+    return __longlong_as_double((long long)(order >> 63 ? order & ~(1ull << 63) : ~order));
+}
+
+// keys, tokens [rows, beams]: the rows' candidates, best first, as the last block of a request finds them.
+__global__ void __launch_bounds__(WARPS * 32)
+beam_choice_kernel(const float* logits, long long stride, int vocab, const float* maxima_in, const float* sums_in,
+                   int parts, int beams, const float* scores, const unsigned char* ended, const int* ends,
+                   int end_count, unsigned long long* keys, int* tokens, int* arrived, float* scores_out,
+                   int* parents_out, int* tokens_out, unsigned char* ended_out) {
+    __shared__ unsigned long long list[LISTED];
+    __shared__ unsigned long long sorted[MAX_BEAMS];
+    __shared__ int chosen[CHOSEN];
+    __shared__ uint32_t bounds[MAX_BEAMS];                       // as ranked() orders
+    __shared__ double whole_of_row;
+    __shared__ int chosen_count, listed, is_last;
     griddep_launch();
     griddep_wait();
-    const float* part_sums = settled(parts_in);
-    const unsigned long long* part_ranks = settled(ranks_in);
-    const int request = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = request * beams + warp;
+    const int row = blockIdx.x, request = row / beams;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float score = scores[row];
     const bool over = ended != nullptr && ended[row];
     const double minus = -(double)INFINITY;
-    double value = (double)NAN;
-    int token = lane;
+    unsigned long long key = 0;                                  // thread k < beams: the row's k-th candidate
+    int token = threadIdx.x;
     if (over) {
-        if (lane == 0) {
-            value = isnan(score) ? minus : (double)score;
+        if (threadIdx.x == 0) {
+            key = ordered(isnan(score) ? minus : (double)score);
             token = ends[0];
         }
+    } else if (!isfinite(score)) {
+        if ((int)threadIdx.x < beams) key = ordered(minus);
     } else {
-        double whole = (double)NAN;                        // the logarithm of the row's sum, times log2 e
-        unsigned long long best = 0;
-        if (isfinite(score)) {
-            float top = NOTHING;
-            for (int i = lane; i < parts; i += 32) top = fmaxf(top, part_sums[((size_t)row * parts + i) * 2]);
+        const float* x = logits + (size_t)row * stride;
+        const float* maxima = settled(maxima_in) + (size_t)row * parts * (WARPS * 32);
+        const int threads = parts * WARPS * 32;
+        float most = -INFINITY;
+#pragma unroll 4
+        for (int i = threadIdx.x * 4; i < threads; i += WARPS * 128) {
+            const float4 four = *reinterpret_cast<const float4*>(maxima + i);
+            most = fmaxf(fmaxf(most, fmaxf(four.x, four.y)), fmaxf(four.z, four.w));
+        }
+        if (threadIdx.x == 0) chosen_count = listed = 0;
+        if (warp == WARPS - 1) {
+            // the logarithm of the row's sum, times log2 e
+            const float* part_sums = settled(sums_in) + (size_t)row * parts * 2;
+            float top = NOTHING, sum = 0.f;
+            for (int i = lane; i < parts; i += 32) top = fmaxf(top, part_sums[i * 2]);
             top = warp_max(top);
-            float sum = 0.f;
-            for (int i = lane; i < parts; i += 32) {
-                const float* at = part_sums + ((size_t)row * parts + i) * 2;
-                sum += at[1] * fast_exp2(at[0] - top);
-            }
+            for (int i = lane; i < parts; i += 32) sum += part_sums[i * 2 + 1] * fast_exp2(part_sums[i * 2] - top);
             sum = warp_sum(sum);
-            whole = (double)top + log2((double)sum);
-            // the parts' lists are sorted: a lane looks after every 32nd part's, its first and the one after
-            const unsigned long long* at = part_ranks + (size_t)row * parts * beams;
-            constexpr int MINE = MOST_PARTS / 32;
-            unsigned long long head[MINE], next[MINE];
-            int taken[MINE];
+            // (the logarithm of what is left of the sum without its power of two, in 0..1, is off by 2^-24)
+            int power = 0;
+            const float rest = frexpf(sum, &power);
+            if (lane == 0)
+                whole_of_row = sum > 0.f ? (double)top + (double)(power - 1) + (double)log2f(2.f * rest) : (double)NAN;
+        }
+        // the largest maxima that each warp sees, and what they bound
+        const int each = (beams + WARPS - 1) / WARPS, offered = each * WARPS;
+        uint32_t left = (uint32_t)(ranked(most + 0.f, 0) >> 32);              // (-0 is 0)
+        for (int k = 0; k < each; ++k) {
+            const uint32_t largest = __reduce_max_sync(0xffffffffu, left);
+            if (lane == 0) bounds[warp * each + k] = largest;
+            // (one lane of those that have it leaves)
+            const unsigned have = __ballot_sync(0xffffffffu, left == largest);
+            if (lane == __ffs((int)have) - 1) left = 0;
+        }
+        __syncthreads();
+        const double whole = whole_of_row;
+        const uint32_t mine = lane < offered ? bounds[lane] : 0u;
+        int ahead = 0;
+        for (int k = 0; k < offered; ++k) ahead += bounds[k] > mine || (bounds[k] == mine && k < lane);
+        const unsigned last = __ballot_sync(0xffffffffu, lane < offered && ahead == beams - 1);
+        const float least = value_of((unsigned long long)__shfl_sync(0xffffffffu, mine, __ffs((int)last) - 1) << 32);
+        if (most >= least) {
+            for (int i = threadIdx.x * 4; i < threads; i += WARPS * 128) {
+                const float4 four = *reinterpret_cast<const float4*>(maxima + i);
+                const float of[4] = {four.x, four.y, four.z, four.w};
 #pragma unroll
-            for (int i = 0; i < MINE; ++i) {
-                const bool there = lane + 32 * i < parts;
-                head[i] = there ? at[(size_t)(lane + 32 * i) * beams] : 0;
-                next[i] = there && beams > 1 ? at[(size_t)(lane + 32 * i) * beams + 1] : 0;
-                taken[i] = 2;
-            }
-            for (int k = 0; k < beams; ++k) {
-                unsigned long long mine = head[0];
-#pragma unroll
-                for (int i = 1; i < MINE; ++i) mine = head[i] > mine ? head[i] : mine;
-                const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(mine >> 32));
-                const uint32_t low = __reduce_max_sync(0xffffffffu, (uint32_t)(mine >> 32) == high ? (uint32_t)mine : 0u);
-                const unsigned long long found = (unsigned long long)high << 32 | low;
-                if (lane == k) best = found;
-#pragma unroll
-                for (int i = 0; i < MINE; ++i)
-                    if (head[i] == found && found != 0) {
-                        head[i] = next[i];
-                        next[i] = taken[i] < beams ? at[(size_t)(lane + 32 * i) * beams + taken[i]] : 0;
-                        ++taken[i];
+                for (int k = 0; k < 4; ++k)
+                    if (of[k] >= least) {
+                        const int at = atomicAdd(&chosen_count, 1);
+                        if (at < CHOSEN) chosen[at] = i + k;
                     }
             }
         }
-        if (lane < beams) {
-            value = minus;
+        __syncthreads();
+        const int chosen_here = chosen_count;
+        bool few = chosen_here <= CHOSEN;
+        if (few) {
+            // (a warp a thread's values, a lane a value)
+#pragma unroll 4
+            for (int i = warp; i < chosen_here; i += WARPS) {
+                const int place = place_in_row(chosen[i], lane);
+                const float logit = place < vocab ? logit_of(x[place]) : -INFINITY;
+                if (place < vocab && logit >= least) {
+                    const int at = atomicAdd(&listed, 1);
+                    if (at < LISTED) list[at] = ranked(logit + 0.f, place);
+                }
+            }
+            __syncthreads();
+            few = listed <= LISTED;
+        }
+        if (few) {
+            // (all different, so every rank has one owner; at least B of them)
+            const int count = listed;
+            for (int i = threadIdx.x; i < count; i += WARPS * 32) {
+                const unsigned long long rank = list[i];
+                int better = 0;
+#pragma unroll 8
+                for (int k = 0; k < count; ++k) better += list[k] > rank;
+                if (better < beams) sorted[better] = rank;
+            }
+        } else {
+            // ties, or hardly a logit above minus infinity: eight sorted lists, then one
+            __syncthreads();
+            Best best;
+            for (int from = 0; from < vocab; from += WARPS * 32) {
+                const int place = from + threadIdx.x;
+                best.offer(place < vocab ? ranked(logit_of(x[place]) + 0.f, place) : 0, beams, lane);
+            }
+            list[warp * MAX_BEAMS + lane] = best.mine;
+            __syncthreads();
+            if (warp == 0) {
+                for (int w = 1; w < WARPS; ++w) best.offer(lane < beams ? list[w * MAX_BEAMS + lane] : 0, beams, lane);
+                if (lane < beams) sorted[lane] = best.mine;
+            }
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < beams) {
+            key = ordered(minus);
             if (isfinite(whole)) {
-                const float logit = value_of(best);
+                const unsigned long long best = sorted[threadIdx.x];
                 token = place_of(best);
-                value = (double)score + ((double)logit - whole * 0.6931471805599453094);
+                key = ordered((double)score + ((double)value_of(best) - whole * 0.6931471805599453094));
             }
         }
     }
-    if (lane < beams) {
-        values[warp * beams + lane] = value;
-        tokens[warp * beams + lane] = token;
+    if ((int)threadIdx.x < beams) {
+        keys[(size_t)row * beams + threadIdx.x] = key;
+        tokens[(size_t)row * beams + threadIdx.x] = token;
+        __threadfence();
     }
     __syncthreads();
-    // (a hypothesis' candidates are sorted, so the order of the array is the order of ties)
-    for (int i = threadIdx.x; i < beams * beams; i += blockDim.x) {
-        const double mine = values[i];
-        if (isnan(mine)) continue;
-        int ahead = 0;
-        for (int k = 0; k < beams * beams; ++k) ahead += values[k] > mine || (values[k] == mine && k < i);
+    if (threadIdx.x == 0) is_last = atomicAdd(arrived + request, 1) == beams - 1;
+    __syncthreads();
+    if (!is_last) return;
+    __threadfence();
+    // (a row's candidates are sorted, so the order of the array is the order of ties)
+    const int among = beams * beams, held = request * beams;
+    const unsigned long long* all = settled(keys) + (size_t)held * beams;
+    for (int i = threadIdx.x; i < among && i < LISTED; i += WARPS * 32) list[i] = __ldcg(all + i);
+    // (thread i's first candidate's token and whether its hypothesis had ended, asked for beside the list)
+    int taken = (int)threadIdx.x < among ? __ldcg(tokens + (size_t)held * beams + threadIdx.x) : 0;
+    bool stops = ended != nullptr && (int)threadIdx.x < among && ended[held + threadIdx.x / beams];
+    const int first_end = end_count > 0 ? ends[0] : -1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < among; i += WARPS * 32) {
+        const unsigned long long own = i < LISTED ? list[i] : __ldcg(all + i);
+        int ahead = own == 0 ? beams : 0;
+#pragma unroll 8
+        for (int k = 0; k < min(among, LISTED); ++k) ahead += list[k] > own || (list[k] == own && k < i);
+        for (int k = LISTED; k < among; ++k) {
+            const unsigned long long other = __ldcg(all + k);
+            ahead += other > own || (other == own && k < i);
+        }
         if (ahead >= beams) continue;
-        const int at = request * beams + ahead, parent = i / beams, chosen = tokens[i];
-        bool stops = ended != nullptr && ended[request * beams + parent];
-        for (int k = 0; k < end_count; ++k) stops = stops || chosen == ends[k];
-        scores_out[at] = (float)mine;
+        const int at = held + ahead, parent = i / beams;
+        if (i >= WARPS * 32) {
+            taken = __ldcg(tokens + (size_t)held * beams + i);
+            stops = ended != nullptr && ended[held + parent];
+        }
+        stops = stops || (end_count > 0 && taken == first_end);
+        for (int k = 1; k < end_count; ++k) stops = stops || taken == ends[k];
+        scores_out[at] = (float)of_order(own);
         parents_out[at] = parent;
-        tokens_out[at] = chosen;
+        tokens_out[at] = taken;
         ended_out[at] = stops ? 1 : 0;
     }
 }
@@ -372,50 +405,41 @@ reorder_pages_kernel(unsigned char* storage, long long pages, long long bytes, c
 
 }  // namespace
 
-// Vectors of four that a thread takes: as many as leave two blocks an SM and more.
-static int beam_vectors(int rows, int vocab) {
-    int v = 8;
-    while (v > 1 && (long long)rows * ceil_div_host(vocab, 1024 * v) < 2 * 148) v >>= 1;
-    while (v < 8 && ceil_div_host(vocab, 1024 * v) > 64) v <<= 1;
-    return v;
-}
+static int beam_part_count(int vocab) { return ceil_div_host(vocab, PART); }
 
-// Scratch of mlxone_beam_select: into how many parts a row's vocabulary is cut.
-MLXONE_API int mlxone_beam_parts(int rows, int vocab) {
-    if (rows <= 0 || vocab <= 0) return 1;
-    return ceil_div_host(vocab, 1024 * beam_vectors(rows, vocab));
+// Bytes of scratch that mlxone_beam_select needs: thread maxima, sums, candidates, counters.
+MLXONE_API long long mlxone_beam_scratch(int requests, int beams, int vocab) {
+    if (requests <= 0 || beams <= 0 || vocab <= 0) return 0;
+    const long long rows = (long long)requests * beams;
+    return rows * beam_part_count(vocab) * (WARPS * 32 + 2) * 4 + rows * beams * 12 + requests * 4LL;
 }
 
 // logits float32 [requests * beams, vocab], rows `stride` values apart; scores float32 [requests, beams]; ended bytes
-// [requests, beams] or null; ends int32 [end_count] (at least one with `ended`). partial: requests * beams * parts * 2
-// floats; ranks: requests * beams * parts * beams 64-bit numbers.
+// [requests, beams] or null; ends int32 [end_count] (at least one with `ended`). scratch: mlxone_beam_scratch bytes
+// of this call's own, at a multiple of 16.
 MLXONE_API int mlxone_beam_select(const float* logits, long long stride, int requests, int beams, int vocab,
                                   const float* scores, const unsigned char* ended, const int* ends, int end_count,
-                                  int parts, float* partial, unsigned long long* ranks, float* scores_out,
-                                  int* parents_out, int* tokens_out, unsigned char* ended_out,
-                                  cudaStream_t stream) {
+                                  void* scratch, float* scores_out, int* parents_out, int* tokens_out,
+                                  unsigned char* ended_out, cudaStream_t stream) {
     if (requests == 0) return 0;
     MLXONE_REQUIRE(requests > 0 && beams >= 1 && beams <= MAX_BEAMS, "beam_select: 1 to %d hypotheses, not %d",
                    MAX_BEAMS, beams);
-    MLXONE_REQUIRE(vocab >= beams, "beam_select: %d tokens are fewer than %d hypotheses", vocab, beams);
+    MLXONE_REQUIRE(vocab >= beams && vocab <= 1 << 30, "beam_select: %d tokens for %d hypotheses", vocab, beams);
     MLXONE_REQUIRE((long long)requests * beams <= 65535, "beam_select: too many rows");
-    MLXONE_REQUIRE(parts == mlxone_beam_parts(requests * beams, vocab) && end_count >= 0 &&
-                       (ended == nullptr || end_count > 0), "beam_select: bad sizes");
-    MLXONE_REQUIRE(parts <= MOST_PARTS, "beam_select: a vocabulary of %d tokens is too large", vocab);
-#define CALL(V)                                                                                               \
-    launch_kernel(beam_parts_kernel<V>, dim3(parts, requests * beams), dim3(WARPS * 32), 0, stream, true,     \
-                  logits, stride, vocab, beams, scores, ended, partial, ranks)
-    switch (beam_vectors(requests * beams, vocab)) {
-        case 1: CALL(1); break;
-        case 2: CALL(2); break;
-        case 4: CALL(4); break;
-        default: CALL(8); break;
-    }
-#undef CALL
-    MLXONE_LAUNCH_CHECK("beam_parts");
-    launch_kernel(beam_choice_kernel, dim3(requests), dim3(beams * 32), 0, stream, true, (const float*)partial,
-                  (const unsigned long long*)ranks, parts, beams, scores, ended, ends, end_count, scores_out,
-                  parents_out, tokens_out, ended_out);
+    MLXONE_REQUIRE(end_count >= 0 && (ended == nullptr || end_count > 0) && ((size_t)scratch & 15) == 0,
+                   "beam_select: bad sizes");
+    const int rows = requests * beams, parts = beam_part_count(vocab);
+    float* maxima = static_cast<float*>(scratch);
+    float* sums = maxima + (size_t)rows * parts * (WARPS * 32);
+    unsigned long long* keys = reinterpret_cast<unsigned long long*>(sums + (size_t)rows * parts * 2);
+    int* tokens = reinterpret_cast<int*>(keys + (size_t)rows * beams);
+    int* arrived = tokens + (size_t)rows * beams;
+    launch_kernel(beam_sums_kernel, dim3(parts, rows), dim3(WARPS * 32), 0, stream, true, logits, stride, vocab, beams,
+                  scores, ended, maxima, sums, arrived);
+    MLXONE_LAUNCH_CHECK("beam_sums");
+    launch_kernel(beam_choice_kernel, dim3(rows), dim3(WARPS * 32), 0, stream, true, logits, stride, vocab,
+                  (const float*)maxima, (const float*)sums, parts, beams, scores, ended, ends, end_count, keys, tokens,
+                  arrived, scores_out, parents_out, tokens_out, ended_out);
     MLXONE_LAUNCH_CHECK("beam_choice");
     return 0;
 }

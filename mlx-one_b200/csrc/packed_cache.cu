@@ -3,9 +3,8 @@
 //
 // Writing. For a group of a token's values: lowest = bfloat16(min), step = bfloat16(max(max - lowest, 0) / 15,
 // difference and quotient in 32 bits), code = (x - lowest) / step to the nearest whole number, ties to
-// even, cut to 0..15. The codes are those of exact arithmetic on the stored lowest and step: the 32-bit quotient
-// decides, and where it lies within a thousandth of a tie the comparison is made in 64 bits. A group with a
-// value that is not finite, or whose range is none, gets NaN as step and lowest: it stays visible.
+// even, cut to 0..15. The codes are those of exact arithmetic on the stored lowest and step (codes_of). A group
+// with a value that is not finite, or whose range is none, gets NaN as step and lowest: it stays visible.
 #include "packed_cache.cuh"
 
 namespace {
@@ -38,16 +37,67 @@ __device__ __forceinline__ void load_eight(const T* src, bool wide, float (&x)[8
     }
 }
 
-// The code of x: (x - lowest) / step, about `ratio`, to the nearest whole number in exact arithmetic.
-__device__ __forceinline__ uint32_t code_of(float x, float lowest, float step, float ratio) {
-    float code = rintf(ratio);
-    if (fabsf(ratio - code) > 0.499f) {
-        const float below = floorf(ratio);
-        const double rest = ((double)x - (double)lowest) - ((double)below + 0.5) * (double)step;
-        const bool up = rest > 0.0 || (rest == 0.0 && ((int)fminf(fmaxf(below, -2.f), 32.f) & 1));
-        code = below + (up ? 1.f : 0.f);
+// Whether x lies above the tie between code and code + 1 (on it: whether code is odd), in exact arithmetic: the
+// difference from lowest with its own rounding (a two-term sum), and the tie, (code + 1/2) step, a number of 13
+// bits, which the difference is near enough to be taken from without rounding.
+__device__ __forceinline__ bool above_tie(float x, float lowest, float step, int code) {
+    const float above = x - lowest, back = above - x;
+    const float lost = (x - (above - back)) - (lowest + back);
+    const float rest = above - ((float)code + 0.5f) * step;
+    return rest > 0.f || (rest == 0.f && (lost > 0.f || (lost == 0.f && (code & 1))));
+}
+
+// The codes of eight values, four bits each. The quotient is the 32-bit one (a product with the inverse and one
+// correction); adding 1.5 * 2^23 rounds to a whole number, ties to even, that lies in the sum's last bits. With
+// bfloat16 values that is exact unless one is below 2^-15 of lowest: x - lowest has 24 bits, and a quotient of
+// a number of 24 bits by one of 8 either is a tie or lies 2^-18 of itself away from it. What may be decided
+// wrongly by it (32-bit values within 1e-5 of a tie) is decided again, exactly.
+template <typename T>
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float lowest, float step) {
+    const float inverse = 1.f / step;
+    constexpr float WHOLE = 12582912.f;
+    uint32_t codes = 0;
+    float furthest = 0.f, least = INFINITY;
+#pragma unroll
+    for (int i = 7; i >= 0; --i) {
+        const float above = x[i] - lowest, near = above * inverse;
+        const float ratio = fminf(fmaxf(fmaf(fmaf(-near, step, above), inverse, near), 0.f), 15.f);
+        const float raised = ratio + WHOLE;
+        furthest = fmaxf(furthest, fabsf(ratio - (raised - WHOLE)));
+        if (sizeof(T) == 2) least = fminf(least, fabsf(x[i]));
+        codes = codes * 16u + (__float_as_uint(raised) - __float_as_uint(WHOLE));
     }
-    return (uint32_t)fminf(fmaxf(code, 0.f), 15.f);
+    const bool doubtful = sizeof(T) == 4 || least < fabsf(lowest) * 3.0517578e-5f;
+    // (or a step so small that its inverse, or what the correction works with, is none)
+    if ((doubtful && !(furthest <= 0.49999f)) || !(inverse < 1e30f)) {
+        codes = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float ratio = fminf(fmaxf((x[i] - lowest) / step, 0.f), 15.f);
+            int code = (int)ratio;
+            const float past = ratio - (float)code;
+            if (fabsf(past - 0.5f) > 2e-5f) code += past > 0.5f;
+            else code += above_tie(x[i], lowest, step, code);
+            codes |= (uint32_t)min(code, 15) << (4 * i);
+        }
+    }
+    return codes;
+}
+// the larger (smaller) of two and NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float c;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+    return c;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float c;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+    return c;
+}
+// four neighbouring codes (16 bits) to a byte each
+__device__ __forceinline__ uint32_t spread(uint32_t four) {
+    four = (four | four << 8) & 0x00ff00ffu;
+    return (four | four << 4) & 0x0f0f0f0fu;
 }
 
 // One block: the runs of tokens that begin among 16 tokens of the step and share a unit (a run ends with its
@@ -61,7 +111,7 @@ __global__ void __launch_bounds__(256)
 pack_kernel(const T* keys, long long key_stride, const T* values,
             long long value_stride, int wide, const int* positions,
             const int* token_request, const int* request_start,
-            const int* block_table, int table_width, int page_size, int pages, int kv_heads,
+            const int* block_table, int table_width, int page_shift, int pages, int kv_heads,
             int tokens, unsigned char* cache, int* error_flag) {
     using P = Packed<HD>;
     constexpr int LANES = HD == 96 ? 16 : HD / 8;            // lanes of a row (four of 16 idle with 96 values)
@@ -85,20 +135,20 @@ pack_kernel(const T* keys, long long key_stride, const T* values,
         const int last = 31 - __clz((int)(starts | 1u));
         const int end = __shfl_sync(0xffffffffu, t + length, last);
         if (lane == 0) {
-            span[0] = blockIdx.x * TOKENS + (starts ? __ffs(starts) - 1 : 0);
+            span[0] = blockIdx.x * TOKENS + (starts ? __ffs((int)starts) - 1 : 0);
             span[1] = starts ? min(end, tokens) : span[0];
-            span[2] = full ? blockIdx.x * TOKENS + __ffs(full) - 1 : -1;
+            span[2] = full ? blockIdx.x * TOKENS + __ffs((int)full) - 1 : -1;
         }
     }
     __syncthreads();
     const int first = span[0], count = span[1] - span[0], whole = span[2];
-    const int units = page_size >> 4;
+    const int units = 1 << (page_shift - 4);
     auto unit_of = [&](int t) -> unsigned char* {
-        const int position = positions[t], block = position / page_size;
+        const int position = positions[t], block = position >> page_shift;
         const int page = position >= 0 && block < table_width
                              ? block_table[(size_t)token_request[t] * table_width + block] : -1;
         if (page < 0 || page >= pages) return nullptr;
-        return cache + (((size_t)page * kv_heads + head) * units + (position % page_size >> 4)) * P::UNIT;
+        return cache + (((size_t)page * kv_heads + head) * units + (position >> 4 & (units - 1))) * P::UNIT;
     };
     const int sub = threadIdx.x % LANES;                     // this thread's place in its row
     const bool live_lane = sub * 8 < HD;
@@ -117,37 +167,26 @@ pack_kernel(const T* keys, long long key_stride, const T* values,
             load_eight<T>(src, wide, x);
         }
         float least = x[0], most = x[0];
-        bool fine = true;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            least = fminf(least, x[i]);
-            most = fmaxf(most, x[i]);
-            fine = fine && isfinite(x[i]);
+        for (int i = 1; i < 8; ++i) {
+            least = min_nan(least, x[i]);
+            most = max_nan(most, x[i]);
         }
 #pragma unroll
         for (int offset = 1; offset < GROUP_LANES; offset <<= 1) {
-            least = fminf(least, __shfl_xor_sync(0xffffffffu, least, offset));
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, offset));
-            fine = __shfl_xor_sync(0xffffffffu, (int)fine, offset) && fine;
+            least = min_nan(least, __shfl_xor_sync(0xffffffffu, least, offset));
+            most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, offset));
         }
         const bf16 lowest_stored = __float2bfloat16_rn(least);
         const float lowest = __bfloat162float(lowest_stored);
         const bf16 step_stored = __float2bfloat16_rn(fmaxf(most - lowest, 0.f) / 15.f);
         const float step = __bfloat162float(step_stored);
-        fine = fine && isfinite(lowest) && isfinite(step);
-        uint32_t mine = 0;
-        if (fine && step > 0.f) {
-            // (a step so small that its inverse is none: the quotient itself)
-            const float inverse = 1.f / step;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float above = x[i] - lowest;
-                const float ratio = isfinite(inverse) ? above * inverse : above / step;
-                mine |= code_of(x[i], lowest, step, ratio) << (4 * i);
-            }
-        }
+        const bool fine = isfinite(least) && isfinite(most) && isfinite(lowest) && isfinite(step);
+        const uint32_t mine = fine && step > 0.f ? codes_of<T>(x, lowest, step) : 0u;
+        // this lane's four bytes: dimensions e and e + 8 of the run, e from 4 (sub & 1) on
         const uint32_t other = __shfl_xor_sync(0xffffffffu, mine, 1);
-        const uint32_t low = sub & 1 ? other : mine, high = sub & 1 ? mine : other;   // dimensions e, e + 8
+        const uint32_t bytes = sub & 1 ? spread(other >> 16) | spread(mine >> 16) << 4
+                                       : spread(mine & 0xffffu) | spread(other & 0xffffu) << 4;
         if (live) {
             const bool imaged = whole >= 0 && t >= whole && t < whole + 16;
             unsigned char* unit = imaged ? image : unit_of(t);
@@ -159,12 +198,14 @@ pack_kernel(const T* keys, long long key_stride, const T* values,
                 const uint32_t words = fine ? (uint32_t)__bfloat16_as_ushort(step_stored) |
                                                   (uint32_t)__bfloat16_as_ushort(lowest_stored) << 16
                                             : 0x7fc07fc0u;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int e = 4 * (sub & 1) + i;
-                    const unsigned char both = (unsigned char)((low >> (4 * e) & 15u) | (high >> (4 * e) & 15u) << 4);
-                    unit[part ? P::value_byte(key, run, e) : P::key_byte(key, run, e)] = both;
-                }
+                // bytes e = 4 (sub & 1) + 0 .. 3: neighbouring pairs of a key's lanes, or every fourth lane
+                const int half = sub & 1, lane_bytes = 4 * P::block_runs(run);
+                unsigned char* at = unit + (part ? P::value_byte(key, run, 4 * half) : P::key_byte(key, run, 4 * half));
+                const int second = part ? 4 * lane_bytes : 2, third = part ? 8 * lane_bytes : lane_bytes;
+                at[0] = (unsigned char)bytes;
+                at[second] = (unsigned char)(bytes >> 8);
+                at[third] = (unsigned char)(bytes >> 16);
+                at[third + second] = (unsigned char)(bytes >> 24);
                 if (sub % GROUP_LANES == 0)
                     *reinterpret_cast<uint32_t*>(unit + P::scale_at(key, sub / GROUP_LANES)) = words;
             }
@@ -182,18 +223,29 @@ pack_kernel(const T* keys, long long key_stride, const T* values,
     }
 }
 
-// Sixteen neighbouring values (run s of a key) from a part's codes, as one thread reads them. `first` and
-// `second`: where the byte of e = 0 lies and how far the next ones are: keys' bytes go by pairs of e.
+// Sixteen neighbouring values (run s of a key) from a part's codes, as one thread reads them.
 template <int HD>
 __device__ __forceinline__ void read_run(const unsigned char* part, int which, int key, int s, float (&x)[16]) {
     using P = Packed<HD>;
     const uint32_t word = *reinterpret_cast<const uint32_t*>(part + P::scale_at(key, s * 16 / P::GROUP));
     const float step = packed_step(word), lowest = packed_lowest(word);
+    if (which) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const uint32_t both = part[which ? P::value_byte(key, s, e) : P::key_byte(key, s, e)];
-        x[e] = fmaf(step, (float)(both & 15u), lowest);
-        x[e + 8] = fmaf(step, (float)(both >> 4), lowest);
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t both = part[P::value_byte(key, s, e)];
+            x[e] = fmaf(step, (float)(both & 15u), lowest);
+            x[e + 8] = fmaf(step, (float)(both >> 4), lowest);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            // (dimensions e and e + 1 lie in one word)
+            const uint32_t both = *reinterpret_cast<const uint32_t*>(part + (P::key_byte(key, s, e) & ~3)) >> (key & 8);
+            x[e] = fmaf(step, (float)(both & 15u), lowest);
+            x[e + 8] = fmaf(step, (float)(both >> 4 & 15u), lowest);
+            x[e + 1] = fmaf(step, (float)(both >> 16 & 15u), lowest);
+            x[e + 9] = fmaf(step, (float)(both >> 20 & 15u), lowest);
+        }
     }
 }
 
@@ -219,17 +271,17 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(256)
 read_kernel(const unsigned char* cache, const int* positions,
             const int* token_request, const int* block_table, int table_width,
-            int page_size, int pages, int kv_heads, int tokens, T* keys, T* values,
+            int page_shift, int pages, int kv_heads, int tokens, T* keys, T* values,
             int* error_flag) {
     using P = Packed<HD>;
     griddep_launch();
     griddep_wait();
-    const int head = blockIdx.y, units = page_size >> 4;
+    const int head = blockIdx.y, units = 1 << (page_shift - 4);
     const unsigned char* from = settled(cache);
     for (int i = threadIdx.x; i < TOKENS * 2 * P::RUNS; i += blockDim.x) {
         const int s = i % P::RUNS, which = i / P::RUNS & 1, t = blockIdx.x * TOKENS + i / (2 * P::RUNS);
         if (t >= tokens) continue;
-        const int position = positions[t], block = position / page_size;
+        const int position = positions[t], block = position >> page_shift;
         const int page = position >= 0 && block < table_width
                              ? block_table[(size_t)token_request[t] * table_width + block] : -1;
         float x[16];
@@ -239,7 +291,7 @@ read_kernel(const unsigned char* cache, const int* positions,
             atomicExch(error_flag, ERROR_READ);
         } else {
             const unsigned char* unit =
-                from + (((size_t)page * kv_heads + head) * units + (position % page_size >> 4)) * P::UNIT;
+                from + (((size_t)page * kv_heads + head) * units + (position >> 4 & (units - 1))) * P::UNIT;
             read_run<HD>(unit + which * P::PART, which, position & 15, s, x);
         }
         store_run((which ? values : keys) + ((size_t)t * kv_heads + head) * HD + s * 16, x);
@@ -249,14 +301,16 @@ read_kernel(const unsigned char* cache, const int* positions,
 // Requests opened: every unit that the requests' tables name, up to their last token, as plain values in
 // pages [2, requests * blocks, open_heads, open_size, HD] of their own, request r's block b in page r * blocks
 // + b, of the key heads from first_head on; rows behind the last token, and of units without a page, are zeros,
-// so that no reader meets a number that is none. `table` gets those page numbers. A thread takes a run of two keys.
+// so that no reader meets a number that is none. `table` gets those page numbers. A thread takes a run of four
+// keys, 2j, 2j + 1, 2j + 8 and 2j + 9: every byte of its eight words is theirs, of the keys' part as of the
+// values'.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256)
-open_kernel(const unsigned char* cache, const int* block_table, int table_width,
-            int page_size, int pages, const int* request_start, const int* history,
-            int span, int first_request, int first_head, int kv_heads, int blocks, int open_size, long long half,
-            T* opened, int* table) {
+open_kernel(const unsigned char* cache, const int* block_table, int table_width, int page_shift, int pages,
+            const int* request_start, const int* history, int span, int first_request, int first_head, int kv_heads,
+            int blocks, int open_size, long long half, T* opened, int* table) {
     using P = Packed<HD>;
+    constexpr int THREADS = 8 * P::RUNS;                         // of a unit
     griddep_launch();
     griddep_wait();
     const unsigned char* from = settled(cache);
@@ -265,38 +319,65 @@ open_kernel(const unsigned char* cache, const int* block_table, int table_width,
     const int held = history[request];
     const int length = held + request_start[request + 1] - request_start[request];
     const int per_block = open_size / 16;
-    const int unit = blockIdx.x * (256 / (P::RUNS * 16)) + threadIdx.x / (P::RUNS * 16);
-    if (open_head == 0 && threadIdx.x % (P::RUNS * 16) == 0 && unit < blocks * per_block && unit % per_block == 0)
-        table[(size_t)r * blocks + unit / per_block] = r * blocks + unit / per_block;
-    if (unit >= blocks * per_block || unit / per_block * open_size >= length) return;
-    const int inside = threadIdx.x % (P::RUNS * 16);
-    const int s = inside % P::RUNS, which = inside / P::RUNS & 1, pair = inside / (2 * P::RUNS);   // pair < 8
+    const int inside = threadIdx.x % THREADS;
+    const int unit = blockIdx.x * (blockDim.x / THREADS) + threadIdx.x / THREADS;
+    if (unit >= blocks * per_block) return;
+    const int open_block = unit / per_block;
+    if (open_head == 0 && inside == 0 && unit % per_block == 0)
+        table[(size_t)r * blocks + open_block] = r * blocks + open_block;
+    if (open_block * open_size >= length) return;
+    const int s = inside % P::RUNS, which = inside / P::RUNS & 1, j = inside / (2 * P::RUNS);
     const int first = unit * 16;
     const bool seen = first < length && first + 15 >= first_visible_key(held, span);
-    const int block = first / page_size;
+    const int block = first >> page_shift;
     int page = seen && block < table_width ? block_table[(size_t)request * table_width + block] : -1;
     if (page >= pages) page = -1;
-    const unsigned char* part = page < 0 ? nullptr
-        : from + (((size_t)page * kv_heads + head) * (page_size >> 4) + (first % page_size >> 4)) * P::UNIT +
-              which * P::PART;
-    T* to = opened + which * half +
-            (((size_t)r * blocks + unit / per_block) * gridDim.y + open_head) * open_size * HD +
-            (size_t)(unit % per_block) * 16 * HD;
+    uint32_t words[8];
+    float step[4], lowest[4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int key = pair * 2 + i;
+    for (int k = 0; k < 8; ++k) words[k] = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) step[k] = lowest[k] = 0.f;
+    if (page >= 0) {
+        const int units = 1 << (page_shift - 4);
+        const unsigned char* part =
+            from + (((size_t)page * kv_heads + head) * units + (first >> 4 & (units - 1))) * P::UNIT + which * P::PART;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)      // keys: rows 2j and 2j + 1, c = k % 4; values: r = k, c = j
+            words[k] = *reinterpret_cast<const uint32_t*>(
+                part + P::word_at(which ? 4 * k + j : 4 * (2 * j + k / 4) + k % 4, s));
+        // (the words of keys 2j, 2j + 8, 2j + 1, 2j + 9 lie side by side)
+        const uint4 scale = *reinterpret_cast<const uint4*>(part + P::scale_at(2 * j, s * 16 / P::GROUP));
+        const uint32_t of_key[4] = {scale.x, scale.z, scale.y, scale.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int key = first + 2 * j + (k & 1) + 8 * (k >> 1);
+            step[k] = key < length ? packed_step(of_key[k]) : 0.f;
+            lowest[k] = key < length ? packed_lowest(of_key[k]) : 0.f;
+        }
+    }
+    T* to = opened + which * half + (((size_t)r * blocks + open_block) * gridDim.y + open_head) * open_size * HD +
+            (size_t)(unit % per_block) * 16 * HD + s * 16;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {        // key 2j + (k & 1) + 8 (k / 2)
         float x[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = 0.f;
-        if (part != nullptr && first + key < length) read_run<HD>(part, which, key, s, x);
-        store_run(to + key * HD + s * 16, x);
+        for (int e = 0; e < 8; ++e) {
+            // keys' words: row 2j + (k & 1), c = e / 2, the byte of the upper half of keys and of odd e; values'
+            // words: r = e, the byte of the upper half of keys and of the odd key
+            const uint32_t both = which ? words[e] >> (8 * (k >> 1) + 16 * (k & 1))
+                                        : words[4 * (k & 1) + e / 2] >> (8 * (k >> 1) + 16 * (e & 1));
+            x[e] = fmaf(step[k], (float)(both & 15u), lowest[k]);
+            x[e + 8] = fmaf(step[k], (float)(both >> 4 & 15u), lowest[k]);
+        }
+        store_run(to + (2 * j + (k & 1) + 8 * (k >> 1)) * HD, x);
     }
 }
 
 int check_geometry(const char* name, int head_dim, int page_size, int pages, int kv_heads, int table_width,
                    const void* cache) {
-    MLXONE_REQUIRE(page_size >= 16 && page_size % 16 == 0, "%s: pages of 4 bits hold a multiple of 16 tokens, not %d",
-                   name, page_size);
+    MLXONE_REQUIRE(page_size >= 16 && (page_size & (page_size - 1)) == 0,
+                   "%s: pages of 4 bits hold a power of two of tokens, 16 or more, not %d", name, page_size);
     MLXONE_REQUIRE(pages > 0 && table_width > 0 && kv_heads > 0 && kv_heads <= 65535, "%s: bad page geometry", name);
     MLXONE_REQUIRE(((size_t)cache & 15) == 0, "%s: the cache starts at a multiple of 16 bytes", name);
     MLXONE_REQUIRE(head_dim % 32 == 0 && head_dim >= 32 && head_dim <= 128,
@@ -325,16 +406,17 @@ MLXONE_API int mlxone_pack_key_values(const void* keys, long long key_stride, co
     const int wide = ((size_t)keys & 15) == 0 && ((size_t)values & 15) == 0 && key_stride * size % 16 == 0 &&
                      value_stride * size % 16 == 0;
     const dim3 grid(ceil_div_host(tokens, TOKENS), kv_heads);
+    const int page_shift = 31 - __builtin_clz((unsigned)page_size);
 #define CALL(HD)                                                                                          \
     if (dtype == MLXONE_BF16)                                                                             \
         launch_kernel(pack_kernel<bf16, HD>, grid, dim3(256), 0, stream, true, (const bf16*)keys,         \
                       key_stride, (const bf16*)values, value_stride, wide, positions, token_request,      \
-                      request_start, block_table, table_width, page_size, pages, kv_heads, tokens,        \
+                      request_start, block_table, table_width, page_shift, pages, kv_heads, tokens,        \
                       (unsigned char*)cache, error_flag);                                                 \
     else                                                                                                  \
         launch_kernel(pack_kernel<float, HD>, grid, dim3(256), 0, stream, true, (const float*)keys,       \
                       key_stride, (const float*)values, value_stride, wide, positions, token_request,     \
-                      request_start, block_table, table_width, page_size, pages, kv_heads, tokens,        \
+                      request_start, block_table, table_width, page_shift, pages, kv_heads, tokens,        \
                       (unsigned char*)cache, error_flag)
     MLXONE_PACKED_DIMS(CALL)
 #undef CALL
@@ -350,14 +432,15 @@ MLXONE_API int mlxone_read_key_values(const void* cache, const int* positions, c
     if (check_geometry("read_key_values", head_dim, page_size, pages, kv_heads, table_width, cache)) return 1;
     MLXONE_REQUIRE(tokens > 0, "read_key_values: bad token count");
     const dim3 grid(ceil_div_host(tokens, TOKENS), kv_heads);
+    const int page_shift = 31 - __builtin_clz((unsigned)page_size);
 #define CALL(HD)                                                                                          \
     if (dtype == MLXONE_BF16)                                                                             \
         launch_kernel(read_kernel<bf16, HD>, grid, dim3(256), 0, stream, true, (const unsigned char*)cache, \
-                      positions, token_request, block_table, table_width, page_size, pages, kv_heads,     \
+                      positions, token_request, block_table, table_width, page_shift, pages, kv_heads,    \
                       tokens, (bf16*)keys, (bf16*)values, error_flag);                                    \
     else                                                                                                  \
         launch_kernel(read_kernel<float, HD>, grid, dim3(256), 0, stream, true, (const unsigned char*)cache, \
-                      positions, token_request, block_table, table_width, page_size, pages, kv_heads,     \
+                      positions, token_request, block_table, table_width, page_shift, pages, kv_heads,    \
                       tokens, (float*)keys, (float*)values, error_flag)
     MLXONE_PACKED_DIMS(CALL)
 #undef CALL
@@ -379,18 +462,19 @@ MLXONE_API int mlxone_open_key_values(const void* cache, const int* block_table,
                        open_size % 16 == 0 && first_head >= 0 && open_heads > 0 &&
                        first_head + open_heads <= kv_heads, "open_key_values: bad sizes");
     const long long half = (long long)requests * blocks * open_heads * open_size * head_dim;
-    const int per = 256 / head_dim;               // units of a block (RUNS * 16 = head_dim threads a unit)
+    const int per = 256 / (head_dim / 2);         // units of a block (8 RUNS = head_dim / 2 threads a unit)
     MLXONE_REQUIRE(((size_t)opened & 15) == 0, "open_key_values: the output starts at a multiple of 16 bytes");
     const dim3 grid(ceil_div_host((long long)blocks * (open_size / 16), per), open_heads, requests);
+    const int page_shift = 31 - __builtin_clz((unsigned)page_size);
 #define CALL(HD)                                                                                          \
     if (dtype == MLXONE_BF16)                                                                             \
-        launch_kernel(open_kernel<bf16, HD>, grid, dim3(per * HD), 0, stream, true,                       \
-                      (const unsigned char*)cache, block_table, table_width, page_size, pages,            \
+        launch_kernel(open_kernel<bf16, HD>, grid, dim3(per * HD / 2), 0, stream, true,                       \
+                      (const unsigned char*)cache, block_table, table_width, page_shift, pages,           \
                       request_start, history, span, first_request, first_head, kv_heads, blocks, open_size, half,     \
                       (bf16*)opened, table);                                                              \
     else                                                                                                  \
-        launch_kernel(open_kernel<float, HD>, grid, dim3(per * HD), 0, stream, true,                      \
-                      (const unsigned char*)cache, block_table, table_width, page_size, pages,            \
+        launch_kernel(open_kernel<float, HD>, grid, dim3(per * HD / 2), 0, stream, true,                      \
+                      (const unsigned char*)cache, block_table, table_width, page_shift, pages,           \
                       request_start, history, span, first_request, first_head, kv_heads, blocks, open_size, half,     \
                       (float*)opened, table)
     MLXONE_PACKED_DIMS(CALL)

@@ -62,6 +62,7 @@ class CudaOps:
         self.lib.mlxone_lightning_scratch.restype = ctypes.c_longlong
         self.lib.mlxone_state_space_scratch.restype = ctypes.c_longlong
         self.lib.mlxone_gated_recurrence_scratch.restype = ctypes.c_longlong
+        self.lib.mlxone_beam_scratch.restype = ctypes.c_longlong
         if self.lib.mlxone_abi_version() != 1:
             raise KernelBuildError("the CUDA extension is of another version; rebuild it")
         self.error_flag = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -2191,16 +2192,15 @@ class CudaOps:
         over = torch.empty((requests, beams), dtype=torch.uint8, device=self.device)
         rows = requests * beams
         if rows:
-            parts = self.lib.mlxone_beam_parts(rows, vocab)
-            scratch = torch.empty(rows * parts * (beams + 1), dtype=torch.int64, device=self.device)
-            sums = scratch.data_ptr() + 8 * rows * parts * beams
+            scratch = torch.empty(self.lib.mlxone_beam_scratch(requests, beams, vocab), dtype=torch.uint8,
+                                  device=self.device)
             self._call("mlxone_beam_select", _c_void_p(_ptr(logits)), _c_ll(logits.stride(0)),
                        _c_int(requests), _c_int(beams), _c_int(vocab), _c_void_p(_ptr(scores)),
                        _c_void_p(_ptr(ended)), _c_void_p(_ptr(end_tokens)),
-                       _c_int(0 if end_tokens is None else end_tokens.numel()), _c_int(parts),
-                       _c_void_p(sums), _c_void_p(_ptr(scratch)), _c_void_p(_ptr(chosen)),
-                       _c_void_p(_ptr(parents)), _c_void_p(_ptr(tokens)), _c_void_p(_ptr(over)))
-            self.launches += 1              # the parts, then the choice
+                       _c_int(0 if end_tokens is None else end_tokens.numel()), _c_void_p(_ptr(scratch)),
+                       _c_void_p(_ptr(chosen)), _c_void_p(_ptr(parents)), _c_void_p(_ptr(tokens)),
+                       _c_void_p(_ptr(over)))
+            self.launches += 1              # the sums, then the choice
         return chosen, parents, tokens, over
 
     def _need_parents(self, parents) -> None:
