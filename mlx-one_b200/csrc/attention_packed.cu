@@ -758,11 +758,6 @@ int launch_packed(const void* q, const void* cache, const int* block_table, int 
 // Splits that a cluster merges; more need `partial`.
 MLXONE_API int mlxone_attention_packed_cluster() { return CLUSTER; }
 
-// Blocks of the kernel that an SM holds at once.
-MLXONE_API int mlxone_attention_packed_resident(int head_dim, int dtype) {
-    return head_dim <= 64 || dtype == MLXONE_BF16 ? 2 : 1;
-}
-
 // One token a request: q [requests, heads, head_dim], positions [requests] (each token's own position: the last key
 // that it sees; below 0: none). window: as first_visible_key's span. sinks: float32 [heads] or null. partial:
 // null where `splits` is at most mlxone_attention_packed_cluster(), else requests * heads * splits *

@@ -301,8 +301,8 @@ read_kernel(const unsigned char* cache, const int* positions,
 // Requests opened: every unit that the requests' tables name, up to their last token, as plain values in
 // pages [2, requests * blocks, open_heads, open_size, HD] of their own, request r's block b in page r * blocks
 // + b, of the key heads from first_head on; rows behind the last token, and of units without a page, are zeros,
-// so that no reader meets a number that is none. `table` gets those page numbers. A thread takes a run of four
-// keys, 2j, 2j + 1, 2j + 8 and 2j + 9: every byte of its eight words is theirs, of the keys' part as of the
+// so that no reader meets a number that is none. `table` gets those page numbers and, behind them, where the
+// requests' tokens start, counted from the first one's. A thread takes a run of four keys, 2j, 2j + 1, 2j + 8 and 2j + 9: every byte of its eight words is theirs, of the keys' part as of the
 // values'.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256)
@@ -323,8 +323,15 @@ open_kernel(const unsigned char* cache, const int* block_table, int table_width,
     const int unit = blockIdx.x * (blockDim.x / THREADS) + threadIdx.x / THREADS;
     if (unit >= blocks * per_block) return;
     const int open_block = unit / per_block;
-    if (open_head == 0 && inside == 0 && unit % per_block == 0)
+    if (open_head == 0 && inside == 0 && unit % per_block == 0) {
         table[(size_t)r * blocks + open_block] = r * blocks + open_block;
+        if (unit == 0) {
+            int* starts = table + (size_t)gridDim.z * blocks;
+            const int base = request_start[first_request];
+            starts[r] = request_start[request] - base;
+            if (r + 1 == (int)gridDim.z) starts[r + 1] = request_start[request + 1] - base;
+        }
+    }
     if (open_block * open_size >= length) return;
     const int s = inside % P::RUNS, which = inside / P::RUNS & 1, j = inside / (2 * P::RUNS);
     const int first = unit * 16;
@@ -450,7 +457,7 @@ MLXONE_API int mlxone_read_key_values(const void* cache, const int* positions, c
 
 // Requests first_request.. (`requests` of them) and key heads first_head.. (`open_heads` of kv_heads), `blocks`
 // pages of `open_size` tokens (a multiple of 16) for each request: opened [2, requests * blocks, open_heads,
-// open_size, head_dim], table int32 [requests, blocks]. `span`: see first_visible_key; units that no token of the
+// open_size, head_dim], table int32 [requests * blocks + requests + 1]. `span`: see first_visible_key; units that no token of the
 // step sees are zeros.
 MLXONE_API int mlxone_open_key_values(const void* cache, const int* block_table, int table_width, int page_size,
                                       int pages, const int* request_start, const int* history, int span,

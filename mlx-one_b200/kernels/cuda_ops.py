@@ -13,12 +13,11 @@ products of the values' parts (24 bits of every value, sums in 32 bits).
 from __future__ import annotations
 
 import ctypes
-from dataclasses import replace
 from typing import Any
 
 import torch
 
-from ..parts.base import NormedInput, NormedUpdate, PackedView, PagedView
+from ..parts.base import NormedInput, NormedUpdate, PackedView, PagedView, StepContext
 from .build import KernelBuildError, library_path
 
 _F32, _BF16 = 0, 1
@@ -63,6 +62,20 @@ class CudaOps:
         self.lib.mlxone_state_space_scratch.restype = ctypes.c_longlong
         self.lib.mlxone_gated_recurrence_scratch.restype = ctypes.c_longlong
         self.lib.mlxone_beam_scratch.restype = ctypes.c_longlong
+        # (entry points that small calls go through: their arguments are converted by ctypes, which costs a
+        # fraction of wrapping each of them here)
+        pointer, whole, long, real = _c_void_p, _c_int, _c_ll, _c_float
+        for name, kinds in {
+                "mlxone_pack_key_values": [pointer, long, pointer, long, *[pointer] * 4, *[whole] * 6, pointer, whole,
+                                           pointer, pointer],
+                "mlxone_read_key_values": [*[pointer] * 4, *[whole] * 6, pointer, pointer, whole, pointer, pointer],
+                "mlxone_attention_packed": [*[pointer] * 3, *[whole] * 3, *[pointer] * 3, *[whole] * 5, real, whole,
+                                            pointer, whole, pointer, pointer],
+                "mlxone_beam_select": [pointer, long, *[whole] * 3, *[pointer] * 3, whole, *[pointer] * 5, pointer],
+                "mlxone_reorder_slots": [pointer, *[long] * 3, pointer, pointer, whole, whole, pointer, pointer],
+                "mlxone_reorder_pages": [pointer, *[long] * 3, pointer, whole, *[pointer] * 3, *[whole] * 3, pointer,
+                                         pointer]}.items():
+            getattr(self.lib, name).argtypes = kinds
         if self.lib.mlxone_abi_version() != 1:
             raise KernelBuildError("the CUDA extension is of another version; rebuild it")
         self.error_flag = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -142,6 +155,7 @@ class CudaOps:
         self.open_page = 64
         self.open_bytes = 1 << 29
         self._packed_cluster = self.lib.mlxone_attention_packed_cluster()
+        self._packed_shapes: dict[tuple, tuple] = {}       # geometry of packed pages -> their trailing shape
         # the gated recurrence of few single tokens: the gates' product in the recurrence's kernel
         self.fused_recurrence = True
         self._sample_scratch: torch.Tensor | None = None
@@ -160,6 +174,13 @@ class CudaOps:
     def _call(self, name: str, *args: Any) -> None:
         code = getattr(self.lib, name)(*args, _c_void_p(self._stream()))
         if code != 0:
+            raise KernelError(self.lib.mlxone_last_error().decode())
+        self.launches += 1
+
+    def _launch(self, function, *args) -> None:
+        """``_call`` of an entry point whose argument types are declared (see ``__init__``): plain numbers
+        and addresses."""
+        if function(*args, self._stream()) != 0:
             raise KernelError(self.lib.mlxone_last_error().decode())
         self.launches += 1
 
@@ -1979,19 +2000,23 @@ class CudaOps:
 
     def _need_packed(self, view) -> int:
         """Checks a view of packed pages; returns how many pages there are."""
-        kv, need, size = view.kv, view.need, view.page_size
-        if size < 16 or size & (size - 1):
-            raise KernelError(f"pages of 4 bits hold a power of two of tokens, 16 or more, not {size}")
-        unit = self.lib.mlxone_packed_unit_bytes(need.head_dim)
-        if not unit or need.planes != 2:
-            raise KernelError(f"a cache of 4 bits takes keys and values of 32, 64, 96 or 128 values a "
-                              f"head, not {need.head_dim} in {need.planes} planes")
-        if (kv.dtype != torch.uint8 or not kv.is_contiguous() or kv.device != self.device
-                or kv.dim() != 5 or kv.shape[1:] != (need.kv_heads, size // 16, 2, unit // 2)):
-            raise KernelError(f"packed pages must be contiguous uint8 [pages, {need.kv_heads}, {size // 16}, "
-                              f"2, {unit // 2}] on {self.device}, got {kv.dtype} {tuple(kv.shape)} on "
-                              f"{kv.device}")
-        self._need(view.block_table, torch.int32, "block table")
+        kv, need, size, table = view.kv, view.need, view.page_size, view.block_table
+        geometry = (need.kv_heads, need.head_dim, need.planes, size)
+        shape = self._packed_shapes.get(geometry)
+        if shape is None:
+            if size < 16 or size & (size - 1):
+                raise KernelError(f"pages of 4 bits hold a power of two of tokens, 16 or more, not {size}")
+            unit = self.lib.mlxone_packed_unit_bytes(need.head_dim)
+            if not unit or need.planes != 2:
+                raise KernelError(f"a cache of 4 bits takes keys and values of 32, 64, 96 or 128 values a "
+                                  f"head, not {need.head_dim} in {need.planes} planes")
+            shape = self._packed_shapes[geometry] = (need.kv_heads, size // 16, 2, unit // 2)
+        if kv.dtype != torch.uint8 or kv.shape[1:] != shape or not kv.is_contiguous() or kv.device != self.device:
+            raise KernelError(f"packed pages must be contiguous uint8 [pages, {', '.join(map(str, shape))}] on "
+                              f"{self.device}, got {kv.dtype} {tuple(kv.shape)} on {kv.device}")
+        if table.dtype != torch.int32 or table.dim() != 2:
+            raise KernelError(f"a block table must be int32 [requests, width], got {table.dtype} {tuple(table.shape)}")
+        self._need(table, torch.int32, "block table")
         return kv.shape[0]
 
     def pack_key_values(self, keys, values, *, ctx, view):
@@ -2000,36 +2025,30 @@ class CudaOps:
         ``view``. Every group of a token's values (64; 32 where 64 do not divide the head) is held as its
         lowest value and a step in bfloat16 and a code of 0 to 15 a value, the nearest; a group with a
         value that is not finite reads as NaN. Other tokens' bytes stay as they are."""
-        pages = self._need_packed(view)
-        kv_heads, head_dim = view.need.kv_heads, view.need.head_dim
-        tokens = keys.shape[0]
+        pages, code = self._need_packed(view), _dtype_code(keys.dtype)
+        need, table = view.need, view.block_table
+        wanted, dtype = (ctx.tokens, need.kv_heads * need.head_dim), keys.dtype
         for rows, what in ((keys, "keys"), (values, "values")):
-            self._need_rows(rows, keys.dtype, what)
-            if rows.shape != (tokens, kv_heads * head_dim):
-                raise KernelError(f"{what} must be [{tokens}, {kv_heads} * {head_dim}], got {tuple(rows.shape)}")
-        if tokens != ctx.tokens:
-            raise KernelError(f"the step has {ctx.tokens} tokens, {tokens} rows were given")
-        self._call("mlxone_pack_key_values", _c_void_p(_ptr(keys)), _c_ll(keys.stride(0)),
-                   _c_void_p(_ptr(values)), _c_ll(values.stride(0)), _c_void_p(_ptr(ctx.positions)),
-                   _c_void_p(_ptr(ctx.token_request)), _c_void_p(_ptr(ctx.request_start)),
-                   _c_void_p(_ptr(view.block_table)), _c_int(view.block_table.shape[1]),
-                   _c_int(view.page_size), _c_int(pages), _c_int(kv_heads), _c_int(head_dim),
-                   _c_int(tokens), _c_void_p(_ptr(view.kv)), _c_int(_dtype_code(keys.dtype)),
-                   _c_void_p(_ptr(self.error_flag)))
+            self._need_rows(rows, dtype, what)
+            if rows.shape != wanted:
+                raise KernelError(f"{what} of a step of {ctx.tokens} tokens must be {wanted}, got {tuple(rows.shape)}")
+        self._launch(self.lib.mlxone_pack_key_values, keys.data_ptr(), keys.stride(0), values.data_ptr(),
+                     values.stride(0), ctx.positions.data_ptr(), ctx.token_request.data_ptr(),
+                     ctx.request_start.data_ptr(), table.data_ptr(), table.shape[1], view.page_size, pages,
+                     need.kv_heads, need.head_dim, ctx.tokens, view.kv.data_ptr(), code,
+                     self.error_flag.data_ptr())
 
     def read_key_values(self, *, ctx, view, dtype=torch.bfloat16):
         """What attention finds at the step's tokens' places in packed pages: (keys, values), each
         [tokens, kv_heads, head_dim] in ``dtype``."""
-        pages = self._need_packed(view)
-        kv_heads, head_dim = view.need.kv_heads, view.need.head_dim
-        keys = torch.empty((ctx.tokens, kv_heads, head_dim), dtype=dtype, device=self.device)
+        pages, code = self._need_packed(view), _dtype_code(dtype)
+        need, table = view.need, view.block_table
+        keys = torch.empty((ctx.tokens, need.kv_heads, need.head_dim), dtype=dtype, device=self.device)
         values = torch.empty_like(keys)
-        self._call("mlxone_read_key_values", _c_void_p(_ptr(view.kv)), _c_void_p(_ptr(ctx.positions)),
-                   _c_void_p(_ptr(ctx.token_request)), _c_void_p(_ptr(view.block_table)),
-                   _c_int(view.block_table.shape[1]), _c_int(view.page_size), _c_int(pages),
-                   _c_int(kv_heads), _c_int(head_dim), _c_int(ctx.tokens), _c_void_p(_ptr(keys)),
-                   _c_void_p(_ptr(values)), _c_int(_dtype_code(dtype)),
-                   _c_void_p(_ptr(self.error_flag)))
+        self._launch(self.lib.mlxone_read_key_values, view.kv.data_ptr(), ctx.positions.data_ptr(),
+                     ctx.token_request.data_ptr(), table.data_ptr(), table.shape[1], view.page_size, pages,
+                     need.kv_heads, need.head_dim, ctx.tokens, keys.data_ptr(), values.data_ptr(), code,
+                     self.error_flag.data_ptr())
         return keys, values
 
     def _prepare_packed(self, qkv, *, kv_heads, ctx, view, write, **how):
@@ -2052,7 +2071,7 @@ class CudaOps:
         others are opened into pages of the compute dtype, a scratch of this call, which the prefill
         kernels read: a portion has many queries for every key that is opened. So do single tokens whose
         scores are shaped or that see first positions behind a window."""
-        pages = self._need_packed(view)
+        pages, code = self._need_packed(view), _dtype_code(q.dtype)
         self._need(q, q.dtype, "q")
         tokens, requests, width = q.shape[0], ctx.requests, view.block_table.shape[1]
         if q.numel() != tokens * heads * head_dim or heads % kv_heads or \
@@ -2070,11 +2089,14 @@ class CudaOps:
                 raise KernelError("one sink per query head")
         if out is None:
             out = torch.empty((tokens, heads * head_dim), dtype=q.dtype, device=self.device)
-        shaped = bool(score_cap) or slopes is not None or (bool(keep_first) and window > 0)
         singles = requests if ctx.max_portion == 1 and tokens == requests else min(ctx.leading_single, requests)
-        if shaped:
+        if score_cap or slopes is not None or (keep_first and window > 0):
             singles = 0
         bound = min(ctx.max_context, width * view.page_size)
+        if requests > singles and tokens > singles:
+            self._opened_attention(q, out, singles, bound, heads, kv_heads, head_dim, scale, window, ctx, view, pages,
+                                   sinks=sinks, keep_first=keep_first, score_cap=score_cap, slopes=slopes,
+                                   least_slope=least_slope)
         if singles:
             splits = self.packed_splits(singles, heads, kv_heads, head_dim, bound, window, q.dtype)
             partial = None
@@ -2082,38 +2104,46 @@ class CudaOps:
                 partial = torch.empty(singles * heads * splits * (head_dim + 2), dtype=torch.float32,
                                       device=self.device)
                 self.launches += 1          # the merge kernel
-            self._call("mlxone_attention_packed", _c_void_p(_ptr(q)), _c_void_p(_ptr(view.kv)),
-                       _c_void_p(_ptr(view.block_table)), _c_int(width), _c_int(view.page_size),
-                       _c_int(pages), _c_void_p(_ptr(ctx.positions)), _c_void_p(_ptr(out)),
-                       _c_void_p(_ptr(partial)), _c_int(singles), _c_int(heads), _c_int(kv_heads),
-                       _c_int(head_dim), _c_int(splits), _c_float(scale), _c_int(window),
-                       _c_void_p(_ptr(sinks)), _c_int(_dtype_code(q.dtype)),
-                       _c_void_p(_ptr(self.error_flag)))
-        rest = requests - singles
-        if not rest or tokens == singles:
-            return out
+            self._launch(self.lib.mlxone_attention_packed, q.data_ptr(), view.kv.data_ptr(),
+                         view.block_table.data_ptr(), width, view.page_size, pages, ctx.positions.data_ptr(),
+                         out.data_ptr(), _ptr(partial), singles, heads, kv_heads, head_dim, splits, scale, window,
+                         _ptr(sinks), code, self.error_flag.data_ptr())
+        return out
+
+    def _opened_attention(self, q, out, singles, bound, heads, kv_heads, head_dim, scale, window, ctx, view, pages, *,
+                          sinks, keep_first, score_cap, slopes, least_slope) -> None:
+        """The requests of a step behind the first ``singles``, whose keys are opened."""
+        tokens, rest = q.shape[0], ctx.requests - singles
+        blocks = max(-(-bound // self.open_page), 1)
+        group, width = heads // kv_heads, view.block_table.shape[1]
+        table = torch.empty(rest * blocks + rest + 1, dtype=torch.int32, device=self.device)
+        queries, result = q, out
+        if singles:
+            # the rest as a step of its own (the 32-bit kernels go by token, the others by request)
+            positions, token_request = ctx.positions, ctx.token_request
+            if q.dtype == torch.float32:
+                positions, token_request = positions[singles:], token_request[singles:tokens] - singles
+            step = StepContext(tokens=tokens - singles, requests=rest, token_ids=positions, positions=positions,
+                               token_request=token_request, request_start=table[rest * blocks:],
+                               history=ctx.history[singles:], max_portion=0, max_context=ctx.max_context)
+            queries, result = q.view(tokens, heads, head_dim)[singles:], out[singles:]
+        else:
+            step = StepContext(tokens=tokens, requests=rest, token_ids=ctx.token_ids, positions=ctx.positions,
+                               token_request=ctx.token_request, request_start=ctx.request_start,
+                               history=ctx.history, max_portion=0, max_context=ctx.max_context)
         # (never as a step of single tokens: their kernels read pages ahead of the wait for the kernel before
         # them, which here is the one that fills the pages)
-        step = replace(ctx, leading_single=0, max_portion=max(ctx.max_portion, 2))
-        if singles:
-            step = replace(step, tokens=tokens - singles, requests=rest, token_ids=ctx.token_ids[singles:],
-                           positions=ctx.positions[singles:],
-                           token_request=ctx.token_request[singles:tokens] - singles,
-                           request_start=ctx.request_start[singles:] - singles,
-                           history=ctx.history[singles:])
-        blocks = max(-(-bound // self.open_page), 1)
-        group = heads // kv_heads
+        step.max_portion = max(ctx.max_portion, 2)
         each = 2 * rest * blocks * self.open_page * head_dim * q.element_size()      # bytes a key head
         at_once = max(min(self.open_bytes // each, kv_heads), 1)
-        queries = q.view(tokens, heads, head_dim)[singles:]
         opened = torch.empty((2, rest * blocks, at_once, self.open_page, head_dim), dtype=q.dtype,
                              device=self.device)
-        table = torch.empty((rest, blocks), dtype=torch.int32, device=self.device)
+        numbers = table[:rest * blocks].view(rest, blocks)
         for first in range(0, kv_heads, at_once):
             count = min(at_once, kv_heads - first)
             here = opened if count == at_once else opened.view(-1)[:opened.numel() // at_once * count].view(
                 2, rest * blocks, count, self.open_page, head_dim)
-            # (chunks, and windows with first positions that stay, open everything)
+            # (windows with first positions that stay open everything)
             self._call("mlxone_open_key_values", _c_void_p(_ptr(view.kv)), _c_void_p(_ptr(view.block_table)),
                        _c_int(width), _c_int(view.page_size), _c_int(pages),
                        _c_void_p(_ptr(ctx.request_start)), _c_void_p(_ptr(ctx.history)),
@@ -2121,19 +2151,18 @@ class CudaOps:
                        _c_int(first), _c_int(count), _c_int(head_dim), _c_int(blocks),
                        _c_int(self.open_page), _c_void_p(_ptr(here)), _c_void_p(_ptr(table)),
                        _c_int(_dtype_code(q.dtype)))
-            plain = PagedView(here, table, self.open_page, view.need)
+            plain = PagedView(here, numbers, self.open_page, view.need)
             own = slice(first * group, (first + count) * group)
-            common = dict(heads=count * group, kv_heads=count, head_dim=head_dim, scale=scale, window=window,
-                          ctx=step, view=plain, sinks=None if sinks is None else sinks[own],
-                          keep_first=keep_first, score_cap=score_cap,
-                          slopes=None if slopes is None else slopes[own], least_slope=least_slope)
+            how = dict(heads=count * group, kv_heads=count, head_dim=head_dim, scale=scale, window=window, ctx=step,
+                       view=plain, keep_first=keep_first, score_cap=score_cap, least_slope=least_slope)
             if count == kv_heads:
-                self.paged_attention(queries, out=out[singles:], **common)
-            else:
-                # (more than the scratch holds: some key heads after the others)
-                part = self.paged_attention(queries[:, own].contiguous(), **common)
-                out.view(tokens, heads, head_dim)[singles:, own] = part.view(-1, count * group, head_dim)
-        return out
+                self.paged_attention(queries, out=result, sinks=sinks, slopes=slopes, **how)
+                return
+            # (more than the scratch holds: some key heads after the others)
+            part = self.paged_attention(queries.view(-1, heads, head_dim)[:, own].contiguous(),
+                                        sinks=None if sinks is None else sinks[own],
+                                        slopes=None if slopes is None else slopes[own], **how)
+            result.view(-1, heads, head_dim)[:, own] = part.view(-1, count * group, head_dim)
 
     def packed_splits(self, requests: int, heads: int, kv_heads: int, head_dim: int, context_bound: int,
                       window: int, dtype=torch.bfloat16) -> int:
@@ -2153,7 +2182,8 @@ class CudaOps:
         if tiles <= 16:
             return 1
         blocks = requests * kv_heads * -(-(heads // kv_heads) // 8)
-        resident = self._sm_count * self.lib.mlxone_attention_packed_resident(head_dim, _dtype_code(dtype))
+        # (blocks that an SM holds: the kernel's launch bounds)
+        resident = self._sm_count * (2 if head_dim <= 64 or dtype == torch.bfloat16 else 1)
         if tiles >= 64 * self._packed_cluster and resident // blocks > self._packed_cluster:
             return max(min(resident // blocks, tiles // 20), self._packed_cluster)
         return max(min(resident * 9 // (10 * blocks), -(-tiles // 4), self._packed_cluster), 1)
@@ -2186,20 +2216,18 @@ class CudaOps:
                 raise KernelError("ended needs an entry per hypothesis, and a token that ends one")
         if end_tokens is not None:
             self._need(end_tokens, torch.int32, "end tokens")
-        chosen = torch.empty((requests, beams), dtype=torch.float32, device=self.device)
-        parents = torch.empty((requests, beams), dtype=torch.int32, device=self.device)
-        tokens = torch.empty((requests, beams), dtype=torch.int32, device=self.device)
-        over = torch.empty((requests, beams), dtype=torch.uint8, device=self.device)
+        chosen = torch.empty_like(scores)
+        parents = torch.empty_like(scores, dtype=torch.int32)
+        tokens = torch.empty_like(parents)
+        over = torch.empty_like(scores, dtype=torch.uint8)
         rows = requests * beams
         if rows:
             scratch = torch.empty(self.lib.mlxone_beam_scratch(requests, beams, vocab), dtype=torch.uint8,
                                   device=self.device)
-            self._call("mlxone_beam_select", _c_void_p(_ptr(logits)), _c_ll(logits.stride(0)),
-                       _c_int(requests), _c_int(beams), _c_int(vocab), _c_void_p(_ptr(scores)),
-                       _c_void_p(_ptr(ended)), _c_void_p(_ptr(end_tokens)),
-                       _c_int(0 if end_tokens is None else end_tokens.numel()), _c_void_p(_ptr(scratch)),
-                       _c_void_p(_ptr(chosen)), _c_void_p(_ptr(parents)), _c_void_p(_ptr(tokens)),
-                       _c_void_p(_ptr(over)))
+            self._launch(self.lib.mlxone_beam_select, logits.data_ptr(), logits.stride(0), requests, beams, vocab,
+                         scores.data_ptr(), _ptr(ended), _ptr(end_tokens),
+                         0 if end_tokens is None else end_tokens.numel(), scratch.data_ptr(), chosen.data_ptr(),
+                         parents.data_ptr(), tokens.data_ptr(), over.data_ptr())
             self.launches += 1              # the sums, then the choice
         return chosen, parents, tokens, over
 
@@ -2222,10 +2250,9 @@ class CudaOps:
         if requests == 0 or state.numel() == 0:
             return
         entries, count = state.shape[:2]
-        self._call("mlxone_reorder_slots", _c_void_p(_ptr(state)), _c_ll(entries), _c_ll(count),
-                   _c_ll(state.numel() // (entries * count) * state.element_size()), _c_void_p(_ptr(slots)),
-                   _c_void_p(_ptr(parents)), _c_int(requests), _c_int(beams),
-                   _c_void_p(_ptr(self.error_flag)))
+        self._launch(self.lib.mlxone_reorder_slots, state.data_ptr(), entries, count,
+                     state.numel() // (entries * count) * state.element_size(), slots.data_ptr(), parents.data_ptr(),
+                     requests, beams, self.error_flag.data_ptr())
 
     def reorder_pages(self, storage, block_table, parents, starts, lengths, *, page_size) -> None:
         """In place: in every entry of ``storage`` [entries, pages, ...] (any type, contiguous; planes are
@@ -2247,11 +2274,10 @@ class CudaOps:
         if requests == 0 or storage.numel() == 0 or block_table.shape[1] == 0:
             return
         outer, pages = storage.shape[:2]
-        self._call("mlxone_reorder_pages", _c_void_p(_ptr(storage)), _c_ll(outer), _c_ll(pages),
-                   _c_ll(storage.numel() // (outer * pages) * storage.element_size()),
-                   _c_void_p(_ptr(block_table)), _c_int(block_table.shape[1]), _c_void_p(_ptr(parents)),
-                   _c_void_p(_ptr(starts)), _c_void_p(_ptr(lengths)), _c_int(page_size), _c_int(requests),
-                   _c_int(beams), _c_void_p(_ptr(self.error_flag)))
+        self._launch(self.lib.mlxone_reorder_pages, storage.data_ptr(), outer, pages,
+                     storage.numel() // (outer * pages) * storage.element_size(), block_table.data_ptr(),
+                     block_table.shape[1], parents.data_ptr(), starts.data_ptr(), lengths.data_ptr(), page_size,
+                     requests, beams, self.error_flag.data_ptr())
 
     def argmax(self, logits):
         self._need(logits, torch.float32, "logits")

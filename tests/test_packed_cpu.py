@@ -14,9 +14,6 @@ class Library:
     def mlxone_packed_unit_bytes(self, dim):
         return 2 * packed_part_bytes(dim) if dim in (32, 64, 96, 128) else 0
 
-    def mlxone_attention_packed_resident(self, dim, dtype):
-        return 2
-
     def __getattr__(self, name):
         raise AssertionError(f"{name} was launched")
 
@@ -26,7 +23,7 @@ def ops():
     ops = CudaOps.__new__(CudaOps)
     ops.device, ops.lib, ops._sm_count = torch.device("cpu"), Library(), 148
     ops.error_flag = torch.zeros(1, dtype=torch.int32)
-    ops._packed_cluster, ops._device_index = 8, 0
+    ops._packed_cluster, ops._device_index, ops._packed_shapes = 8, 0, {}
     return ops
 
 
