@@ -256,30 +256,32 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
     unsigned char* ring = shared + warp * R::STAGES * R::STAGE;
     auto barrier = [&](int stage) { return shared_address(&barriers[warp * R::STAGES + stage]); };
     // Where the units of a warp's tiles lie, a lane each for AHEAD tiles at a time (lane = tile of these * UNITS +
-    // unit; -1: no key of it is seen); the next ones are looked up half a turn before the first is wanted.
+    // unit; -1: no key of it is seen); the next ones are looked up half a turn before the first is wanted. A unit
+    // that has keys to be seen but no page makes every tile go by the mask, which then looks at the pages.
     constexpr int AHEAD = 32 / UNITS;
-    auto look_up = [&](int first_tile) -> long long {
+    bool holes = false;
+    auto look_up = [&](int first_tile) -> int {
         const int tile = first_tile + lane / UNITS * WARPS;
         const int key = tile * KEYS + 16 * (lane % UNITS);
         if (tile >= to || key > position || key + 15 < lowest_key) return -1;
         const int block = key >> page_shift;
         const int page = block < table_width ? table[block] : -1;
-        if (page < 0 || page >= pages) return -1;
-        return ((long long)page * kv_heads + kv_head) * units_per_page + ((key & ((1 << page_shift) - 1)) >> 4);
+        if (page < 0 || page >= pages) {
+            holes = true;
+            return -1;
+        }
+        return (page * kv_heads + kv_head) * units_per_page + ((key & ((1 << page_shift) - 1)) >> 4);
     };
-    uint32_t live_units = 0;               // UNITS bits a stage: which units it holds
-    constexpr uint32_t EVERY = (1u << UNITS) - 1;
     int tile = from + warp, turn = 0;          // turn: of AHEAD, the place of the next tile to be asked for
-    long long units_now = look_up(tile), units_next = -1;
+    int units_now = look_up(tile), units_next = -1;
+    const uint32_t my_ring = shared_address(ring) + lane * P::UNIT;
     auto fetch = [&](int stage, int asked) {
-        const long long unit = __shfl_sync(0xffffffffu, units_now, turn * UNITS + (lane & (UNITS - 1)));
-        const unsigned live = __ballot_sync(0xffffffffu, unit >= 0) & EVERY;
-        live_units = (live_units & ~(EVERY << (UNITS * stage))) | live << (UNITS * stage);
+        const int unit = __shfl_sync(0xffffffffu, units_now, turn * UNITS + (lane & (UNITS - 1)));
+        const unsigned live = __ballot_sync(0xffffffffu, lane < UNITS && unit >= 0);
         if (lane == 0) barrier_expect(barrier(stage), (uint32_t)__popc(live) * P::UNIT);
         __syncwarp();
         if (lane < UNITS && unit >= 0)
-            bulk_load(shared_address(ring + stage * R::STAGE + lane * P::UNIT), codes + (size_t)unit * P::UNIT,
-                      P::UNIT, barrier(stage));
+            bulk_load(my_ring + stage * R::STAGE, codes + (size_t)unit * P::UNIT, P::UNIT, barrier(stage));
         if (turn == AHEAD / 2) units_next = look_up(asked + (AHEAD - AHEAD / 2) * WARPS);
         if (++turn == AHEAD) {
             turn = 0;
@@ -373,8 +375,8 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) lows[g][0] = lows[g][1] = 0.f;
 
-    // One tile: `held` its units, of which `live` are there; `first` its first key.
-    auto attend = [&](auto masked, const unsigned char* held, uint32_t live, int first) {
+    // One tile: `held` its units, `first` its first key, `some` whether a unit with keys to be seen has no page.
+    auto attend = [&](auto masked, const unsigned char* held, int first, bool some) {
         constexpr bool MASKED = decltype(masked)::value;
         // which of this lane's keys are seen: two bits a unit, r and r + 8
         uint32_t seen = 0;
@@ -382,7 +384,13 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
 #pragma unroll
             for (int i = 0; i < 2 * UNITS; ++i) {
                 const int key = first + 8 * i + r;
-                if ((live >> (i >> 1) & 1u) && key >= lowest_key && key <= position) seen |= 1u << i;
+                bool there = key >= lowest_key && key <= position;
+                if (some && there) {
+                    const int block = key >> page_shift;
+                    const int page = block < table_width ? table[block] : -1;
+                    there = page >= 0 && page < pages;
+                }
+                if (there) seen |= 1u << i;
             }
         }
         // scores (times log2 e), less what they are taken against
@@ -554,14 +562,13 @@ attention_packed_kernel(const T* q, const unsigned char* cache,
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const unsigned char* held = ring + stage * R::STAGE;
-        const uint32_t live = live_units >> (UNITS * stage) & EVERY;
         const int first = tile * KEYS;
-
         // (a tile whose keys are all seen needs no mask)
-        if (live == EVERY && first >= lowest_key && first + KEYS - 1 <= position)
-            attend(std::false_type{}, held, live, first);
+        const bool some = __any_sync(0xffffffffu, holes);
+        if (first >= lowest_key && first + KEYS - 1 <= position && !some)
+            attend(std::false_type{}, held, first, false);
         else
-            attend(std::true_type{}, held, live, first);
+            attend(std::true_type{}, held, first, some);
         stage = stage + 1 == R::STAGES ? 0 : stage + 1;
         if (stage == 0) parity ^= 1;
     }
@@ -776,6 +783,8 @@ MLXONE_API int mlxone_attention_packed(const void* q, const void* cache, const i
                    "attention_packed: %d splits need scratch", splits);
     MLXONE_REQUIRE(kv_heads * (long long)ceil_div_host(heads / kv_heads, HEADS) <= 65535,
                    "attention_packed: too many heads");
+    MLXONE_REQUIRE((long long)pages * kv_heads * (page_size / 16) <= 0x7fffffff,
+                   "attention_packed: a cache of more than 2^31 units of 16 tokens of a head");
     MLXONE_REQUIRE((((size_t)cache | (size_t)q) & 15) == 0,
                    "attention_packed: cache and queries start at multiples of 16 bytes");
     const int page_shift = 31 - __builtin_clz((unsigned)page_size);
