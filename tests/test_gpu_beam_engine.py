@@ -208,3 +208,55 @@ def test_beams_beside_requests(folders):
         assert [h.result().token_ids for h in handles] == want
         assert engine.cache_bytes_per_token() * 3.5 < sum(
             4 * need.kv_heads * need.head_dim for need in engine.model.cache_needs.values() if hasattr(need, "kv_heads"))
+
+
+ARCHITECTURES = [("galarax", "G1"), ("galarax", "G3"), ("galarax", "G5"), ("farorax", "F1"), ("farorax", "F6"),
+                 ("lamisun", "L1"), ("lamisun", "L4"), ("tirudra", "T1"), ("tirudra", "T5"), ("susalorn", None),
+                 ("zinizen", None)]
+
+
+def rescored(engine, prompt, tokens):
+    """The sum of the tokens' logarithms when prompt and tokens run through the step function at once."""
+    cache, runner = engine.cache, engine.runner
+    whole = list(prompt) + list(tokens)
+    cache.open("again")
+    logits = runner.step([StepEntry("again", whole[:-1], range(len(prompt) - 1, len(whole) - 1))])
+    cache.close("again")
+    logs = torch.log_softmax(logits.double(), -1)
+    return float(logs[torch.arange(len(tokens)), list(tokens)].sum())
+
+
+@pytest.mark.parametrize("bits", [None, 4])
+@pytest.mark.parametrize("family,name", ARCHITECTURES)
+def test_every_kind_of_state_follows_its_hypothesis(tmp_path, family, name, bits):
+    """Delta rules, lightning and latent attention, convolutions, state spaces, recurrences, hashes of neighbouring
+    tokens: a hypothesis has the score that its tokens get when they run at once, and one hypothesis is greedy
+    decoding. With 4 bits, models whose pages are keys and values of 32, 64, 96 or 128; others are refused."""
+    import importlib
+
+    module = importlib.import_module(family + "_models")
+    name = name or list(module.CONFIGS)[0]
+    config = module.CONFIGS[name][0]
+    folder = module.make_model_dir(name, tmp_path)
+    how = dict(execution_dtype="float32", cache_config=CacheConfig(block_size_tokens=16, capacity_tokens=2048,
+                                                                   max_requests=6, bits=bits),
+               batching_config=BatchingConfig(max_sequences=2, prefill_chunk_size=16))
+    try:
+        engine = Engine(folder, **how)
+    except ValueError as error:
+        assert bits == 4 and ("held in 4 bits" in str(error) or "32, 64, 96 or 128" in str(error))
+        return
+    vocab = engine.model.spec.vocab_size
+    (prompt,) = prompts(vocab, (37,), seed=3)
+    greedy = engine.generate_ids(prompt, max_tokens=12, ignore_eos=True).token_ids
+    found = engine.generate_beams_ids(prompt, max_tokens=12, ignore_eos=True, beams=1)
+    assert found[0].token_ids == greedy
+    found = engine.generate_beams_ids(prompt, max_tokens=20, ignore_eos=True, beams=min(4, vocab))
+    assert len({r.token_ids for r in found}) == len(found)
+    for result in found:
+        # 32 bits: 20 logarithms, each within the engine's 1e-4; 4 bits: a code may go either way between
+        # the two runs, by which a token's logarithm moves by a few 1e-3
+        assert abs(rescored(engine, prompt, result.token_ids) - result.score) <= (4e-3 if bits is None else 0.2), config
+    stats = engine.cache.stats()
+    assert stats.pages_free == stats.pages_total and stats.requests == 0
+    engine.close()
