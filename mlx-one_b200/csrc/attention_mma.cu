@@ -15,6 +15,7 @@
 //            memory and a second kernel merges the splits.
 //
 // Head sizes: multiples of 16 up to 128. Anything else runs the general kernel.
+#include <cuda_fp16.h>
 #include <cuda_pipeline_primitives.h>
 
 #include "common.cuh"
@@ -66,6 +67,15 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// the same with half-precision operands
+__device__ __forceinline__ void mma_half(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 // 2^x for x <= 0 (softmax weights): the hardware approximation, two units in the last place
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
@@ -75,6 +85,16 @@ __device__ __forceinline__ float fast_exp2(float x) {
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// A pair of weights as the second product takes them. HALF: values in half-precision, weights too, 2^15 times
+// what they are (the sum has the same factor), so that weights down to 2^-39 of the largest count.
+constexpr float HALF_RAISED = 15.f;
+template <bool HALF>
+__device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
+    if (!HALF) return pack_bf16(lo, hi);
+    const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
@@ -153,7 +173,7 @@ __device__ __forceinline__ void load_tile(bf16* k_tile, bf16* v_tile, const Page
 // Updates the running max `m` (of score * scale * log2 e), the sum `l` and `o`. With SHAPED the scores
 // pass `shape` first, the distance bias with slope `slope` (in units of log2 e) from the rows'
 // positions `at` on.
-template <int HD, int KEYS, bool MASKED, bool SHAPED>
+template <int HD, int KEYS, bool MASKED, bool SHAPED, bool HALF = false>
 __device__ __forceinline__ void attend_tile(const uint32_t (&qf)[HD / 16][4], const bf16* k_tile,
                                             const bf16* v_tile, int first, const int (&limit_lo)[2],
                                             const int (&limit_hi)[2], float scale_log2,
@@ -219,7 +239,8 @@ __device__ __forceinline__ void attend_tile(const uint32_t (&qf)[HD / 16][4], co
         m[i] = new_max;
     }
     float tile_sum[2] = {0.f, 0.f};
-    const float shift[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+    constexpr float RAISED = HALF ? HALF_RAISED : 0.f;
+    const float shift[2] = {(m[0] == -INFINITY ? 0.f : m[0]) - RAISED, (m[1] == -INFINITY ? 0.f : m[1]) - RAISED};
 #pragma unroll
     for (int j = 0; j < KEYS / 8; ++j)
 #pragma unroll
@@ -245,17 +266,22 @@ __device__ __forceinline__ void attend_tile(const uint32_t (&qf)[HD / 16][4], co
 #pragma unroll
     for (int kk = 0; kk < KEYS / 16; ++kk) {
         uint32_t a[4];
-        a[0] = pack_bf16(s[2 * kk][0], s[2 * kk][1]);
-        a[1] = pack_bf16(s[2 * kk][2], s[2 * kk][3]);
-        a[2] = pack_bf16(s[2 * kk + 1][0], s[2 * kk + 1][1]);
-        a[3] = pack_bf16(s[2 * kk + 1][2], s[2 * kk + 1][3]);
+        a[0] = pack_weights<HALF>(s[2 * kk][0], s[2 * kk][1]);
+        a[1] = pack_weights<HALF>(s[2 * kk][2], s[2 * kk][3]);
+        a[2] = pack_weights<HALF>(s[2 * kk + 1][0], s[2 * kk + 1][1]);
+        a[3] = pack_weights<HALF>(s[2 * kk + 1][2], s[2 * kk + 1][3]);
 #pragma unroll
         for (int nn = 0; nn < HD / 16; ++nn) {
             uint32_t b[4];
             ldmatrix_x4_trans(b, v_tile + (kk * 16 + r + (matrix & 1) * 8) * T::STRIDE + nn * 16 +
                                      (matrix >> 1) * 8);
-            mma_16816(o[2 * nn], a, b[0], b[1]);
-            mma_16816(o[2 * nn + 1], a, b[2], b[3]);
+            if (HALF) {
+                mma_half(o[2 * nn], a, b[0], b[1]);
+                mma_half(o[2 * nn + 1], a, b[2], b[3]);
+            } else {
+                mma_16816(o[2 * nn], a, b[0], b[1]);
+                mma_16816(o[2 * nn + 1], a, b[2], b[3]);
+            }
         }
     }
 }
@@ -265,14 +291,16 @@ __device__ __forceinline__ void attend_tile(const uint32_t (&qf)[HD / 16][4], co
 constexpr int PREFILL_WARPS = 4;       // 8 warps (128 rows) measured the same on long prompts
 constexpr int ROWS = 16 * PREFILL_WARPS;      // query rows per block
 
-template <int HD, bool SHAPED>
+// HALF: values in half-precision times a power of two of their request and key head, whose inverse
+// `value_factors` [requests, kv_heads] holds.
+template <int HD, bool SHAPED, bool HALF>
 __global__ void __launch_bounds__(PREFILL_WARPS * 32)
 attention_prefill_kernel(const bf16* __restrict__ q, const bf16* __restrict__ kv, long long kv_half,
                          const int* __restrict__ block_table, int table_width, int page_size,
                          const int* __restrict__ request_start, const int* __restrict__ history,
                          bf16* __restrict__ out, int requests, int heads, int kv_heads,
                          float scale_log2, int window, const float* __restrict__ sinks,
-                         int keep_first, ScoreShape shape) {
+                         int keep_first, ScoreShape shape, const float* __restrict__ value_factors) {
     using T = Tile<HD>;
     constexpr int KEYS = PREFILL_KEYS;
     extern __shared__ __align__(16) unsigned char shared_bytes[];
@@ -352,7 +380,7 @@ attention_prefill_kernel(const bf16* __restrict__ q, const bf16* __restrict__ kv
         // a sink is a term exp(sink) of the denominator without a key or a value: the softmax
         // starts from it (maximum in units of log2, sum 1, output 0)
         m[0] = m[1] = sinks[head] * LOG2E;
-        l[0] = l[1] = 1.f;
+        l[0] = l[1] = HALF ? 32768.f : 1.f;
     }
     float o[HD / 8][4];
 #pragma unroll
@@ -397,10 +425,10 @@ attention_prefill_kernel(const bf16* __restrict__ q, const bf16* __restrict__ kv
             const bool open = warp_whole && tile * KEYS >= open_lo &&
                               tile * KEYS + KEYS - 1 <= warp_first;
             if (open)
-                attend_tile<HD, KEYS, false, SHAPED>(qf, k_now, v_now, tile * KEYS, limit_lo, limit_hi,
+                attend_tile<HD, KEYS, false, SHAPED, HALF>(qf, k_now, v_now, tile * KEYS, limit_lo, limit_hi,
                                                      scale_log2, m, l, o, lane, 0, shape, slope, at);
             else
-                attend_tile<HD, KEYS, true, SHAPED>(qf, k_now, v_now, tile * KEYS, limit_lo, limit_hi,
+                attend_tile<HD, KEYS, true, SHAPED, HALF>(qf, k_now, v_now, tile * KEYS, limit_lo, limit_hi,
                                                     scale_log2, m, l, o, lane, keep_first, shape, slope,
                                                     at);
         }
@@ -411,7 +439,8 @@ attention_prefill_kernel(const bf16* __restrict__ q, const bf16* __restrict__ kv
     for (int i = 0; i < 2; ++i) {
         const int row = warp * 16 + (lane >> 2) + i * 8;
         if (row >= rows) continue;
-        const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
+        float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
+        if (HALF) inv *= value_factors[(size_t)request * kv_heads + head / (heads / kv_heads)];
         bf16* dst = out + ((size_t)(first_token + row_start + row) * heads + head) * HD +
                     (lane & 3) * 2;
 #pragma unroll
@@ -974,22 +1003,22 @@ __global__ void attention_merge_kernel(const float* __restrict__ partial, bf16* 
     }
 }
 
-template <int HD, bool SHAPED = false>
+template <int HD, bool SHAPED = false, bool HALF = false>
 int launch_prefill(const void* q, const void* kv, long long kv_half, const int* block_table,
                    int table_width, int page_size, const int* request_start, const int* history,
                    void* out, int tokens, int requests, int heads, int kv_heads, float scale,
                    int window, const float* sinks, cudaStream_t stream, int keep_first = 0,
-                   ScoreShape shape = ScoreShape()) {
+                   ScoreShape shape = ScoreShape(), const float* value_factors = nullptr) {
     using T = Tile<HD>;
     const size_t shared = (size_t)(ROWS + 4 * PREFILL_KEYS) * T::STRIDE * 2;
-    auto kernel = attention_prefill_kernel<HD, SHAPED>;
+    auto kernel = attention_prefill_kernel<HD, SHAPED, HALF>;
     if (shared > 48 * 1024)
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
     const dim3 grid((tokens + ROWS - 1) / ROWS + requests, heads);
     kernel<<<grid, PREFILL_WARPS * 32, shared, stream>>>(
         (const bf16*)q, (const bf16*)kv, kv_half, block_table, table_width, page_size,
         request_start, history, (bf16*)out, requests, heads, kv_heads, scale * LOG2E, window,
-        sinks, keep_first, shape);
+        sinks, keep_first, shape, value_factors);
     return 0;
 }
 
@@ -1226,6 +1255,39 @@ MLXONE_API int mlxone_attention_decode_shaped(const void* q, const void* kv, con
     MLXONE_HEAD_DIMS(CALL)
 #undef CALL
     MLXONE_LAUNCH_CHECK("attention_decode");
+    return 0;
+}
+
+// As mlxone_attention_prefill over values in half-precision, which are their values times the inverse of
+// value_factors [requests, kv_heads], a power of two; with a window, the first keep_first positions of a
+// sequence stay visible. Heads of 32, 64, 96 or 128 values.
+MLXONE_API int mlxone_attention_prefill_half(const void* q, const void* kv, const int* block_table,
+                                             int table_width, int page_size, int pages,
+                                             const int* request_start, const int* history, void* out,
+                                             int tokens, int requests, int heads, int kv_heads,
+                                             int head_dim, float scale, int window, int keep_first,
+                                             const float* sinks, const float* value_factors,
+                                             cudaStream_t stream) {
+    if (tokens == 0) return 0;
+    MLXONE_REQUIRE(tokens > 0 && requests > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 &&
+                       heads <= 65535 && value_factors != nullptr, "attention_prefill: bad sizes");
+    MLXONE_REQUIRE(page_size > 0 && pages > 0 && table_width > 0,
+                   "attention_prefill: bad page geometry");
+    const long long kv_half = (long long)pages * kv_heads * page_size * head_dim;
+#define CALL(HD)                                                                               \
+    launch_prefill<HD, false, true>(q, kv, kv_half, block_table, table_width, page_size,       \
+                                    request_start, history, out, tokens, requests, heads,      \
+                                    kv_heads, scale, window, sinks, stream, keep_first,        \
+                                    ScoreShape(), value_factors)
+    switch (head_dim) {
+        case 32: CALL(32); break;
+        case 64: CALL(64); break;
+        case 96: CALL(96); break;
+        case 128: CALL(128); break;
+        default: mlxone_set_error("attention_prefill: no half-precision values for heads of %d", head_dim); return 1;
+    }
+#undef CALL
+    MLXONE_LAUNCH_CHECK("attention_prefill");
     return 0;
 }
 

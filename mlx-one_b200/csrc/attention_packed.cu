@@ -162,12 +162,6 @@ __device__ __forceinline__ void expand_small(uint32_t word, uint32_t (&pair)[4])
 }
 constexpr float CODE_UNIT = 16777216.f;                // 2^24
 
-// 2^(to - floor(log2 x)) for x > 0, and its inverse; x is taken for 2^-113 at least
-__device__ __forceinline__ float power_towards(float x, int to, float& inverse) {
-    const int exponent = max((int)(__float_as_uint(x) >> 23 & 255u), 14);
-    inverse = __uint_as_float((uint32_t)(exponent - to) << 23);
-    return __uint_as_float((uint32_t)(254 - (exponent - to)) << 23);
-}
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);

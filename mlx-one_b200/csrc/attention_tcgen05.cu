@@ -37,6 +37,7 @@
 // Every wait on an mbarrier gives up after a bounded number of polls, raises the error flag
 // (code 9) and lets the block run to its end, where tensor memory is given back.
 #include <cuda.h>
+#include <cuda_fp16.h>
 
 #include "common.cuh"
 #include "float_pairs.cuh"
@@ -210,6 +211,13 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+template <bool HALF>
+__device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
+    if (!HALF) return pack_bf16(lo, hi);
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 // Shared-memory operand descriptor for tiles whose rows are 128 bytes, swizzled in atoms of 8
 // rows x 128 bytes that follow one another every 1024 bytes: start address, stride between
 // atoms, version 1, swizzle mode 2 (128 bytes). It serves K-major operands (rows = M or N, 64
@@ -223,9 +231,9 @@ __device__ __forceinline__ uint64_t operand_descriptor(uint32_t address) {
     d |= (uint64_t)2 << 61;
     return d;
 }
-// float32 accumulator, bfloat16 operands, A K-major; B K-major or MN-major; N and M.
-__host__ __device__ constexpr uint32_t instruction_descriptor(int m, int n, bool b_mn_major) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) |
+// float32 accumulator, bfloat16 (or half-precision) operands, A K-major; B K-major or MN-major; N and M.
+__host__ __device__ constexpr uint32_t instruction_descriptor(int m, int n, bool b_mn_major, bool half = false) {
+    return (1u << 4) | (half ? 0u : (1u << 7) | (1u << 10)) | ((b_mn_major ? 1u : 0u) << 16) |
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
@@ -335,7 +343,11 @@ __device__ __forceinline__ void shape_tile(float (&v)[N], const ScoreShape& shap
     }
 }
 
-template <int KEYS, int PARTS, bool SHAPED>
+// HALF: values are half-precision and times a power of two of their request and key head, whose inverse
+// `value_factors` [requests, kv_heads] holds (the output is multiplied by it); the weights are then
+// half-precision too, 2^7 times what they are otherwise (at most 2^15; the sum has the same factor), so that
+// weights down to 2^-31 of the largest count.
+template <int KEYS, int PARTS, bool SHAPED, bool HALF>
 __global__ void __launch_bounds__((4 * PARTS + 2) * 32, Shape<KEYS>::BLOCKS_PER_SM)
 attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q,
                          const __grid_constant__ CUtensorMap map_kv, long long value_rows,
@@ -344,8 +356,10 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q,
                          const int* __restrict__ history, bf16* __restrict__ out, int requests,
                          int heads, int kv_heads, float scale_log2, int window, int token_tiles,
                          int splits, float* __restrict__ partial, const float* __restrict__ sinks,
-                         int* __restrict__ error_flag, int keep_first, ScoreShape shape) {
+                         int* __restrict__ error_flag, int keep_first, ScoreShape shape,
+                         const float* __restrict__ value_factors) {
     using S = Shape<KEYS>;
+    constexpr float RAISED = HALF ? 7.f : 0.f;
     constexpr int COPY_WARP = 4 * PARTS, MMA_WARP = 4 * PARTS + 1;
     constexpr int THREADS = (4 * PARTS + 2) * 32;     // softmax warps, the copy warp, the product warp
     constexpr int Q_BUFFERS = S::Q_BUFFERS, K_BYTES = S::K_BYTES, STAGE_BYTES = S::STAGE_BYTES;
@@ -516,7 +530,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q,
     } else if (warp == MMA_WARP) {
         if (lane == 0) {
             constexpr uint32_t idesc_scores = instruction_descriptor(ROWS, KEYS, false);
-            constexpr uint32_t idesc_out = instruction_descriptor(ROWS, HD, true);
+            constexpr uint32_t idesc_out = instruction_descriptor(ROWS, HD, true, HALF);
             // a place in the walk: item n, its tile j; `taken` and `t` as above
             struct Place { int n, j, taken, t; };
             auto settle = [&](Place& place) {          // skips items without work
@@ -688,7 +702,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q,
                     tmem_store<MY_DIMS>(my_out, sofar);
                 }
                 if (follow) m = running;
-                const float shift = m == -INFINITY ? 0.f : m;
+                const float shift = (m == -INFINITY ? 0.f : m) - RAISED;
                 unsigned long long partial[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
                 const unsigned long long scale_pair = pair_of(scale_log2, scale_log2);
                 const unsigned long long shift_pair = pair_of(-shift, -shift);
@@ -707,10 +721,10 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q,
                         partial[(i >> 1) & 1] = add_pair(partial[(i >> 1) & 1], pair_of(p[i], p[i + 1]));
                     }
                     uint4 packed;
-                    packed.x = pack_bf16(p[0], p[1]);
-                    packed.y = pack_bf16(p[2], p[3]);
-                    packed.z = pack_bf16(p[4], p[5]);
-                    packed.w = pack_bf16(p[6], p[7]);
+                    packed.x = pack_weights<HALF>(p[0], p[1]);
+                    packed.y = pack_weights<HALF>(p[2], p[3]);
+                    packed.z = pack_weights<HALF>(p[4], p[5]);
+                    packed.w = pack_weights<HALF>(p[6], p[7]);
                     // 16-byte piece `at` of the row: block at / 8 of 64 keys, swizzled within it
                     const int at = (part * MY_KEYS) / 8 + piece;
                     *reinterpret_cast<uint4*>(p_tile_row + (at >> 3) * (ROWS * 128) +
@@ -750,8 +764,13 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q,
                 // against (every part holds the same m and, by now, the same l); a row that saw
                 // no key in this split is left with the sink alone. Counted once: by split 0.
                 const float sink = sinks[item.kv_head * group + row % group] * 1.4426950408889634f;
-                if (m == -INFINITY) { m = sink; l = 1.f; }
-                else l += fast_exp2(fminf(sink - m, 126.f));
+                if (m == -INFINITY) { m = sink; l = HALF ? 128.f : 1.f; }
+                else l += fast_exp2(fminf(sink - m + RAISED, 126.f));
+            }
+            if (HALF) {
+                const float factor = value_factors[(size_t)item.request * kv_heads + item.kv_head];
+#pragma unroll
+                for (int d = 0; d < MY_DIMS; ++d) o[d] *= factor;
             }
             if (ok && valid && split_row != nullptr) {
                 // unnormalised, against m: the merge scales the splits to their common maximum
@@ -895,7 +914,8 @@ static int prefill_tcgen05(const void* q, const void* kv, const int* block_table
                                                 int kv_heads, int head_dim, float scale, int window,
                                                 int splits, float* partial, const float* sinks,
                                                 int keys, int* error_flag, cudaStream_t stream, int keep_first,
-                                                bool shaped = false, ScoreShape shape = ScoreShape()) {
+                                                bool shaped = false, ScoreShape shape = ScoreShape(),
+                                                const float* value_factors = nullptr) {
     if (tokens == 0) return 0;
     MLXONE_REQUIRE(keep_first >= 0 && (keep_first == 0 || window > 0),
                    "attention_prefill_tcgen05: first positions are kept behind a window only");
@@ -954,8 +974,12 @@ static int prefill_tcgen05(const void* q, const void* kv, const int* block_table
     if ((all_items + blocks - 1) / blocks > MAX_ITEMS) blocks = (all_items + MAX_ITEMS - 1) / MAX_ITEMS;
     const int shared = small_tiles ? Shape<64>::SHARED_BYTES : Shape<128>::SHARED_BYTES;
     const int threads = ((small_tiles ? 1 : 2) * 4 + 2) * 32;
-    auto kernel = shaped ? (small_tiles ? attention_tcgen05_kernel<64, 1, true> : attention_tcgen05_kernel<128, 2, true>)
-                         : (small_tiles ? attention_tcgen05_kernel<64, 1, false> : attention_tcgen05_kernel<128, 2, false>);
+    auto kernel = shaped ? (small_tiles ? attention_tcgen05_kernel<64, 1, true, false>
+                                        : attention_tcgen05_kernel<128, 2, true, false>)
+                  : value_factors != nullptr ? (small_tiles ? attention_tcgen05_kernel<64, 1, false, true>
+                                                            : attention_tcgen05_kernel<128, 2, false, true>)
+                                             : (small_tiles ? attention_tcgen05_kernel<64, 1, false, false>
+                                                            : attention_tcgen05_kernel<128, 2, false, false>);
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
     if (err != cudaSuccess) {
         mlxone_set_error("attention_prefill_tcgen05: %s", cudaGetErrorString(err));
@@ -964,7 +988,7 @@ static int prefill_tcgen05(const void* q, const void* kv, const int* block_table
     kernel<<<dim3((unsigned)blocks), threads, shared, stream>>>(
         map_q, map_kv, value_rows, block_table, table_width, page_size, box_keys, request_start,
         history, static_cast<bf16*>(out), requests, heads, kv_heads, scale * 1.4426950408889634f,
-        window, token_tiles, splits, partial, sinks, error_flag, keep_first, shape);
+        window, token_tiles, splits, partial, sinks, error_flag, keep_first, shape, value_factors);
     MLXONE_LAUNCH_CHECK("attention_prefill_tcgen05");
     return 0;
 }
@@ -994,6 +1018,23 @@ MLXONE_API int mlxone_attention_prefill_tcgen05_keep(const void* q, const void* 
     return prefill_tcgen05(q, kv, block_table, table_width, page_size, pages, request_start, history,
                            out, tokens, requests, heads, kv_heads, head_dim, scale, window, splits,
                            partial, sinks, keys, error_flag, stream, keep_first);
+}
+
+// ... over keys in bfloat16 and values in half-precision, which are their values times the inverse of
+// value_factors [requests, kv_heads], a power of two (both planes have rows of 128 bytes)
+MLXONE_API int mlxone_attention_prefill_tcgen05_half(const void* q, const void* kv, const int* block_table,
+                                                     int table_width, int page_size, int pages,
+                                                     const int* request_start, const int* history, void* out,
+                                                     int tokens, int requests, int heads, int kv_heads,
+                                                     int head_dim, float scale, int window, int keep_first,
+                                                     int splits, float* partial, const float* sinks, int keys,
+                                                     const float* value_factors, int* error_flag,
+                                                     cudaStream_t stream) {
+    MLXONE_REQUIRE(value_factors != nullptr, "attention_prefill_tcgen05: values without their factors");
+    return prefill_tcgen05(q, kv, block_table, table_width, page_size, pages, request_start, history,
+                           out, tokens, requests, heads, kv_heads, head_dim, scale, window, splits,
+                           partial, sinks, keys, error_flag, stream, keep_first, false, ScoreShape(),
+                           value_factors);
 }
 
 // ... with scores s that become cap tanh(s / cap) (cap 0: none) and then lose slopes[head] (float32

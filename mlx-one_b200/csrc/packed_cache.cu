@@ -5,6 +5,8 @@
 // difference and quotient in 32 bits), code = (x - lowest) / step to the nearest whole number, ties to
 // even, cut to 0..15. The codes are those of exact arithmetic on the stored lowest and step (codes_of). A group
 // with a value that is not finite, or whose range is none, gets NaN as step and lowest: it stays visible.
+#include <cuda_fp16.h>
+
 #include "packed_cache.cuh"
 
 namespace {
@@ -298,17 +300,63 @@ read_kernel(const unsigned char* cache, const int* positions,
     }
 }
 
+// The largest value (of the values' part, by its size) that 1,024 keys of a request and key head may open to:
+// largest [requests, open heads, chunks].
+constexpr int CHUNK_UNITS = 64;
+
+template <int HD>
+__global__ void __launch_bounds__(256)
+value_range_kernel(const unsigned char* cache, const int* block_table, int table_width, int page_shift, int pages,
+                   const int* request_start, const int* history, int span, int first_request, int first_head,
+                   int kv_heads, float* largest) {
+    using P = Packed<HD>;
+    __shared__ float scratch[33];
+    griddep_launch();
+    griddep_wait();
+    const unsigned char* from = settled(cache);
+    const int chunk = blockIdx.x, head = first_head + blockIdx.y, request = first_request + blockIdx.z;
+    const int held = history[request];
+    const int length = held + request_start[request + 1] - request_start[request];
+    const int lowest_key = first_visible_key(held, span), units = 1 << (page_shift - 4);
+    float most = 0.f;
+#pragma unroll
+    for (int i = threadIdx.x; i < CHUNK_UNITS * 16; i += 256) {
+        const int first = (chunk * CHUNK_UNITS + i / 16) * 16, place = i % 16;
+        if (first + place / 2 + 8 * (place & 1) >= length || first + 15 < lowest_key) continue;
+        const int block = first >> page_shift;
+        const int page = block < table_width ? block_table[(size_t)request * table_width + block] : -1;
+        if (page < 0 || page >= pages) continue;
+        const unsigned char* part =
+            from + (((size_t)page * kv_heads + head) * units + (first >> 4 & (units - 1))) * P::UNIT + P::PART;
+#pragma unroll
+        for (int g = 0; g < P::GROUPS; ++g) {
+            const uint32_t word = *reinterpret_cast<const uint32_t*>(part + P::CODES + 64 * g + 4 * place);
+            const float lowest = packed_lowest(word);
+            // (what is no number counts as nothing)
+            most = fmaxf(most, fmaxf(fabsf(lowest), fabsf(fmaf(15.f, packed_step(word), lowest))));
+        }
+    }
+    most = block_max(most, scratch);
+    if (threadIdx.x == 0) largest[((size_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + chunk] = most;
+}
+
 // Requests opened: every unit that the requests' tables name, up to their last token, as plain values in
 // pages [2, requests * blocks, open_heads, open_size, HD] of their own, request r's block b in page r * blocks
 // + b, of the key heads from first_head on; rows behind the last token, and of units without a page, are zeros,
-// so that no reader meets a number that is none. `table` gets those page numbers and, behind them, where the
-// requests' tokens start, counted from the first one's. A thread takes a run of four keys, 2j, 2j + 1, 2j + 8 and 2j + 9: every byte of its eight words is theirs, of the keys' part as of the
-// values'.
+// so that no reader meets a number that is none. A token whose keys or values are none has NaN for its keys and
+// zeros for its values: queries that see it get NaN by their scores, the others nothing, since a reader drops
+// scores that are masked but multiplies every value. `table` gets the page numbers and, behind them, where the
+// requests' tokens start, counted from the first one's. With `largest` (value_range_kernel's, `chunks` of them
+// each) values are half-precision, times the power of two that brings the largest of a request and key head to
+// 2^9, whose inverse goes to `factors` [requests, open heads]: 11 bits of every value of 2^-23 of the largest and
+// more, where bfloat16 has 8. A thread takes a run of four keys, 2j, 2j + 1, 2j + 8 and 2j + 9: every byte of its
+// eight words is theirs, of the keys' part as of the values'.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256)
 open_kernel(const unsigned char* cache, const int* block_table, int table_width, int page_shift, int pages,
             const int* request_start, const int* history, int span, int first_request, int first_head, int kv_heads,
-            int blocks, int open_size, long long half, T* opened, int* table) {
+            int blocks, int open_size, long long half, T* opened, int* table, const float* largest, int chunks,
+            float* factors) {
     using P = Packed<HD>;
     constexpr int THREADS = 8 * P::RUNS;                         // of a unit
     griddep_launch();
@@ -321,6 +369,14 @@ open_kernel(const unsigned char* cache, const int* block_table, int table_width,
     const int per_block = open_size / 16;
     const int inside = threadIdx.x % THREADS;
     const int unit = blockIdx.x * (blockDim.x / THREADS) + threadIdx.x / THREADS;
+    float raise = 1.f;
+    if (largest != nullptr) {
+        const float* mine = settled(largest) + ((size_t)r * gridDim.y + open_head) * chunks;
+        float most = 0.f, inverse;
+        for (int i = threadIdx.x & 31; i < chunks; i += 32) most = fmaxf(most, mine[i]);
+        raise = power_towards(warp_max(most), 9, inverse);
+        if (blockIdx.x == 0 && threadIdx.x == 0) factors[(size_t)r * gridDim.y + open_head] = inverse;
+    }
     if (unit >= blocks * per_block) return;
     const int open_block = unit / per_block;
     if (open_head == 0 && inside == 0 && unit % per_block == 0) {
@@ -354,13 +410,28 @@ open_kernel(const unsigned char* cache, const int* block_table, int table_width,
             words[k] = *reinterpret_cast<const uint32_t*>(
                 part + P::word_at(which ? 4 * k + j : 4 * (2 * j + k / 4) + k % 4, s));
         // (the words of keys 2j, 2j + 8, 2j + 1, 2j + 9 lie side by side)
-        const uint4 scale = *reinterpret_cast<const uint4*>(part + P::scale_at(2 * j, s * 16 / P::GROUP));
-        const uint32_t of_key[4] = {scale.x, scale.z, scale.y, scale.w};
+        uint32_t none = 0;
+#pragma unroll
+        for (int g = 0; g < 2 * P::GROUPS; ++g) {
+            const uint4 scale = *reinterpret_cast<const uint4*>(part + (g % 2 - which) * P::PART + P::scale_at(2 * j, g / 2));
+            const uint32_t of_key[4] = {scale.x, scale.z, scale.y, scale.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (!isfinite(packed_step(of_key[k]))) none |= 1u << k;
+                if (g == 2 * (s * 16 / P::GROUP) + which) {
+                    step[k] = packed_step(of_key[k]);
+                    lowest[k] = packed_lowest(of_key[k]);
+                }
+            }
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int key = first + 2 * j + (k & 1) + 8 * (k >> 1);
-            step[k] = key < length ? packed_step(of_key[k]) : 0.f;
-            lowest[k] = key < length ? packed_lowest(of_key[k]) : 0.f;
+            const bool is_none = none >> k & 1u;
+            if (key >= length || is_none) step[k] = 0.f;
+            if (key >= length || is_none) lowest[k] = key < length && !which ? NAN : 0.f;
+            step[k] *= which ? raise : 1.f;
+            lowest[k] *= which ? raise : 1.f;
         }
     }
     T* to = opened + which * half + (((size_t)r * blocks + open_block) * gridDim.y + open_head) * open_size * HD +
@@ -377,7 +448,19 @@ open_kernel(const unsigned char* cache, const int* block_table, int table_width,
             x[e] = fmaf(step[k], (float)(both & 15u), lowest[k]);
             x[e + 8] = fmaf(step[k], (float)(both >> 4 & 15u), lowest[k]);
         }
-        store_run(to + (2 * j + (k & 1) + 8 * (k >> 1)) * HD, x);
+        T* row = to + (2 * j + (k & 1) + 8 * (k >> 1)) * HD;
+        if (sizeof(T) == 2 && which && largest != nullptr) {
+            uint32_t pairs[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const __half2 pair = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+                pairs[e] = *reinterpret_cast<const uint32_t*>(&pair);
+            }
+            *reinterpret_cast<uint4*>(row) = make_uint4(pairs[0], pairs[1], pairs[2], pairs[3]);
+            *reinterpret_cast<uint4*>(row + 8) = make_uint4(pairs[4], pairs[5], pairs[6], pairs[7]);
+        } else {
+            store_run(row, x);
+        }
     }
 }
 
@@ -455,35 +538,58 @@ MLXONE_API int mlxone_read_key_values(const void* cache, const int* positions, c
     return 0;
 }
 
+// Floats that mlxone_open_key_values needs as `factors` for half-precision values.
+MLXONE_API long long mlxone_open_factors(int requests, int open_heads, int blocks, int open_size) {
+    if (requests <= 0 || open_heads <= 0 || blocks <= 0 || open_size <= 0) return 0;
+    return (long long)requests * open_heads * (1 + ceil_div_host((long long)blocks * open_size, 16 * CHUNK_UNITS));
+}
+
 // Requests first_request.. (`requests` of them) and key heads first_head.. (`open_heads` of kv_heads), `blocks`
 // pages of `open_size` tokens (a multiple of 16) for each request: opened [2, requests * blocks, open_heads,
-// open_size, head_dim], table int32 [requests * blocks + requests + 1]. `span`: see first_visible_key; units that no token of the
-// step sees are zeros.
+// open_size, head_dim], table int32 [requests * blocks + requests + 1]. `span`: see first_visible_key; units that
+// no token of the step sees are zeros. factors: null, or (bfloat16) mlxone_open_factors floats: values are then
+// half-precision, and the first requests * open_heads of them are what they are to be multiplied by.
 MLXONE_API int mlxone_open_key_values(const void* cache, const int* block_table, int table_width, int page_size,
                                       int pages, const int* request_start, const int* history, int span,
                                       int first_request, int requests, int kv_heads, int first_head,
-                                      int open_heads, int head_dim, int blocks, int open_size, void* opened, int* table, int dtype, cudaStream_t stream) {
+                                      int open_heads, int head_dim, int blocks, int open_size, void* opened,
+                                      int* table, float* factors, int dtype, cudaStream_t stream) {
     if (requests == 0) return 0;
     if (check_geometry("open_key_values", head_dim, page_size, pages, kv_heads, table_width, cache)) return 1;
     MLXONE_REQUIRE(requests > 0 && requests <= 65535 && first_request >= 0 && blocks > 0 && open_size >= 16 &&
                        open_size % 16 == 0 && first_head >= 0 && open_heads > 0 &&
                        first_head + open_heads <= kv_heads, "open_key_values: bad sizes");
-    const long long half = (long long)requests * blocks * open_heads * open_size * head_dim;
-    const int per = 256 / (head_dim / 2);         // units of a block (8 RUNS = head_dim / 2 threads a unit)
+    MLXONE_REQUIRE(factors == nullptr || dtype == MLXONE_BF16, "open_key_values: half-precision values beside bfloat16 keys");
     MLXONE_REQUIRE(((size_t)opened & 15) == 0, "open_key_values: the output starts at a multiple of 16 bytes");
-    const dim3 grid(ceil_div_host((long long)blocks * (open_size / 16), per), open_heads, requests);
+    const long long half = (long long)requests * blocks * open_heads * open_size * head_dim;
     const int page_shift = 31 - __builtin_clz((unsigned)page_size);
+    const int chunks = ceil_div_host((long long)blocks * open_size, 16 * CHUNK_UNITS);
+    const unsigned char* held = (const unsigned char*)cache;
+    float* largest = nullptr;
+    if (factors != nullptr) {
+        largest = factors + (size_t)requests * open_heads;
+#define CALL(HD)                                                                                          \
+    launch_kernel(value_range_kernel<HD>, dim3(chunks, open_heads, requests), dim3(256), 0, stream, true, \
+                  held, block_table, table_width, page_shift, pages, request_start, history, span,        \
+                  first_request, first_head, kv_heads, largest)
+        MLXONE_PACKED_DIMS(CALL)
+#undef CALL
+        MLXONE_LAUNCH_CHECK("open_key_values range");
+    }
+    // units of a block (8 RUNS = head_dim / 2 threads a unit), whole warps
+    const int per = head_dim == 96 ? 4 : 512 / head_dim;
+    const dim3 grid(ceil_div_host((long long)blocks * (open_size / 16), per), open_heads, requests);
 #define CALL(HD)                                                                                          \
     if (dtype == MLXONE_BF16)                                                                             \
-        launch_kernel(open_kernel<bf16, HD>, grid, dim3(per * HD / 2), 0, stream, true,                       \
-                      (const unsigned char*)cache, block_table, table_width, page_shift, pages,           \
-                      request_start, history, span, first_request, first_head, kv_heads, blocks, open_size, half,     \
-                      (bf16*)opened, table);                                                              \
+        launch_kernel(open_kernel<bf16, HD>, grid, dim3(per * HD / 2), 0, stream, true, held,             \
+                      block_table, table_width, page_shift, pages, request_start, history, span,          \
+                      first_request, first_head, kv_heads, blocks, open_size, half, (bf16*)opened, table, \
+                      (const float*)largest, chunks, factors);                                            \
     else                                                                                                  \
-        launch_kernel(open_kernel<float, HD>, grid, dim3(per * HD / 2), 0, stream, true,                      \
-                      (const unsigned char*)cache, block_table, table_width, page_shift, pages,           \
-                      request_start, history, span, first_request, first_head, kv_heads, blocks, open_size, half,     \
-                      (float*)opened, table)
+        launch_kernel(open_kernel<float, HD>, grid, dim3(per * HD / 2), 0, stream, true, held,            \
+                      block_table, table_width, page_shift, pages, request_start, history, span,          \
+                      first_request, first_head, kv_heads, blocks, open_size, half, (float*)opened,       \
+                      table, (const float*)nullptr, chunks, (float*)nullptr)
     MLXONE_PACKED_DIMS(CALL)
 #undef CALL
     MLXONE_LAUNCH_CHECK("open_key_values");

@@ -59,6 +59,13 @@ struct Packed {
 __device__ __forceinline__ float packed_step(uint32_t word) { return __uint_as_float(word << 16); }
 __device__ __forceinline__ float packed_lowest(uint32_t word) { return __uint_as_float(word & 0xffff0000u); }
 
+// 2^(to - floor(log2 x)) for x > 0, and its inverse; x is taken for 2^-113 at least
+__device__ __forceinline__ float power_towards(float x, int to, float& inverse) {
+    const int exponent = max((int)(__float_as_uint(x) >> 23 & 255u), 14);
+    inverse = __uint_as_float((uint32_t)(exponent - to) << 23);
+    return __uint_as_float((uint32_t)(254 - (exponent - to)) << 23);
+}
+
 #define MLXONE_PACKED_DIMS(CALL)                                                                  \
     switch (head_dim) {                                                                           \
         case 32: CALL(32); break;                                                                 \

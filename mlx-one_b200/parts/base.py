@@ -77,6 +77,15 @@ class PackedView:
     need: PagedKeyValues
 
 
+@dataclass
+class OpenedView(PagedView):
+    """Pages that were opened from packed ones for one call: keys in bfloat16, and values in
+    half-precision (in the same storage, by their bits) that are to be multiplied by ``factors``
+    (float32 [requests, kv_heads], powers of two)."""
+
+    factors: torch.Tensor | None = None
+
+
 def packed_part_bytes(head_dim: int) -> int:
     """Bytes of the keys (or values) of 16 tokens of one head, held in 4 bits: the codes, and a step
     and a lowest value in bfloat16 for every 64 values of a token (32 where 64 do not divide the

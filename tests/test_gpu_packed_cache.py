@@ -347,3 +347,52 @@ def test_shaped_scores_over_packed_pages(ops):
                 # (both within 2^-8 of a weight and of the result, values below 4.2)
                 torch.testing.assert_close(got.float(), want.float(), atol=0.07 if dtype == BF16 else 1e-4, rtol=0)
     ops.check_errors()
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (96, 32), (128, 64), (32, 16)])
+@pytest.mark.parametrize("size", [1e-30, 1.0, 2e4, 1e30])
+def test_portions_of_values_of_any_size(ops, dim, page, size):
+    """Values that half-precision by itself could not hold: opened times a power of two of their request and head."""
+    portions, histories = [40, 21], [30, 100]
+    ctx, table, kv, view = packed_case(2, dim, page, portions, [0, 0], BF16, stale=0)
+    whole, _, _ = make_batch([70, 121], [0, 0], page, DEVICE)
+    ctx, table, pages = make_batch(portions, histories, page, DEVICE)
+    view = PackedView(torch.full((pages, 2, page // 16, 2, plain.part_bytes(dim)), 0xFF, dtype=torch.uint8, device=DEVICE),
+                      table, page, PagedKeyValues(2, dim))
+    keys = rows_of(191, 2, dim, BF16, 3, 0.3)
+    values = rows_of(191, 2, dim, F32, 4, 0.3)
+    values[:, 1] *= 1e3                                       # a head's values are its own matter
+    values = (values * size).to(BF16)
+    ops.pack_key_values(keys.view(191, -1).to(DEVICE), values.view(191, -1).to(DEVICE), ctx=whole, view=view)
+    q = torch.randn(61, 4, dim, generator=torch.Generator().manual_seed(1)).to(BF16)
+    got = ops.paged_attention(q.to(DEVICE), heads=4, kv_heads=2, head_dim=dim, scale=dim ** -0.5, window=None, ctx=ctx,
+                              view=view).view(61, 4, dim).cpu().double()
+    want = plain.attend(q, view.kv.cpu(), table.cpu(), page, portions, histories, 4, 2, dim ** -0.5)
+    t = 0
+    for r, (n, held) in enumerate(zip(portions, histories)):
+        both = plain.read(view.kv.cpu(), table.cpu(), page, r, held + n, dim)
+        for h in range(2):
+            bound = bound_of(both[:, :, h], q[t:t + n], dim ** -0.5, dim, BF16, held + n)["portion"]
+            assert (got[t:t + n, 2 * h:2 * h + 2] - want[t:t + n, 2 * h:2 * h + 2]).abs().max() <= bound, (r, h)
+        t += n
+    ops.check_errors()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dim,window", [(64, 0), (96, 0), (128, 30), (64, 50)])
+@pytest.mark.parametrize("of_values", [False, True])
+def test_what_is_not_a_number_in_a_portion(ops, dtype, dim, window, of_values):
+    """Queries ahead of a key that is none, other heads' and other requests' get their numbers; the ones that see it do not."""
+    ctx, table, kv, view = packed_case(2, dim, 16, [60, 20], [0, 0], dtype, stale=0)
+    keys, values = rows_of(80, 2, dim, dtype, 1, 0.3), rows_of(80, 2, dim, dtype, 2, 0.3)
+    (values if of_values else keys)[17, 1, 5] = math.nan
+    ops.pack_key_values(keys.view(80, -1).to(DEVICE), values.view(80, -1).to(DEVICE), ctx=ctx, view=view)
+    q = torch.randn(80, 6, dim, device=DEVICE).to(dtype)
+    got = ops.paged_attention(q, heads=6, kv_heads=2, head_dim=dim, scale=dim ** -0.5, window=window or None, ctx=ctx,
+                              view=view).view(80, 6, dim)
+    spoilt = torch.isnan(got).any(-1).cpu()
+    sees = torch.zeros(80, 6, dtype=torch.bool)
+    sees[17:min(17 + window, 60) if window else 60, 3:] = True
+    assert torch.equal(spoilt, sees)
+    assert torch.isfinite(got.float()[~sees.to(DEVICE)]).all()
+    ops.check_errors()
