@@ -176,7 +176,7 @@ __device__ __forceinline__ void load_tile(bf16* k_tile, bf16* v_tile, const Page
 template <int HD, int KEYS, bool MASKED, bool SHAPED, bool HALF = false>
 __device__ __forceinline__ void attend_tile(const uint32_t (&qf)[HD / 16][4], const bf16* k_tile,
                                             const bf16* v_tile, int first, const int (&limit_lo)[2],
-                                            const int (&limit_hi)[2], float scale_log2,
+                                            const int (&limit_hi)[2], const float (&to_log2)[2],
                                             float (&m)[2], float (&l)[2], float (&o)[HD / 8][4],
                                             int lane, int kept, const ScoreShape& shape, float slope,
                                             const int (&at)[2]) {
@@ -195,8 +195,13 @@ __device__ __forceinline__ void attend_tile(const uint32_t (&qf)[HD / 16][4], co
             uint32_t b[4];
             ldmatrix_x4(b, k_tile + (jj * 16 + r + (matrix >> 1) * 8) * T::STRIDE + kk * 16 +
                                (matrix & 1) * 8);
-            mma_16816(s[2 * jj], qf[kk], b[0], b[1]);
-            mma_16816(s[2 * jj + 1], qf[kk], b[2], b[3]);
+            if (HALF) {
+                mma_half(s[2 * jj], qf[kk], b[0], b[1]);
+                mma_half(s[2 * jj + 1], qf[kk], b[2], b[3]);
+            } else {
+                mma_16816(s[2 * jj], qf[kk], b[0], b[1]);
+                mma_16816(s[2 * jj + 1], qf[kk], b[2], b[3]);
+            }
         }
     }
 
@@ -215,8 +220,8 @@ __device__ __forceinline__ void attend_tile(const uint32_t (&qf)[HD / 16][4], co
                 s[j + (c >> 2)][c & 3] = fmaf(-slope, (float)(at[(c >> 1) & 1] - key), piece[c]);
             }
         }
-        scale_log2 = 1.f;
     }
+    const float scale_log2[2] = {SHAPED ? 1.f : to_log2[0], SHAPED ? 1.f : to_log2[1]};
     float tile_max[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int j = 0; j < KEYS / 8; ++j)
@@ -234,7 +239,7 @@ __device__ __forceinline__ void attend_tile(const uint32_t (&qf)[HD / 16][4], co
     for (int i = 0; i < 2; ++i) {
         tile_max[i] = fmaxf(tile_max[i], __shfl_xor_sync(0xffffffffu, tile_max[i], 1));
         tile_max[i] = fmaxf(tile_max[i], __shfl_xor_sync(0xffffffffu, tile_max[i], 2));
-        const float new_max = fmaxf(m[i], tile_max[i] * scale_log2);
+        const float new_max = fmaxf(m[i], tile_max[i] * scale_log2[i]);
         correction[i] = new_max == -INFINITY ? 1.f : fast_exp2(m[i] - new_max);
         m[i] = new_max;
     }
@@ -246,7 +251,7 @@ __device__ __forceinline__ void attend_tile(const uint32_t (&qf)[HD / 16][4], co
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             const int i = c >> 1;
-            const float p = fast_exp2(fmaf(s[j][c], scale_log2, -shift[i]));   // exp2(-inf) = 0
+            const float p = fast_exp2(fmaf(s[j][c], scale_log2[i], -shift[i]));   // exp2(-inf) = 0
             s[j][c] = p;
             tile_sum[i] += p;
         }
@@ -291,8 +296,8 @@ __device__ __forceinline__ void attend_tile(const uint32_t (&qf)[HD / 16][4], co
 constexpr int PREFILL_WARPS = 4;       // 8 warps (128 rows) measured the same on long prompts
 constexpr int ROWS = 16 * PREFILL_WARPS;      // query rows per block
 
-// HALF: values in half-precision times a power of two of their request and key head, whose inverse
-// `value_factors` [requests, kv_heads] holds.
+// HALF: queries, keys and values in half-precision times powers of two, whose inverses `query_factors` [tokens,
+// heads] and `factors` [requests, kv_heads, 2] (keys', values') hold.
 template <int HD, bool SHAPED, bool HALF>
 __global__ void __launch_bounds__(PREFILL_WARPS * 32)
 attention_prefill_kernel(const bf16* __restrict__ q, const bf16* __restrict__ kv, long long kv_half,
@@ -300,7 +305,8 @@ attention_prefill_kernel(const bf16* __restrict__ q, const bf16* __restrict__ kv
                          const int* __restrict__ request_start, const int* __restrict__ history,
                          bf16* __restrict__ out, int requests, int heads, int kv_heads,
                          float scale_log2, int window, const float* __restrict__ sinks,
-                         int keep_first, ScoreShape shape, const float* __restrict__ value_factors) {
+                         int keep_first, ScoreShape shape, const float* __restrict__ query_factors,
+                         const float* __restrict__ factors) {
     using T = Tile<HD>;
     constexpr int KEYS = PREFILL_KEYS;
     extern __shared__ __align__(16) unsigned char shared_bytes[];
@@ -375,6 +381,18 @@ attention_prefill_kernel(const bf16* __restrict__ q, const bf16* __restrict__ kv
         limit_hi[i] = row < rows ? position : -1;
         limit_lo[i] = first_visible_key(position, window);
     }
+    float to_log2[2] = {scale_log2, scale_log2};
+    const float* own_factors = HALF ? factors + ((size_t)request * kv_heads + head / (heads / kv_heads)) * 2 : nullptr;
+    if (HALF) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = warp * 16 + (lane >> 2) + i * 8;
+            to_log2[i] *= own_factors[0] *
+                          (row < rows ? query_factors[(size_t)(first_token + row_start + row) * heads + head] : 1.f);
+            // (neither zero nor infinite: a hidden score of -inf stays one, a score of zero too)
+            to_log2[i] = fminf(fmaxf(to_log2[i], 0x1p-126f), 0x1p127f);
+        }
+    }
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     if (sinks != nullptr) {
         // a sink is a term exp(sink) of the denominator without a key or a value: the softmax
@@ -426,10 +444,10 @@ attention_prefill_kernel(const bf16* __restrict__ q, const bf16* __restrict__ kv
                               tile * KEYS + KEYS - 1 <= warp_first;
             if (open)
                 attend_tile<HD, KEYS, false, SHAPED, HALF>(qf, k_now, v_now, tile * KEYS, limit_lo, limit_hi,
-                                                     scale_log2, m, l, o, lane, 0, shape, slope, at);
+                                                           to_log2, m, l, o, lane, 0, shape, slope, at);
             else
                 attend_tile<HD, KEYS, true, SHAPED, HALF>(qf, k_now, v_now, tile * KEYS, limit_lo, limit_hi,
-                                                    scale_log2, m, l, o, lane, keep_first, shape, slope,
+                                                          to_log2, m, l, o, lane, keep_first, shape, slope,
                                                     at);
         }
         __syncthreads();
@@ -440,7 +458,7 @@ attention_prefill_kernel(const bf16* __restrict__ q, const bf16* __restrict__ kv
         const int row = warp * 16 + (lane >> 2) + i * 8;
         if (row >= rows) continue;
         float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
-        if (HALF) inv *= value_factors[(size_t)request * kv_heads + head / (heads / kv_heads)];
+        if (HALF) inv *= own_factors[1];
         bf16* dst = out + ((size_t)(first_token + row_start + row) * heads + head) * HD +
                     (lane & 3) * 2;
 #pragma unroll
@@ -1008,7 +1026,8 @@ int launch_prefill(const void* q, const void* kv, long long kv_half, const int* 
                    int table_width, int page_size, const int* request_start, const int* history,
                    void* out, int tokens, int requests, int heads, int kv_heads, float scale,
                    int window, const float* sinks, cudaStream_t stream, int keep_first = 0,
-                   ScoreShape shape = ScoreShape(), const float* value_factors = nullptr) {
+                   ScoreShape shape = ScoreShape(), const float* query_factors = nullptr,
+                   const float* factors = nullptr) {
     using T = Tile<HD>;
     const size_t shared = (size_t)(ROWS + 4 * PREFILL_KEYS) * T::STRIDE * 2;
     auto kernel = attention_prefill_kernel<HD, SHAPED, HALF>;
@@ -1018,7 +1037,7 @@ int launch_prefill(const void* q, const void* kv, long long kv_half, const int* 
     kernel<<<grid, PREFILL_WARPS * 32, shared, stream>>>(
         (const bf16*)q, (const bf16*)kv, kv_half, block_table, table_width, page_size,
         request_start, history, (bf16*)out, requests, heads, kv_heads, scale * LOG2E, window,
-        sinks, keep_first, shape, value_factors);
+        sinks, keep_first, shape, query_factors, factors);
     return 0;
 }
 
@@ -1258,19 +1277,20 @@ MLXONE_API int mlxone_attention_decode_shaped(const void* q, const void* kv, con
     return 0;
 }
 
-// As mlxone_attention_prefill over values in half-precision, which are their values times the inverse of
-// value_factors [requests, kv_heads], a power of two; with a window, the first keep_first positions of a
-// sequence stay visible. Heads of 32, 64, 96 or 128 values.
+// As mlxone_attention_prefill with queries, keys and values in half-precision, times the inverses of query_factors
+// [tokens, heads] and of factors [requests, kv_heads, 2] (keys', values'), powers of two; with a window, the first
+// keep_first positions of a sequence stay visible. Heads of 32, 64, 96 or 128 values; the output is bfloat16.
 MLXONE_API int mlxone_attention_prefill_half(const void* q, const void* kv, const int* block_table,
                                              int table_width, int page_size, int pages,
                                              const int* request_start, const int* history, void* out,
                                              int tokens, int requests, int heads, int kv_heads,
                                              int head_dim, float scale, int window, int keep_first,
-                                             const float* sinks, const float* value_factors,
-                                             cudaStream_t stream) {
+                                             const float* sinks, const float* query_factors,
+                                             const float* factors, cudaStream_t stream) {
     if (tokens == 0) return 0;
     MLXONE_REQUIRE(tokens > 0 && requests > 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0 &&
-                       heads <= 65535 && value_factors != nullptr, "attention_prefill: bad sizes");
+                       heads <= 65535 && query_factors != nullptr && factors != nullptr,
+                   "attention_prefill: bad sizes");
     MLXONE_REQUIRE(page_size > 0 && pages > 0 && table_width > 0,
                    "attention_prefill: bad page geometry");
     const long long kv_half = (long long)pages * kv_heads * page_size * head_dim;
@@ -1278,13 +1298,13 @@ MLXONE_API int mlxone_attention_prefill_half(const void* q, const void* kv, cons
     launch_prefill<HD, false, true>(q, kv, kv_half, block_table, table_width, page_size,       \
                                     request_start, history, out, tokens, requests, heads,      \
                                     kv_heads, scale, window, sinks, stream, keep_first,        \
-                                    ScoreShape(), value_factors)
+                                    ScoreShape(), query_factors, factors)
     switch (head_dim) {
         case 32: CALL(32); break;
         case 64: CALL(64); break;
         case 96: CALL(96); break;
         case 128: CALL(128); break;
-        default: mlxone_set_error("attention_prefill: no half-precision values for heads of %d", head_dim); return 1;
+        default: mlxone_set_error("attention_prefill: no half-precision form for heads of %d", head_dim); return 1;
     }
 #undef CALL
     MLXONE_LAUNCH_CHECK("attention_prefill");

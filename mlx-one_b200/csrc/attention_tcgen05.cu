@@ -343,10 +343,11 @@ __device__ __forceinline__ void shape_tile(float (&v)[N], const ScoreShape& shap
     }
 }
 
-// HALF: values are half-precision and times a power of two of their request and key head, whose inverse
-// `value_factors` [requests, kv_heads] holds (the output is multiplied by it); the weights are then
-// half-precision too, 2^7 times what they are otherwise (at most 2^15; the sum has the same factor), so that
-// weights down to 2^-31 of the largest count.
+// HALF: queries, keys and values are half-precision and times powers of two, a query's row by itself and the
+// keys and the values of a request and key head; `query_factors` [tokens, heads] and `factors` [requests,
+// kv_heads, 2] (keys', values') hold the inverses, by which scores and outputs are multiplied. The weights are
+// then half-precision too, 2^7 times what they are otherwise (at most 2^15; the sum has the same factor), so
+// that weights down to 2^-31 of the largest count.
 template <int KEYS, int PARTS, bool SHAPED, bool HALF>
 __global__ void __launch_bounds__((4 * PARTS + 2) * 32, Shape<KEYS>::BLOCKS_PER_SM)
 attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q,
@@ -357,7 +358,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q,
                          int heads, int kv_heads, float scale_log2, int window, int token_tiles,
                          int splits, float* __restrict__ partial, const float* __restrict__ sinks,
                          int* __restrict__ error_flag, int keep_first, ScoreShape shape,
-                         const float* __restrict__ value_factors) {
+                         const float* __restrict__ query_factors, const float* __restrict__ factors) {
     using S = Shape<KEYS>;
     constexpr float RAISED = HALF ? 7.f : 0.f;
     constexpr int COPY_WARP = 4 * PARTS, MMA_WARP = 4 * PARTS + 1;
@@ -529,7 +530,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q,
         }
     } else if (warp == MMA_WARP) {
         if (lane == 0) {
-            constexpr uint32_t idesc_scores = instruction_descriptor(ROWS, KEYS, false);
+            constexpr uint32_t idesc_scores = instruction_descriptor(ROWS, KEYS, false, HALF);
             constexpr uint32_t idesc_out = instruction_descriptor(ROWS, HD, true, HALF);
             // a place in the walk: item n, its tile j; `taken` and `t` as above
             struct Place { int n, j, taken, t; };
@@ -635,6 +636,14 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q,
             const int last_position = item.first_position + item.tokens_here - 1;
             const int limit_hi = valid ? position : -1;
             const int limit_lo = first_visible_key(position, item.window);
+            float to_log2 = scale_log2;            // from a product of a query and a key to the exponent
+            if (HALF) {
+                to_log2 *= factors[((size_t)item.request * kv_heads + item.kv_head) * 2];
+                to_log2 *= valid ? query_factors[(size_t)(item.q_token + token) * heads + item.kv_head * group +
+                                                 row % group] : 1.f;
+                // (neither zero nor infinite: a hidden score of -inf stays one, a score of zero too)
+                to_log2 = fminf(fmaxf(to_log2, 0x1p-126f), 0x1p127f);
+            }
             float slope = 0.f;
             if (SHAPED && shape.slopes != nullptr)
                 slope = shape.slopes[item.kv_head * group + row % group] * 1.4426950408889634f;
@@ -683,7 +692,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q,
                     for (int other = 0; other < PARTS; ++other)
                         top = fmaxf(top, maxima[((t & 1) * PARTS + other) * ROWS + row]);
                 }
-                const float running = fmaxf(m, SHAPED ? top : top * scale_log2);
+                const float running = fmaxf(m, SHAPED ? top : top * to_log2);
                 // both threads of a row see the same maxima and take the same decision
                 const bool follow = running > m + LAZY || (m == -INFINITY && running > m);
                 const float moved = !follow ? 1.f : m == -INFINITY ? 0.f : fast_exp2(m - running);
@@ -704,7 +713,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q,
                 if (follow) m = running;
                 const float shift = (m == -INFINITY ? 0.f : m) - RAISED;
                 unsigned long long partial[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
-                const unsigned long long scale_pair = pair_of(scale_log2, scale_log2);
+                const unsigned long long scale_pair = pair_of(to_log2, to_log2);
                 const unsigned long long shift_pair = pair_of(-shift, -shift);
                 unsigned char* p_tile_row = p_row + (t & 1) * P_BYTES;
 #pragma unroll
@@ -768,7 +777,7 @@ attention_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q,
                 else l += fast_exp2(fminf(sink - m + RAISED, 126.f));
             }
             if (HALF) {
-                const float factor = value_factors[(size_t)item.request * kv_heads + item.kv_head];
+                const float factor = factors[((size_t)item.request * kv_heads + item.kv_head) * 2 + 1];
 #pragma unroll
                 for (int d = 0; d < MY_DIMS; ++d) o[d] *= factor;
             }
@@ -915,7 +924,8 @@ static int prefill_tcgen05(const void* q, const void* kv, const int* block_table
                                                 int splits, float* partial, const float* sinks,
                                                 int keys, int* error_flag, cudaStream_t stream, int keep_first,
                                                 bool shaped = false, ScoreShape shape = ScoreShape(),
-                                                const float* value_factors = nullptr) {
+                                                const float* query_factors = nullptr,
+                                                const float* factors = nullptr) {
     if (tokens == 0) return 0;
     MLXONE_REQUIRE(keep_first >= 0 && (keep_first == 0 || window > 0),
                    "attention_prefill_tcgen05: first positions are kept behind a window only");
@@ -976,7 +986,7 @@ static int prefill_tcgen05(const void* q, const void* kv, const int* block_table
     const int threads = ((small_tiles ? 1 : 2) * 4 + 2) * 32;
     auto kernel = shaped ? (small_tiles ? attention_tcgen05_kernel<64, 1, true, false>
                                         : attention_tcgen05_kernel<128, 2, true, false>)
-                  : value_factors != nullptr ? (small_tiles ? attention_tcgen05_kernel<64, 1, false, true>
+                  : factors != nullptr ? (small_tiles ? attention_tcgen05_kernel<64, 1, false, true>
                                                             : attention_tcgen05_kernel<128, 2, false, true>)
                                              : (small_tiles ? attention_tcgen05_kernel<64, 1, false, false>
                                                             : attention_tcgen05_kernel<128, 2, false, false>);
@@ -988,7 +998,7 @@ static int prefill_tcgen05(const void* q, const void* kv, const int* block_table
     kernel<<<dim3((unsigned)blocks), threads, shared, stream>>>(
         map_q, map_kv, value_rows, block_table, table_width, page_size, box_keys, request_start,
         history, static_cast<bf16*>(out), requests, heads, kv_heads, scale * 1.4426950408889634f,
-        window, token_tiles, splits, partial, sinks, error_flag, keep_first, shape, value_factors);
+        window, token_tiles, splits, partial, sinks, error_flag, keep_first, shape, query_factors, factors);
     MLXONE_LAUNCH_CHECK("attention_prefill_tcgen05");
     return 0;
 }
@@ -1020,21 +1030,22 @@ MLXONE_API int mlxone_attention_prefill_tcgen05_keep(const void* q, const void* 
                            partial, sinks, keys, error_flag, stream, keep_first);
 }
 
-// ... over keys in bfloat16 and values in half-precision, which are their values times the inverse of
-// value_factors [requests, kv_heads], a power of two (both planes have rows of 128 bytes)
+// ... with queries, keys and values in half-precision, times the inverses of query_factors [tokens, heads] and of
+// factors [requests, kv_heads, 2] (keys', values'), powers of two; the output is bfloat16
 MLXONE_API int mlxone_attention_prefill_tcgen05_half(const void* q, const void* kv, const int* block_table,
                                                      int table_width, int page_size, int pages,
                                                      const int* request_start, const int* history, void* out,
                                                      int tokens, int requests, int heads, int kv_heads,
                                                      int head_dim, float scale, int window, int keep_first,
                                                      int splits, float* partial, const float* sinks, int keys,
-                                                     const float* value_factors, int* error_flag,
-                                                     cudaStream_t stream) {
-    MLXONE_REQUIRE(value_factors != nullptr, "attention_prefill_tcgen05: values without their factors");
+                                                     const float* query_factors, const float* factors,
+                                                     int* error_flag, cudaStream_t stream) {
+    MLXONE_REQUIRE(query_factors != nullptr && factors != nullptr,
+                   "attention_prefill_tcgen05: half-precision without its factors");
     return prefill_tcgen05(q, kv, block_table, table_width, page_size, pages, request_start, history,
                            out, tokens, requests, heads, kv_heads, head_dim, scale, window, splits,
                            partial, sinks, keys, error_flag, stream, keep_first, false, ScoreShape(),
-                           value_factors);
+                           query_factors, factors);
 }
 
 // ... with scores s that become cap tanh(s / cap) (cap 0: none) and then lose slopes[head] (float32

@@ -300,13 +300,13 @@ read_kernel(const unsigned char* cache, const int* positions,
     }
 }
 
-// The largest value (of the values' part, by its size) that 1,024 keys of a request and key head may open to:
-// largest [requests, open heads, chunks].
+// The largest number, by its size, that the keys' and the values' part of 1,024 keys of a request and key head may
+// open to: largest [requests, open heads, 2, chunks].
 constexpr int CHUNK_UNITS = 64;
 
 template <int HD>
 __global__ void __launch_bounds__(256)
-value_range_kernel(const unsigned char* cache, const int* block_table, int table_width, int page_shift, int pages,
+range_kernel(const unsigned char* cache, const int* block_table, int table_width, int page_shift, int pages,
                    const int* request_start, const int* history, int span, int first_request, int first_head,
                    int kv_heads, float* largest) {
     using P = Packed<HD>;
@@ -318,7 +318,7 @@ value_range_kernel(const unsigned char* cache, const int* block_table, int table
     const int held = history[request];
     const int length = held + request_start[request + 1] - request_start[request];
     const int lowest_key = first_visible_key(held, span), units = 1 << (page_shift - 4);
-    float most = 0.f;
+    float most[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = threadIdx.x; i < CHUNK_UNITS * 16; i += 256) {
         const int first = (chunk * CHUNK_UNITS + i / 16) * 16, place = i % 16;
@@ -327,17 +327,56 @@ value_range_kernel(const unsigned char* cache, const int* block_table, int table
         const int page = block < table_width ? block_table[(size_t)request * table_width + block] : -1;
         if (page < 0 || page >= pages) continue;
         const unsigned char* part =
-            from + (((size_t)page * kv_heads + head) * units + (first >> 4 & (units - 1))) * P::UNIT + P::PART;
+            from + (((size_t)page * kv_heads + head) * units + (first >> 4 & (units - 1))) * P::UNIT;
 #pragma unroll
-        for (int g = 0; g < P::GROUPS; ++g) {
-            const uint32_t word = *reinterpret_cast<const uint32_t*>(part + P::CODES + 64 * g + 4 * place);
+        for (int g = 0; g < 2 * P::GROUPS; ++g) {
+            const uint32_t word = *reinterpret_cast<const uint32_t*>(part + g % 2 * P::PART + P::CODES + 64 * (g / 2) +
+                                                                     4 * place);
             const float lowest = packed_lowest(word);
             // (what is no number counts as nothing)
-            most = fmaxf(most, fmaxf(fabsf(lowest), fabsf(fmaf(15.f, packed_step(word), lowest))));
+            most[g % 2] = fmaxf(most[g % 2], fmaxf(fabsf(lowest), fabsf(fmaf(15.f, packed_step(word), lowest))));
         }
     }
-    most = block_max(most, scratch);
-    if (threadIdx.x == 0) largest[((size_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + chunk] = most;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const float all = block_max(most[k], scratch);
+        if (threadIdx.x == 0)
+            largest[(((size_t)blockIdx.z * gridDim.y + blockIdx.y) * 2 + k) * gridDim.x + chunk] = all;
+    }
+}
+
+// Queries as half-precision, a row times the power of two that brings its largest to 2^10 (exact but for what is
+// 2^-26 of the largest and less), whose inverse goes to `factors`. HD / 8 lanes a row.
+template <int HD>
+__global__ void __launch_bounds__(256)
+half_queries_kernel(const bf16* q, long long rows, uint4* out, float* factors) {
+    constexpr int LANES = HD == 96 ? 16 : HD / 8;
+    griddep_launch();
+    griddep_wait();
+    const bf16* written = settled(q);
+    const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / LANES;
+    const int sub = threadIdx.x % LANES;
+    const bool live = row < rows && sub * 8 < HD;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+    if (live) load_eight<bf16>(written + row * HD + sub * 8, true, x);
+    float most = 0.f, inverse;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (fabsf(x[i]) < INFINITY) most = fmaxf(most, fabsf(x[i]));
+#pragma unroll
+    for (int offset = 1; offset < LANES; offset <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, offset));
+    const float by = power_towards(most, 10, inverse);
+    if (!live) return;
+    uint32_t pairs[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 pair = __floats2half2_rn(x[2 * i] * by, x[2 * i + 1] * by);
+        pairs[i] = *reinterpret_cast<const uint32_t*>(&pair);
+    }
+    out[row * (HD / 8) + sub] = make_uint4(pairs[0], pairs[1], pairs[2], pairs[3]);
+    if (sub == 0) factors[row] = inverse;
 }
 
 // Requests opened: every unit that the requests' tables name, up to their last token, as plain values in
@@ -346,10 +385,10 @@ value_range_kernel(const unsigned char* cache, const int* block_table, int table
 // so that no reader meets a number that is none. A token whose keys or values are none has NaN for its keys and
 // zeros for its values: queries that see it get NaN by their scores, the others nothing, since a reader drops
 // scores that are masked but multiplies every value. `table` gets the page numbers and, behind them, where the
-// requests' tokens start, counted from the first one's. With `largest` (value_range_kernel's, `chunks` of them
-// each) values are half-precision, times the power of two that brings the largest of a request and key head to
-// 2^9, whose inverse goes to `factors` [requests, open heads]: 11 bits of every value of 2^-23 of the largest and
-// more, where bfloat16 has 8. A thread takes a run of four keys, 2j, 2j + 1, 2j + 8 and 2j + 9: every byte of its
+// requests' tokens start, counted from the first one's. With `largest` (range_kernel's, `chunks` of them each) the
+// pages are half-precision, keys and values times the powers of two that bring the largest of a request and key
+// head to 2^9, whose inverses go to `factors` [requests, open heads, 2]: 11 bits of every number of 2^-23 of the
+// largest and more, where bfloat16 has 8. A thread takes a run of four keys, 2j, 2j + 1, 2j + 8 and 2j + 9: every byte of its
 // eight words is theirs, of the keys' part as of the values'.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256)
@@ -371,11 +410,17 @@ open_kernel(const unsigned char* cache, const int* block_table, int table_width,
     const int unit = blockIdx.x * (blockDim.x / THREADS) + threadIdx.x / THREADS;
     float raise = 1.f;
     if (largest != nullptr) {
-        const float* mine = settled(largest) + ((size_t)r * gridDim.y + open_head) * chunks;
-        float most = 0.f, inverse;
-        for (int i = threadIdx.x & 31; i < chunks; i += 32) most = fmaxf(most, mine[i]);
-        raise = power_towards(warp_max(most), 9, inverse);
-        if (blockIdx.x == 0 && threadIdx.x == 0) factors[(size_t)r * gridDim.y + open_head] = inverse;
+        const float* mine = settled(largest) + ((size_t)r * gridDim.y + open_head) * 2 * chunks;
+        float most[2] = {0.f, 0.f}, inverse[2];
+        for (int i = threadIdx.x & 31; i < chunks; i += 32) {
+            most[0] = fmaxf(most[0], mine[i]);
+            most[1] = fmaxf(most[1], mine[chunks + i]);
+        }
+        const float of_keys = power_towards(warp_max(most[0]), 9, inverse[0]);
+        const float of_values = power_towards(warp_max(most[1]), 9, inverse[1]);
+        raise = inside / P::RUNS & 1 ? of_values : of_keys;
+        if (blockIdx.x == 0 && threadIdx.x < 2)
+            factors[((size_t)r * gridDim.y + open_head) * 2 + threadIdx.x] = inverse[threadIdx.x];
     }
     if (unit >= blocks * per_block) return;
     const int open_block = unit / per_block;
@@ -430,8 +475,8 @@ open_kernel(const unsigned char* cache, const int* block_table, int table_width,
             const bool is_none = none >> k & 1u;
             if (key >= length || is_none) step[k] = 0.f;
             if (key >= length || is_none) lowest[k] = key < length && !which ? NAN : 0.f;
-            step[k] *= which ? raise : 1.f;
-            lowest[k] *= which ? raise : 1.f;
+            step[k] *= raise;
+            lowest[k] *= raise;
         }
     }
     T* to = opened + which * half + (((size_t)r * blocks + open_block) * gridDim.y + open_head) * open_size * HD +
@@ -449,7 +494,7 @@ open_kernel(const unsigned char* cache, const int* block_table, int table_width,
             x[e + 8] = fmaf(step[k], (float)(both >> 4 & 15u), lowest[k]);
         }
         T* row = to + (2 * j + (k & 1) + 8 * (k >> 1)) * HD;
-        if (sizeof(T) == 2 && which && largest != nullptr) {
+        if (sizeof(T) == 2 && largest != nullptr) {
             uint32_t pairs[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -538,17 +583,17 @@ MLXONE_API int mlxone_read_key_values(const void* cache, const int* positions, c
     return 0;
 }
 
-// Floats that mlxone_open_key_values needs as `factors` for half-precision values.
+// Floats that mlxone_open_key_values needs as `factors` for half-precision pages.
 MLXONE_API long long mlxone_open_factors(int requests, int open_heads, int blocks, int open_size) {
     if (requests <= 0 || open_heads <= 0 || blocks <= 0 || open_size <= 0) return 0;
-    return (long long)requests * open_heads * (1 + ceil_div_host((long long)blocks * open_size, 16 * CHUNK_UNITS));
+    return 2LL * requests * open_heads * (1 + ceil_div_host((long long)blocks * open_size, 16 * CHUNK_UNITS));
 }
 
 // Requests first_request.. (`requests` of them) and key heads first_head.. (`open_heads` of kv_heads), `blocks`
 // pages of `open_size` tokens (a multiple of 16) for each request: opened [2, requests * blocks, open_heads,
 // open_size, head_dim], table int32 [requests * blocks + requests + 1]. `span`: see first_visible_key; units that
-// no token of the step sees are zeros. factors: null, or (bfloat16) mlxone_open_factors floats: values are then
-// half-precision, and the first requests * open_heads of them are what they are to be multiplied by.
+// no token of the step sees are zeros. factors: null, or (bfloat16) mlxone_open_factors floats: the pages are then
+// half-precision, and the first requests * open_heads * 2 of them are what keys and values are to be multiplied by.
 MLXONE_API int mlxone_open_key_values(const void* cache, const int* block_table, int table_width, int page_size,
                                       int pages, const int* request_start, const int* history, int span,
                                       int first_request, int requests, int kv_heads, int first_head,
@@ -559,7 +604,7 @@ MLXONE_API int mlxone_open_key_values(const void* cache, const int* block_table,
     MLXONE_REQUIRE(requests > 0 && requests <= 65535 && first_request >= 0 && blocks > 0 && open_size >= 16 &&
                        open_size % 16 == 0 && first_head >= 0 && open_heads > 0 &&
                        first_head + open_heads <= kv_heads, "open_key_values: bad sizes");
-    MLXONE_REQUIRE(factors == nullptr || dtype == MLXONE_BF16, "open_key_values: half-precision values beside bfloat16 keys");
+    MLXONE_REQUIRE(factors == nullptr || dtype == MLXONE_BF16, "open_key_values: half-precision pages for bfloat16 queries only");
     MLXONE_REQUIRE(((size_t)opened & 15) == 0, "open_key_values: the output starts at a multiple of 16 bytes");
     const long long half = (long long)requests * blocks * open_heads * open_size * head_dim;
     const int page_shift = 31 - __builtin_clz((unsigned)page_size);
@@ -567,9 +612,9 @@ MLXONE_API int mlxone_open_key_values(const void* cache, const int* block_table,
     const unsigned char* held = (const unsigned char*)cache;
     float* largest = nullptr;
     if (factors != nullptr) {
-        largest = factors + (size_t)requests * open_heads;
+        largest = factors + (size_t)requests * open_heads * 2;
 #define CALL(HD)                                                                                          \
-    launch_kernel(value_range_kernel<HD>, dim3(chunks, open_heads, requests), dim3(256), 0, stream, true, \
+    launch_kernel(range_kernel<HD>, dim3(chunks, open_heads, requests), dim3(256), 0, stream, true, \
                   held, block_table, table_width, page_shift, pages, request_start, history, span,        \
                   first_request, first_head, kv_heads, largest)
         MLXONE_PACKED_DIMS(CALL)
@@ -593,5 +638,20 @@ MLXONE_API int mlxone_open_key_values(const void* cache, const int* block_table,
     MLXONE_PACKED_DIMS(CALL)
 #undef CALL
     MLXONE_LAUNCH_CHECK("open_key_values");
+    return 0;
+}
+
+// q bfloat16 [rows, head_dim] -> out half-precision [rows, head_dim], factors float32 [rows].
+MLXONE_API int mlxone_half_queries(const void* q, long long rows, int head_dim, void* out, float* factors,
+                                   cudaStream_t stream) {
+    if (rows == 0) return 0;
+    MLXONE_REQUIRE(rows > 0 && (((size_t)q | (size_t)out) & 15) == 0,
+                   "half_queries: rows start at multiples of 16 bytes");
+#define CALL(HD)                                                                                              \
+    launch_kernel(half_queries_kernel<HD>, dim3(ceil_div_host(rows, 256 / (HD == 96 ? 16 : HD / 8))), dim3(256), 0, \
+                  stream, true, (const bf16*)q, rows, (uint4*)out, factors)
+    MLXONE_PACKED_DIMS(CALL)
+#undef CALL
+    MLXONE_LAUNCH_CHECK("half_queries");
     return 0;
 }

@@ -1760,7 +1760,9 @@ class CudaOps:
             rest = ctx.requests - singles
             table = view.block_table[singles:]
             starts, history = ctx.request_start[singles:], ctx.history[singles:]
-            factors = view.factors if isinstance(view, OpenedView) else None
+            factors = ()
+            if isinstance(view, OpenedView) and view.factors is not None:
+                factors = (_c_void_p(_ptr(view.query_factors)), _c_void_p(_ptr(view.factors)))
             if (self.tcgen05_attention and q.dtype == torch.bfloat16
                     and self.lib.mlxone_attention_tcgen05_supports(
                         _c_int(head_dim), _c_int(heads), _c_int(kv_heads), _c_int(view.page_size))):
@@ -1781,9 +1783,9 @@ class CudaOps:
                 if splits > 1:
                     partial = torch.empty(tokens * heads * splits * (head_dim + 2),
                                           dtype=torch.float32, device=self.device)
-                # (half-precision values: an entry of their own, one argument more)
-                self._call("mlxone_attention_prefill_tcgen05_keep" if factors is None
-                           else "mlxone_attention_prefill_tcgen05_half", _c_void_p(_ptr(q)),
+                # (half-precision: an entry of its own, the factors besides)
+                self._call("mlxone_attention_prefill_tcgen05_half" if factors
+                           else "mlxone_attention_prefill_tcgen05_keep", _c_void_p(_ptr(q)),
                            _c_void_p(_ptr(view.kv)), _c_void_p(_ptr(table)),
                            _c_int(width), _c_int(view.page_size), _c_int(pages),
                            _c_void_p(_ptr(starts)), _c_void_p(_ptr(history)),
@@ -1791,8 +1793,7 @@ class CudaOps:
                            _c_int(heads), _c_int(kv_heads), _c_int(head_dim), _c_float(scale),
                            _c_int(window or 0), _c_int(keep_first), _c_int(splits),
                            _c_void_p(_ptr(partial)), _c_void_p(_ptr(sinks)), _c_int(keys),
-                           *(() if factors is None else (_c_void_p(_ptr(factors)),)),
-                           _c_void_p(_ptr(self.error_flag)))
+                           *factors, _c_void_p(_ptr(self.error_flag)))
                 if partial is not None:
                     # (the leading single tokens are the decode kernel's: their rows stay)
                     skip = singles * heads * splits * (head_dim + 2)
@@ -1800,15 +1801,15 @@ class CudaOps:
                                _c_void_p(_ptr(out[singles:])), _c_int((tokens - singles) * heads),
                                _c_int(splits), _c_int(head_dim))
             else:
-                self._call("mlxone_attention_prefill_keep" if factors is None
-                           else "mlxone_attention_prefill_half", _c_void_p(_ptr(q)),
+                self._call("mlxone_attention_prefill_half" if factors
+                           else "mlxone_attention_prefill_keep", _c_void_p(_ptr(q)),
                            _c_void_p(_ptr(view.kv)), _c_void_p(_ptr(table)),
                            _c_int(width), _c_int(view.page_size), _c_int(pages),
                            _c_void_p(_ptr(starts)), _c_void_p(_ptr(history)),
                            _c_void_p(_ptr(out)), _c_int(tokens), _c_int(rest),
                            _c_int(heads), _c_int(kv_heads), _c_int(head_dim), _c_float(scale),
                            _c_int(window or 0), _c_int(keep_first), _c_void_p(_ptr(sinks)),
-                           *(() if factors is None else (_c_void_p(_ptr(factors)),)))
+                           *factors)
             return out
         if (q.dtype == torch.float32 and not window and sinks is None
                 and self.lib.mlxone_attention_f32_supports(_c_int(head_dim), _c_int(heads),
@@ -2146,14 +2147,19 @@ class CudaOps:
         opened = torch.empty((2, rest * blocks, at_once, self.open_page, head_dim), dtype=q.dtype,
                              device=self.device)
         numbers = table[:rest * blocks].view(rest, blocks)
-        # values in half-precision beside bfloat16 keys: weights and values then keep 11 bits, not 8 (portions of
-        # 1,024 tokens behind 3,076 keys are off by 0.0023 of themselves, not 0.0036; 0.0016 is the result's own
-        # rounding). The kernels of shaped scores have no such form.
-        factors = None
+        # Everything in half-precision: keys, values and weights then keep 11 bits, not bfloat16's 8 (portions of
+        # 1,024 tokens behind 3,076 keys are off by 0.0017 of themselves, not 0.0036; 0.0016 is the result's own
+        # rounding; they take 85 us instead of 77, for the range of keys and values is looked for first). The kernels of shaped scores have no such form.
+        factors = query_factors = None
         if q.dtype == torch.bfloat16 and self.tensor_core_attention and not score_cap and slopes is None:
             factors = torch.empty(self.lib.mlxone_open_factors(rest, at_once, blocks, self.open_page),
                                   dtype=torch.float32, device=self.device)
-            self.launches += 1              # the values' range
+            halves = torch.empty((queries.shape[0], heads, head_dim), dtype=q.dtype, device=self.device)
+            query_factors = torch.empty((queries.shape[0], heads), dtype=torch.float32, device=self.device)
+            self._call("mlxone_half_queries", _c_void_p(_ptr(queries)), _c_ll(query_factors.numel()), _c_int(head_dim),
+                       _c_void_p(_ptr(halves)), _c_void_p(_ptr(query_factors)))
+            queries = halves
+            self.launches += 1              # the range of keys and values
         for first in range(0, kv_heads, at_once):
             count = min(at_once, kv_heads - first)
             here = opened if count == at_once else opened.view(-1)[:opened.numel() // at_once * count].view(
@@ -2166,7 +2172,7 @@ class CudaOps:
                        _c_int(first), _c_int(count), _c_int(head_dim), _c_int(blocks),
                        _c_int(self.open_page), _c_void_p(_ptr(here)), _c_void_p(_ptr(table)),
                        _c_void_p(_ptr(factors)), _c_int(_dtype_code(q.dtype)))
-            plain = OpenedView(here, numbers, self.open_page, view.need, factors)
+            plain = OpenedView(here, numbers, self.open_page, view.need, factors, query_factors)
             own = slice(first * group, (first + count) * group)
             how = dict(heads=count * group, kv_heads=count, head_dim=head_dim, scale=scale, window=window, ctx=step,
                        view=plain, keep_first=keep_first, score_cap=score_cap, least_slope=least_slope)
@@ -2174,6 +2180,8 @@ class CudaOps:
                 self.paged_attention(queries, out=result, sinks=sinks, slopes=slopes, **how)
                 return
             # (more than the scratch holds: some key heads after the others)
+            if query_factors is not None:
+                plain.query_factors = query_factors[:, own].contiguous()
             part = self.paged_attention(queries.view(-1, heads, head_dim)[:, own].contiguous(),
                                         sinks=None if sinks is None else sinks[own],
                                         slopes=None if slopes is None else slopes[own], **how)

@@ -79,11 +79,13 @@ class PackedView:
 
 @dataclass
 class OpenedView(PagedView):
-    """Pages that were opened from packed ones for one call: keys in bfloat16, and values in
-    half-precision (in the same storage, by their bits) that are to be multiplied by ``factors``
-    (float32 [requests, kv_heads], powers of two)."""
+    """Pages that were opened from packed ones for one call. With ``factors`` they and the call's
+    queries are half-precision (in bfloat16 tensors, by their bits), times powers of two: ``factors``
+    (float32 [requests, kv_heads, 2], keys' and values') and ``query_factors`` (float32 [tokens, heads])
+    bring them back."""
 
     factors: torch.Tensor | None = None
+    query_factors: torch.Tensor | None = None
 
 
 def packed_part_bytes(head_dim: int) -> int:

@@ -396,3 +396,34 @@ def test_what_is_not_a_number_in_a_portion(ops, dtype, dim, window, of_values):
     assert torch.equal(spoilt, sees)
     assert torch.isfinite(got.float()[~sees.to(DEVICE)]).all()
     ops.check_errors()
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (96, 32), (128, 64), (32, 16)])
+@pytest.mark.parametrize("of_keys,of_queries", [(1e-30, 1e30), (1e-30, 1e-30), (1.0, 1.0), (1e5, 1e-5), (1e30, 1e-30)])
+@pytest.mark.parametrize("window", [0, 24])
+def test_portions_of_keys_and_queries_of_any_size(ops, dim, page, of_keys, of_queries, window):
+    """Keys and queries beyond half-precision's range: times a power of two of their head's, and of their row's."""
+    portions, histories = [40, 21], [30, 100]
+    whole, _, _ = make_batch([70, 121], [0, 0], page, DEVICE)
+    ctx, table, pages = make_batch(portions, histories, page, DEVICE)
+    view = PackedView(torch.full((pages, 2, page // 16, 2, plain.part_bytes(dim)), 0xFF, dtype=torch.uint8, device=DEVICE),
+                      table, page, PagedKeyValues(2, dim))
+    keys = rows_of(191, 2, dim, F32, 3, 0.3)
+    keys[:, 1] *= 1e-3                                        # a head's keys are its own matter
+    keys = (keys * of_keys).to(BF16)
+    values = rows_of(191, 2, dim, BF16, 4, 0.3)
+    ops.pack_key_values(keys.view(191, -1).to(DEVICE), values.view(191, -1).to(DEVICE), ctx=whole, view=view)
+    q = (torch.randn(61, 4, dim, generator=torch.Generator().manual_seed(1)) * of_queries)
+    q[:, 2:] *= 1e3
+    q = q.to(BF16)
+    got = ops.paged_attention(q.to(DEVICE), heads=4, kv_heads=2, head_dim=dim, scale=dim ** -0.5, window=window or None,
+                              ctx=ctx, view=view).view(61, 4, dim).cpu().double()
+    want = plain.attend(q, view.kv.cpu(), table.cpu(), page, portions, histories, 4, 2, dim ** -0.5, window=window)
+    t = 0
+    for r, (n, held) in enumerate(zip(portions, histories)):
+        both = plain.read(view.kv.cpu(), table.cpu(), page, r, held + n, dim)
+        for h in range(2):
+            bound = bound_of(both[:, :, h], q[t:t + n, 2 * h:2 * h + 2], dim ** -0.5, dim, BF16, held + n)["portion"]
+            assert (got[t:t + n, 2 * h:2 * h + 2] - want[t:t + n, 2 * h:2 * h + 2]).abs().max() <= bound, (r, h)
+        t += n
+    ops.check_errors()
