@@ -2418,6 +2418,55 @@ def kernel_case(name: str, batch: int, context: int) -> int:
         steps = torch.zeros(batch, dtype=torch.int32, device=device)
         run = lambda i: ops.sample(logits[i % 4], temperature, top_k, top_p, seed, steps)
         work = f"{batch} rows of {vocab} logits, temperature 0.8, top-k 40, top-p 0.9"
+    elif name in ("packed_attention", "packed_portion", "pack_key_values"):
+        # a cache of 4 bits: a decode step's attention over the codes, a portion of 1,024 tokens behind `context`
+        # keys (ranges, opening, prefill attention), or a portion's keys and values packed
+        from mlx_one_b200.parts.base import PackedView, packed_part_bytes
+
+        portions = [1] * batch if name == "packed_attention" else [1024]
+        ctx, plainly = batch_context(portions, [context - 1] * batch if name == "packed_attention" else [context])
+        ctx.leading_single = batch if name == "packed_attention" else 0
+        pages = plainly.kv.shape[1]
+        kv = torch.zeros(pages, kv_heads, PAGE_SIZE // 16, 2, packed_part_bytes(head_dim), dtype=torch.uint8,
+                         device=device)
+        view = PackedView(kv, plainly.block_table, PAGE_SIZE, plainly.need)
+        every, _ = batch_context([context + n - 1 if name == "packed_attention" else context + n for n in portions],
+                                 [0] * len(portions))
+        rows = torch.randn(2, every.tokens, kv_heads * head_dim, device=device).bfloat16()
+        ops.pack_key_values(rows[0], rows[1], ctx=every, view=view)
+        q = torch.randn(ctx.tokens, heads, head_dim, device=device).bfloat16()
+        if name == "pack_key_values":
+            run = lambda i: ops.pack_key_values(rows[0, :ctx.tokens], rows[1, :ctx.tokens], ctx=ctx, view=view)
+            work = f"{ctx.tokens} tokens of {kv_heads} heads of {head_dim}"
+        else:
+            run = lambda i: ops.paged_attention(q, heads=heads, kv_heads=kv_heads, head_dim=head_dim,
+                                                scale=head_dim ** -0.5, window=None, ctx=ctx, view=view)
+            work = f"{ctx.tokens} tokens, {kv.numel() / 1e6:.1f} MB of codes"
+    elif name in ("beam_select", "reorder_pages", "reorder_slots"):
+        # four hypotheses of each of `batch` requests: the choice over the vocabulary, pages of 4 bits (half a page a
+        # hypothesis) and convolution states brought to the chosen ones
+        from mlx_one_b200.parts.base import packed_part_bytes
+
+        beams, vocab = 4, LFM2_1_2B["vocab_size"]
+        logits = [torch.randn(batch * beams, vocab, device=device) * 3 for _ in range(4)]
+        scores = torch.randn(batch, beams, device=device)
+        parents = torch.randint(0, beams, (batch, beams), device=device).int()
+        if name == "beam_select":
+            run = lambda i: ops.beam_select(logits[i % 4], scores)
+            work = f"{batch} requests of {beams} hypotheses, {vocab} logits each"
+        elif name == "reorder_slots":
+            state = torch.randn(10, batch * beams, 2 * hidden, device=device).bfloat16()
+            slots = torch.arange(batch * beams, dtype=torch.int32, device=device).view(batch, beams)
+            run = lambda i: ops.reorder_slots(state, slots, parents)
+            work = f"{state.numel() * 2 / 1e6:.1f} MB of states"
+        else:
+            kv = torch.zeros(6, batch * beams, kv_heads, PAGE_SIZE // 16, 2, packed_part_bytes(head_dim),
+                             dtype=torch.uint8, device=device)
+            table = torch.arange(batch * beams, dtype=torch.int32, device=device).view(-1, 1)
+            starts = torch.zeros(batch, dtype=torch.int32, device=device)
+            lengths = starts + PAGE_SIZE // 2
+            run = lambda i: ops.reorder_pages(kv, table, parents, starts, lengths, page_size=PAGE_SIZE)
+            work = f"{kv.numel() / 1e6:.1f} MB of pages"
     elif name in ("delta_prefill", "delta_short", "delta_decode"):
         # the gated delta rule alone: 16 heads of 128 x 128, a prompt of 2048 tokens (prepare,
         # chunks, walk, finish), `batch` portions of 48 tokens (prepare, scan, finish) or `batch`

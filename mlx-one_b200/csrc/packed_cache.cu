@@ -300,28 +300,70 @@ read_kernel(const unsigned char* cache, const int* positions,
     }
 }
 
-// The largest number, by its size, that the keys' and the values' part of 1,024 keys of a request and key head may
-// open to: largest [requests, open heads, 2, chunks].
-constexpr int CHUNK_UNITS = 64;
+// Queries as half-precision, a row times the power of two that brings its largest to 2^10 (exact but for what is
+// 2^-26 of the largest and less), whose inverse goes to `factors`. HD / 8 lanes a row, blocks of 256 threads.
+template <int HD>
+__device__ __forceinline__ void half_queries(const bf16* q, long long rows, uint4* out, float* factors,
+                                             long long block, long long blocks) {
+    constexpr int LANES = HD == 96 ? 16 : HD / 8, ROWS = 256 / LANES;
+    const bf16* written = settled(q);
+    const int sub = threadIdx.x % LANES;
+    for (long long first = block * ROWS; first < rows; first += blocks * ROWS) {      // (one for a block)
+        const long long row = first + threadIdx.x / LANES;
+        const bool live = row < rows && sub * 8 < HD;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = 0.f;
+        if (live) load_eight<bf16>(written + row * HD + sub * 8, true, x);
+        float most = 0.f, inverse;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (fabsf(x[i]) < INFINITY) most = fmaxf(most, fabsf(x[i]));
+#pragma unroll
+        for (int offset = 1; offset < LANES; offset <<= 1)
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, offset));
+        const float by = power_towards(most, 10, inverse);
+        if (!live) continue;
+        uint32_t pairs[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 pair = __floats2half2_rn(x[2 * i] * by, x[2 * i + 1] * by);
+            pairs[i] = *reinterpret_cast<const uint32_t*>(&pair);
+        }
+        out[row * (HD / 8) + sub] = make_uint4(pairs[0], pairs[1], pairs[2], pairs[3]);
+        if (sub == 0) factors[row] = inverse;
+    }
+}
 
+// What opening into half-precision has to know ahead: the largest number, by its size, that the keys' and the
+// values' part of `chunk_units` units of a request and key head may open to, largest [requests, open heads, 2,
+// chunks]. And the queries in half-precision, by the layers of the grid behind the requests'.
 template <int HD>
 __global__ void __launch_bounds__(256)
 range_kernel(const unsigned char* cache, const int* block_table, int table_width, int page_shift, int pages,
-                   const int* request_start, const int* history, int span, int first_request, int first_head,
-                   int kv_heads, float* largest) {
+             const int* request_start, const int* history, int span, int first_request, int requests, int first_head,
+             int kv_heads, int chunk_units, float* largest, const bf16* q, long long rows, uint4* halves,
+             float* query_factors) {
     using P = Packed<HD>;
     __shared__ float scratch[33];
     griddep_launch();
     griddep_wait();
+    if ((int)blockIdx.z >= requests) {
+        const long long layer = (long long)gridDim.x * gridDim.y;
+        half_queries<HD>(q, rows, halves, query_factors,
+                         (blockIdx.z - requests) * layer + blockIdx.y * gridDim.x + blockIdx.x,
+                         (gridDim.z - requests) * layer);
+        return;
+    }
     const unsigned char* from = settled(cache);
     const int chunk = blockIdx.x, head = first_head + blockIdx.y, request = first_request + blockIdx.z;
     const int held = history[request];
     const int length = held + request_start[request + 1] - request_start[request];
     const int lowest_key = first_visible_key(held, span), units = 1 << (page_shift - 4);
     float most[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = threadIdx.x; i < CHUNK_UNITS * 16; i += 256) {
-        const int first = (chunk * CHUNK_UNITS + i / 16) * 16, place = i % 16;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < chunk_units * 16; i += 256) {
+        const int first = (chunk * chunk_units + i / 16) * 16, place = i % 16;
         if (first + place / 2 + 8 * (place & 1) >= length || first + 15 < lowest_key) continue;
         const int block = first >> page_shift;
         const int page = block < table_width ? block_table[(size_t)request * table_width + block] : -1;
@@ -343,40 +385,6 @@ range_kernel(const unsigned char* cache, const int* block_table, int table_width
         if (threadIdx.x == 0)
             largest[(((size_t)blockIdx.z * gridDim.y + blockIdx.y) * 2 + k) * gridDim.x + chunk] = all;
     }
-}
-
-// Queries as half-precision, a row times the power of two that brings its largest to 2^10 (exact but for what is
-// 2^-26 of the largest and less), whose inverse goes to `factors`. HD / 8 lanes a row.
-template <int HD>
-__global__ void __launch_bounds__(256)
-half_queries_kernel(const bf16* q, long long rows, uint4* out, float* factors) {
-    constexpr int LANES = HD == 96 ? 16 : HD / 8;
-    griddep_launch();
-    griddep_wait();
-    const bf16* written = settled(q);
-    const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / LANES;
-    const int sub = threadIdx.x % LANES;
-    const bool live = row < rows && sub * 8 < HD;
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    if (live) load_eight<bf16>(written + row * HD + sub * 8, true, x);
-    float most = 0.f, inverse;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (fabsf(x[i]) < INFINITY) most = fmaxf(most, fabsf(x[i]));
-#pragma unroll
-    for (int offset = 1; offset < LANES; offset <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, offset));
-    const float by = power_towards(most, 10, inverse);
-    if (!live) return;
-    uint32_t pairs[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __half2 pair = __floats2half2_rn(x[2 * i] * by, x[2 * i + 1] * by);
-        pairs[i] = *reinterpret_cast<const uint32_t*>(&pair);
-    }
-    out[row * (HD / 8) + sub] = make_uint4(pairs[0], pairs[1], pairs[2], pairs[3]);
-    if (sub == 0) factors[row] = inverse;
 }
 
 // Requests opened: every unit that the requests' tables name, up to their last token, as plain values in
@@ -583,40 +591,54 @@ MLXONE_API int mlxone_read_key_values(const void* cache, const int* positions, c
     return 0;
 }
 
+// Units whose range a block looks for: 256 keys, more where a warp that opens would find more than 128 ranges.
+static int units_of_chunk(int blocks, int open_size) {
+    return 16 * ceil_div_host((long long)blocks * open_size, 256 * 128);
+}
+
 // Floats that mlxone_open_key_values needs as `factors` for half-precision pages.
 MLXONE_API long long mlxone_open_factors(int requests, int open_heads, int blocks, int open_size) {
     if (requests <= 0 || open_heads <= 0 || blocks <= 0 || open_size <= 0) return 0;
-    return 2LL * requests * open_heads * (1 + ceil_div_host((long long)blocks * open_size, 16 * CHUNK_UNITS));
+    return 2LL * requests * open_heads * (1 + ceil_div_host((long long)blocks * open_size, 16 * units_of_chunk(blocks, open_size)));
 }
 
 // Requests first_request.. (`requests` of them) and key heads first_head.. (`open_heads` of kv_heads), `blocks`
 // pages of `open_size` tokens (a multiple of 16) for each request: opened [2, requests * blocks, open_heads,
 // open_size, head_dim], table int32 [requests * blocks + requests + 1]. `span`: see first_visible_key; units that
 // no token of the step sees are zeros. factors: null, or (bfloat16) mlxone_open_factors floats: the pages are then
-// half-precision, and the first requests * open_heads * 2 of them are what keys and values are to be multiplied by.
+// half-precision, and the first requests * open_heads * 2 of them are what keys and values are to be multiplied by;
+// `rows` rows of q (bfloat16, head_dim values) go to `halves` and query_factors [rows] in the same manner.
 MLXONE_API int mlxone_open_key_values(const void* cache, const int* block_table, int table_width, int page_size,
                                       int pages, const int* request_start, const int* history, int span,
                                       int first_request, int requests, int kv_heads, int first_head,
                                       int open_heads, int head_dim, int blocks, int open_size, void* opened,
-                                      int* table, float* factors, int dtype, cudaStream_t stream) {
+                                      int* table, float* factors, const void* q, long long rows, void* halves,
+                                      float* query_factors, int dtype, cudaStream_t stream) {
     if (requests == 0) return 0;
     if (check_geometry("open_key_values", head_dim, page_size, pages, kv_heads, table_width, cache)) return 1;
     MLXONE_REQUIRE(requests > 0 && requests <= 65535 && first_request >= 0 && blocks > 0 && open_size >= 16 &&
                        open_size % 16 == 0 && first_head >= 0 && open_heads > 0 &&
                        first_head + open_heads <= kv_heads, "open_key_values: bad sizes");
-    MLXONE_REQUIRE(factors == nullptr || dtype == MLXONE_BF16, "open_key_values: half-precision pages for bfloat16 queries only");
+    MLXONE_REQUIRE(factors == nullptr || (dtype == MLXONE_BF16 && requests <= 65535 - 32 && rows >= 0 &&
+                                          (((size_t)q | (size_t)halves) & 15) == 0),
+                   "open_key_values: half-precision pages take bfloat16 queries that start at a multiple of 16 bytes");
     MLXONE_REQUIRE(((size_t)opened & 15) == 0, "open_key_values: the output starts at a multiple of 16 bytes");
     const long long half = (long long)requests * blocks * open_heads * open_size * head_dim;
     const int page_shift = 31 - __builtin_clz((unsigned)page_size);
-    const int chunks = ceil_div_host((long long)blocks * open_size, 16 * CHUNK_UNITS);
+    const int chunk_units = units_of_chunk(blocks, open_size);
+    const int chunks = ceil_div_host((long long)blocks * open_size, 16 * chunk_units);
     const unsigned char* held = (const unsigned char*)cache;
     float* largest = nullptr;
     if (factors != nullptr) {
         largest = factors + (size_t)requests * open_heads * 2;
+        // layers of the grid for the queries: a row by HD / 8 threads, once around for up to 32 layers
+        const long long row_blocks = ceil_div_host(rows, 256 / (head_dim == 96 ? 16 : head_dim / 8));
+        const int layers = std::min(ceil_div_host(row_blocks, (long long)chunks * open_heads), 32);
 #define CALL(HD)                                                                                          \
-    launch_kernel(range_kernel<HD>, dim3(chunks, open_heads, requests), dim3(256), 0, stream, true, \
+    launch_kernel(range_kernel<HD>, dim3(chunks, open_heads, requests + layers), dim3(256), 0, stream, true, \
                   held, block_table, table_width, page_shift, pages, request_start, history, span,        \
-                  first_request, first_head, kv_heads, largest)
+                  first_request, requests, first_head, kv_heads, chunk_units, largest, (const bf16*)q,     \
+                  rows, (uint4*)halves, query_factors)
         MLXONE_PACKED_DIMS(CALL)
 #undef CALL
         MLXONE_LAUNCH_CHECK("open_key_values range");
@@ -638,20 +660,5 @@ MLXONE_API int mlxone_open_key_values(const void* cache, const int* block_table,
     MLXONE_PACKED_DIMS(CALL)
 #undef CALL
     MLXONE_LAUNCH_CHECK("open_key_values");
-    return 0;
-}
-
-// q bfloat16 [rows, head_dim] -> out half-precision [rows, head_dim], factors float32 [rows].
-MLXONE_API int mlxone_half_queries(const void* q, long long rows, int head_dim, void* out, float* factors,
-                                   cudaStream_t stream) {
-    if (rows == 0) return 0;
-    MLXONE_REQUIRE(rows > 0 && (((size_t)q | (size_t)out) & 15) == 0,
-                   "half_queries: rows start at multiples of 16 bytes");
-#define CALL(HD)                                                                                              \
-    launch_kernel(half_queries_kernel<HD>, dim3(ceil_div_host(rows, 256 / (HD == 96 ? 16 : HD / 8))), dim3(256), 0, \
-                  stream, true, (const bf16*)q, rows, (uint4*)out, factors)
-    MLXONE_PACKED_DIMS(CALL)
-#undef CALL
-    MLXONE_LAUNCH_CHECK("half_queries");
     return 0;
 }

@@ -72,6 +72,10 @@ class CudaOps:
                 "mlxone_read_key_values": [*[pointer] * 4, *[whole] * 6, pointer, pointer, whole, pointer, pointer],
                 "mlxone_attention_packed": [*[pointer] * 3, *[whole] * 3, *[pointer] * 3, *[whole] * 5, real, whole,
                                             pointer, whole, pointer, pointer],
+                "mlxone_open_key_values": [pointer, pointer, *[whole] * 3, pointer, pointer, *[whole] * 9, *[pointer] * 4,
+                                           long, pointer, pointer, whole, pointer],
+                "mlxone_attention_prefill_tcgen05_half": [*[pointer] * 3, *[whole] * 3, *[pointer] * 3, *[whole] * 5,
+                                                          real, *[whole] * 3, pointer, pointer, whole, *[pointer] * 4],
                 "mlxone_beam_select": [pointer, long, *[whole] * 3, *[pointer] * 3, whole, *[pointer] * 5, pointer],
                 "mlxone_reorder_slots": [pointer, *[long] * 3, pointer, pointer, whole, whole, pointer, pointer],
                 "mlxone_reorder_pages": [pointer, *[long] * 3, pointer, whole, *[pointer] * 3, *[whole] * 3, pointer,
@@ -1758,11 +1762,12 @@ class CudaOps:
             # the other requests: the tables, starts and histories from request ``singles`` on
             # (token numbers in request_start stay those of the whole step)
             rest = ctx.requests - singles
-            table = view.block_table[singles:]
-            starts, history = ctx.request_start[singles:], ctx.history[singles:]
+            table, starts, history = view.block_table, ctx.request_start, ctx.history
+            if singles:
+                table, starts, history = table[singles:], starts[singles:], history[singles:]
             factors = ()
             if isinstance(view, OpenedView) and view.factors is not None:
-                factors = (_c_void_p(_ptr(view.query_factors)), _c_void_p(_ptr(view.factors)))
+                factors = (view.query_factors.data_ptr(), view.factors.data_ptr())
             if (self.tcgen05_attention and q.dtype == torch.bfloat16
                     and self.lib.mlxone_attention_tcgen05_supports(
                         _c_int(head_dim), _c_int(heads), _c_int(kv_heads), _c_int(view.page_size))):
@@ -1783,17 +1788,22 @@ class CudaOps:
                 if splits > 1:
                     partial = torch.empty(tokens * heads * splits * (head_dim + 2),
                                           dtype=torch.float32, device=self.device)
-                # (half-precision: an entry of its own, the factors besides)
-                self._call("mlxone_attention_prefill_tcgen05_half" if factors
-                           else "mlxone_attention_prefill_tcgen05_keep", _c_void_p(_ptr(q)),
-                           _c_void_p(_ptr(view.kv)), _c_void_p(_ptr(table)),
-                           _c_int(width), _c_int(view.page_size), _c_int(pages),
-                           _c_void_p(_ptr(starts)), _c_void_p(_ptr(history)),
-                           _c_void_p(_ptr(out)), _c_int(tokens), _c_int(rest),
-                           _c_int(heads), _c_int(kv_heads), _c_int(head_dim), _c_float(scale),
-                           _c_int(window or 0), _c_int(keep_first), _c_int(splits),
-                           _c_void_p(_ptr(partial)), _c_void_p(_ptr(sinks)), _c_int(keys),
-                           *factors, _c_void_p(_ptr(self.error_flag)))
+                if factors:
+                    self._launch(self.lib.mlxone_attention_prefill_tcgen05_half, q.data_ptr(), view.kv.data_ptr(),
+                                 table.data_ptr(), width, view.page_size, pages, starts.data_ptr(),
+                                 history.data_ptr(), out.data_ptr(), tokens, rest, heads, kv_heads, head_dim, scale,
+                                 window or 0, keep_first, splits, _ptr(partial), _ptr(sinks), keys, *factors,
+                                 self.error_flag.data_ptr())
+                else:
+                    self._call("mlxone_attention_prefill_tcgen05_keep", _c_void_p(_ptr(q)),
+                               _c_void_p(_ptr(view.kv)), _c_void_p(_ptr(table)),
+                               _c_int(width), _c_int(view.page_size), _c_int(pages),
+                               _c_void_p(_ptr(starts)), _c_void_p(_ptr(history)),
+                               _c_void_p(_ptr(out)), _c_int(tokens), _c_int(rest),
+                               _c_int(heads), _c_int(kv_heads), _c_int(head_dim), _c_float(scale),
+                               _c_int(window or 0), _c_int(keep_first), _c_int(splits),
+                               _c_void_p(_ptr(partial)), _c_void_p(_ptr(sinks)), _c_int(keys),
+                               _c_void_p(_ptr(self.error_flag)))
                 if partial is not None:
                     # (the leading single tokens are the decode kernel's: their rows stay)
                     skip = singles * heads * splits * (head_dim + 2)
@@ -1809,7 +1819,7 @@ class CudaOps:
                            _c_void_p(_ptr(out)), _c_int(tokens), _c_int(rest),
                            _c_int(heads), _c_int(kv_heads), _c_int(head_dim), _c_float(scale),
                            _c_int(window or 0), _c_int(keep_first), _c_void_p(_ptr(sinks)),
-                           *factors)
+                           *map(_c_void_p, factors))
             return out
         if (q.dtype == torch.float32 and not window and sinks is None
                 and self.lib.mlxone_attention_f32_supports(_c_int(head_dim), _c_int(heads),
@@ -2122,7 +2132,7 @@ class CudaOps:
                           sinks, keep_first, score_cap, slopes, least_slope) -> None:
         """The requests of a step behind the first ``singles``, whose keys are opened."""
         tokens, rest = q.shape[0], ctx.requests - singles
-        blocks = max(-(-bound // self.open_page), 1)
+        blocks, code = max(-(-bound // self.open_page), 1), _dtype_code(q.dtype)
         group, width = heads // kv_heads, view.block_table.shape[1]
         table = torch.empty(rest * blocks + rest + 1, dtype=torch.int32, device=self.device)
         queries, result = q, out
@@ -2149,29 +2159,26 @@ class CudaOps:
         numbers = table[:rest * blocks].view(rest, blocks)
         # Everything in half-precision: keys, values and weights then keep 11 bits, not bfloat16's 8 (portions of
         # 1,024 tokens behind 3,076 keys are off by 0.0017 of themselves, not 0.0036; 0.0016 is the result's own
-        # rounding; they take 85 us instead of 77, for the range of keys and values is looked for first). The kernels of shaped scores have no such form.
-        factors = query_factors = None
+        # rounding; they take 81 us instead of 77, for the range of keys and values is
+        # looked for first). The kernels of shaped scores have no such form.
+        given = factors = query_factors = None
         if q.dtype == torch.bfloat16 and self.tensor_core_attention and not score_cap and slopes is None:
             factors = torch.empty(self.lib.mlxone_open_factors(rest, at_once, blocks, self.open_page),
                                   dtype=torch.float32, device=self.device)
-            halves = torch.empty((queries.shape[0], heads, head_dim), dtype=q.dtype, device=self.device)
+            given, queries = queries, torch.empty((queries.shape[0], heads, head_dim), dtype=q.dtype, device=self.device)
             query_factors = torch.empty((queries.shape[0], heads), dtype=torch.float32, device=self.device)
-            self._call("mlxone_half_queries", _c_void_p(_ptr(queries)), _c_ll(query_factors.numel()), _c_int(head_dim),
-                       _c_void_p(_ptr(halves)), _c_void_p(_ptr(query_factors)))
-            queries = halves
-            self.launches += 1              # the range of keys and values
         for first in range(0, kv_heads, at_once):
             count = min(at_once, kv_heads - first)
             here = opened if count == at_once else opened.view(-1)[:opened.numel() // at_once * count].view(
                 2, rest * blocks, count, self.open_page, head_dim)
             # (windows with first positions that stay open everything)
-            self._call("mlxone_open_key_values", _c_void_p(_ptr(view.kv)), _c_void_p(_ptr(view.block_table)),
-                       _c_int(width), _c_int(view.page_size), _c_int(pages),
-                       _c_void_p(_ptr(ctx.request_start)), _c_void_p(_ptr(ctx.history)),
-                       _c_int(0 if keep_first else window), _c_int(singles), _c_int(rest), _c_int(kv_heads),
-                       _c_int(first), _c_int(count), _c_int(head_dim), _c_int(blocks),
-                       _c_int(self.open_page), _c_void_p(_ptr(here)), _c_void_p(_ptr(table)),
-                       _c_void_p(_ptr(factors)), _c_int(_dtype_code(q.dtype)))
+            self._launch(self.lib.mlxone_open_key_values, view.kv.data_ptr(), view.block_table.data_ptr(), width,
+                         view.page_size, pages, ctx.request_start.data_ptr(), ctx.history.data_ptr(),
+                         0 if keep_first else window, singles, rest, kv_heads, first, count, head_dim, blocks,
+                         self.open_page, here.data_ptr(), table.data_ptr(), _ptr(factors), _ptr(given),
+                         0 if given is None else query_factors.numel(), queries.data_ptr(), _ptr(query_factors), code)
+            self.launches += factors is not None          # the range of keys and values
+            given = None
             plain = OpenedView(here, numbers, self.open_page, view.need, factors, query_factors)
             own = slice(first * group, (first + count) * group)
             how = dict(heads=count * group, kv_heads=count, head_dim=head_dim, scale=scale, window=window, ctx=step,
