@@ -1,8 +1,9 @@
 // Keys and values of a step's tokens written to pages of 4-bit codes (packed_cache.cuh has the format),
 // read back, and whole requests opened into pages of plain values.
 //
-// Writing. For a group of a token's values: lowest = bfloat16(min), step = bfloat16(max(max - lowest, 0) / 15,
-// difference and quotient in 32 bits), code = (x - lowest) / step to the nearest whole number, ties to
+// Writing. For a group of a token's values: lowest = bfloat16(min), step = bfloat16(max(max - lowest, 0) * (1 / 15),
+// difference, inverse and product in 32 bits: not always the quotient's bits, so it is the product that defines
+// the format, as a tensor divided by the number 15 on this GPU), code = (x - lowest) / step to the nearest whole number, ties to
 // even, cut to 0..15. The codes are those of exact arithmetic on the stored lowest and step (codes_of). A group
 // with a value that is not finite, or whose range is none, gets NaN as step and lowest: it stays visible.
 #include <cuda_fp16.h>
@@ -181,7 +182,7 @@ pack_kernel(const T* keys, long long key_stride, const T* values,
         }
         const bf16 lowest_stored = __float2bfloat16_rn(least);
         const float lowest = __bfloat162float(lowest_stored);
-        const bf16 step_stored = __float2bfloat16_rn(fmaxf(most - lowest, 0.f) / 15.f);
+        const bf16 step_stored = __float2bfloat16_rn(fmaxf(most - lowest, 0.f) * (1.f / 15.f));
         const float step = __bfloat162float(step_stored);
         const bool fine = isfinite(least) && isfinite(most) && isfinite(lowest) && isfinite(step);
         const uint32_t mine = fine && step > 0.f ? codes_of<T>(x, lowest, step) : 0u;

@@ -46,7 +46,8 @@ def quantized(x):
     g = groups_of(dim)
     x = x.float().view(n, g, dim // g)
     low = x.amin(-1).bfloat16()
-    step = ((x.amax(-1) - low.float()).clamp(min=0) / 15).bfloat16()
+    # (a 32-bit product with the 32-bit inverse: division may round to the other side)
+    step = ((x.amax(-1) - low.float()).clamp(min=0) * torch.tensor(1 / 15)).bfloat16()
     fine = torch.isfinite(x).all(-1) & torch.isfinite(step.float()) & torch.isfinite(low.float())
     low = torch.where(fine, low.double(), math.nan)
     step = torch.where(fine, step.double(), math.nan)

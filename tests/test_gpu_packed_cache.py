@@ -77,6 +77,24 @@ def test_packing_and_reading(ops, dtype, dim, heads, page, portions, histories):
     ops.check_errors()
 
 
+def test_steps_next_to_a_border(ops):
+    """Ranges whose fifteenth is another bfloat16 by division than by a product with the inverse: the product's."""
+    span = torch.rand(1 << 23, generator=torch.Generator().manual_seed(0)) * 8
+    border = span[(span / 15).bfloat16() != (span * torch.tensor(1 / 15)).bfloat16()]
+    assert len(border) > 20
+    n = len(border)
+    ctx, table, kv, view = packed_case(1, 64, 16, [n], [0], F32, stale=0)
+    x = torch.rand(n, 1, 64, generator=torch.Generator().manual_seed(1)) * border.view(n, 1, 1)
+    x[:, 0, 3], x[:, 0, 60] = 0.0, border
+    plain.pack(kv, table.cpu(), 16, range(n), [0] * n, x, x)
+    x = x.view(n, 64).to(DEVICE)
+    ops.pack_key_values(x, x, ctx=ctx, view=view)
+    assert torch.equal(view.kv.cpu(), kv)
+    _, steps, _ = plain.quantized(x.cpu())
+    assert torch.equal(steps[:, 0].to(DEVICE), (x.amax(-1) / 15).bfloat16().double())
+    ops.check_errors()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_values_that_are_not_finite(ops, dtype):
     """A group with NaN, infinity or a range that no number holds reads as NaN; its neighbours do not."""
@@ -426,4 +444,35 @@ def test_portions_of_keys_and_queries_of_any_size(ops, dim, page, of_keys, of_qu
             bound = bound_of(both[:, :, h], q[t:t + n, 2 * h:2 * h + 2], dim ** -0.5, dim, BF16, held + n)["portion"]
             assert (got[t:t + n, 2 * h:2 * h + 2] - want[t:t + n, 2 * h:2 * h + 2]).abs().max() <= bound, (r, h)
         t += n
+    ops.check_errors()
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (96, 32), (128, 64), (32, 16)])
+@pytest.mark.parametrize("of_keys,of_queries,of_values", [(1e-30, 1e30, 1e-30), (1e-30, 1e-30, 1e30), (1e5, 1e-5, 2e4),
+                                                          (1e30, 1e-30, 1.0)])
+@pytest.mark.parametrize("dtype,window", [(BF16, 0), (BF16, 24), (F32, 0)])
+def test_single_tokens_of_any_size(ops, dim, page, of_keys, of_queries, of_values, dtype, window):
+    """Keys, queries and values beyond half-precision's range, a head's keys and values its own matter."""
+    histories = [0, 30, 300]
+    lengths = [h + 1 for h in histories]
+    whole, _, _ = make_batch(lengths, [0] * 3, page, DEVICE)
+    ctx, table, pages = make_batch([1] * 3, histories, page, DEVICE)
+    view = PackedView(torch.full((pages, 2, page // 16, 2, plain.part_bytes(dim)), 0xFF, dtype=torch.uint8, device=DEVICE),
+                      table, page, PagedKeyValues(2, dim))
+    keys, values = rows_of(333, 2, dim, F32, 3, 0.3), rows_of(333, 2, dim, F32, 4, 0.3)
+    keys[:, 1] *= 1e-3
+    values[:, 1] *= 1e3
+    keys, values = (keys * of_keys).to(dtype), (values * of_values).to(dtype)
+    ops.pack_key_values(keys.view(333, -1).to(DEVICE), values.view(333, -1).to(DEVICE), ctx=whole, view=view)
+    q = torch.randn(3, 4, dim, generator=torch.Generator().manual_seed(1)) * of_queries
+    q[:, 2:] *= 1e3
+    q = q.to(dtype)
+    got = ops.paged_attention(q.to(DEVICE), heads=4, kv_heads=2, head_dim=dim, scale=dim ** -0.5, window=window or None,
+                              ctx=ctx, view=view).view(3, 4, dim).cpu().double()
+    want = plain.attend(q, view.kv.cpu(), table.cpu(), page, [1] * 3, histories, 4, 2, dim ** -0.5, window=window)
+    for r, held in enumerate(lengths):
+        both = plain.read(view.kv.cpu(), table.cpu(), page, r, held, dim)
+        for h in range(2):
+            bound = bound_of(both[:, :, h], q[r, 2 * h:2 * h + 2], dim ** -0.5, dim, dtype, held)["single"]
+            assert (got[r, 2 * h:2 * h + 2] - want[r, 2 * h:2 * h + 2]).abs().max() <= bound, (r, h)
     ops.check_errors()
