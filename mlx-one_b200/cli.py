@@ -62,6 +62,8 @@ def generate_command(model, prompt, revision, offline, cache_dir, max_tokens, te
                 raise ValueError("a beam search has nothing to stream")
             results = engine.generate_beams_ids(ids, options, beams=beams, length_penalty=length_penalty,
                                                 prompt_text="" if token_ids else prompt)
+            if not results:
+                raise ValueError("no continuation of the prompt has a finite score")
             if as_json:
                 click.echo(json.dumps([r.to_dict() for r in results], sort_keys=True, indent=2))
             elif token_ids:

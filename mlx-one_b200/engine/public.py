@@ -595,7 +595,7 @@ class Engine:
                            **option_kwargs) -> list[BeamResult]:
         """Beam search: the ``beams`` (1 to 32) hypotheses with the largest sums of logarithms, which
         compete with hypotheses that have ended; ranked by sum / (tokens, an end token counted) **
-        ``length_penalty``, best first (fewer where there are fewer continuations). ``options`` name the
+        ``length_penalty`` (-10 to 10), best first (fewer where there are fewer continuations). ``options`` name the
         number of tokens and ``ignore_eos``; sampling and stop strings have no place here. The search holds
         the engine's turn to its end: other requests wait. It needs ``beams`` free requests of the cache and
         pages for prompt and tokens of each (``CacheCapacityError``)."""
@@ -605,6 +605,8 @@ class Engine:
         spec = self._loaded.spec
         if isinstance(beams, bool) or not isinstance(beams, int) or not 1 <= beams <= min(32, spec.vocab_size):
             raise ValueError(f"beams={beams!r}: expected an integer from 1 to {min(32, spec.vocab_size)}")
+        if not -10.0 <= length_penalty <= 10.0:
+            raise ValueError(f"length_penalty={length_penalty!r}: expected a number from -10 to 10")
         prompt = [int(t) for t in prompt_ids]
         if not prompt or len(prompt) >= spec.max_positions:
             raise ValueError(f"a prompt of {len(prompt)} tokens: expected 1 to {spec.max_positions - 1}")

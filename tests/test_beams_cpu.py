@@ -2,6 +2,7 @@
 plain kernels on the CPU."""
 
 import json
+import math
 
 import pytest
 import torch
@@ -133,6 +134,24 @@ def test_command_line(models, monkeypatch):
     monkeypatch.setattr(engines, "Engine", lambda model, **how: (_ for _ in ()).throw(ValueError(str(how["cache_config"].bits))))
     result = CliRunner().invoke(main, call + ["--cache-bits", "4"])
     assert "4" in result.output and result.exit_code != 0
+
+
+def test_penalties_and_searches_without_an_answer(models, monkeypatch):
+    import mlx_one_b200.engine as engines
+    from mlx_one_b200.cli import main
+
+    folder, loaded, plain = models["A"]
+    engine = engine_of(loaded)
+    for penalty in (math.nan, math.inf, -11, 300.0):
+        with pytest.raises(ValueError, match="length_penalty"):
+            engine.generate_beams_ids([1, 2], beams=2, length_penalty=penalty)
+    for penalty in (-10, 0, 10.0):
+        assert len(engine.generate_beams_ids([1, 2], beams=2, max_tokens=3, length_penalty=penalty)) == 2
+    monkeypatch.setattr(engine, "generate_beams_ids", lambda *a, **how: [])
+    monkeypatch.setattr(engines, "Engine", lambda model, **how: engine)
+    result = CliRunner().invoke(main, ["generate", str(folder), "5 17", "--token-ids", "--beams", "2"])
+    assert result.exit_code == 1 and "finite score" in result.output
+    engine.close()
 
 
 # ------------------------------------------------------------------ the cache

@@ -210,6 +210,18 @@ def test_beams_beside_requests(folders):
             4 * need.kv_heads * need.head_dim for need in engine.model.cache_needs.values() if hasattr(need, "kv_heads"))
 
 
+def test_a_search_that_fails_leaves_the_engine_usable(folders):
+    """A token outside the vocabulary is refused by the step function; the next search starts afresh."""
+    (prompt,) = prompts(301, (20,), seed=4)
+    with Engine(folders["D", BF16], cache_config=CacheConfig(block_size_tokens=16, capacity_tokens=1024, max_requests=4,
+                                                             bits=4)) as engine:
+        want = [(r.token_ids, r.score) for r in engine.generate_beams_ids(prompt, max_tokens=9, beams=3)]
+        with pytest.raises(ValueError, match="vocabulary"):
+            engine.generate_beams_ids([*prompt, 301 + 40], max_tokens=9, beams=3)
+        assert engine.cache.stats().requests == 0
+        assert [(r.token_ids, r.score) for r in engine.generate_beams_ids(prompt, max_tokens=9, beams=3)] == want
+
+
 ARCHITECTURES = [("galarax", "G1"), ("galarax", "G3"), ("galarax", "G5"), ("farorax", "F1"), ("farorax", "F6"),
                  ("lamisun", "L1"), ("lamisun", "L4"), ("tirudra", "T1"), ("tirudra", "T5"), ("susalorn", None),
                  ("zinizen", None)]
