@@ -35,6 +35,7 @@
 
 #include <type_traits>
 
+#include "by_words.cuh"
 #include "packed_cache.cuh"
 
 namespace cg = cooperative_groups;
@@ -795,3 +796,4 @@ MLXONE_API int mlxone_attention_packed(const void* q, const void* cache, const i
 #undef CALL
     return 0;
 }
+MLXONE_BY_WORDS(mlxone_attention_packed)

@@ -39,6 +39,7 @@
 #include <cuda.h>
 #include <cuda_fp16.h>
 
+#include "by_words.cuh"
 #include "common.cuh"
 #include "float_pairs.cuh"
 #include "score_shape.cuh"
@@ -1047,6 +1048,7 @@ MLXONE_API int mlxone_attention_prefill_tcgen05_half(const void* q, const void* 
                            partial, sinks, keys, error_flag, stream, keep_first, false, ScoreShape(),
                            query_factors, factors);
 }
+MLXONE_BY_WORDS(mlxone_attention_prefill_tcgen05_half)
 
 // ... with scores s that become cap tanh(s / cap) (cap 0: none) and then lose slopes[head] (float32
 // [heads] or null) times the distance between query and key

@@ -18,6 +18,7 @@
 // Reordering. In place: hypothesis b takes over what hypothesis parent(b) held, both of the same request. A
 // thread owns one place of the state and looks after all hypotheses of the request there: it reads what
 // moves, then writes it, so that cycles and several children of one parent need neither scratch nor order.
+#include "by_words.cuh"
 #include "common.cuh"
 
 namespace {
@@ -443,6 +444,7 @@ MLXONE_API int mlxone_beam_select(const float* logits, long long stride, int req
     MLXONE_LAUNCH_CHECK("beam_choice");
     return 0;
 }
+MLXONE_BY_WORDS(mlxone_beam_select)
 
 #define MLXONE_MOVE(KERNEL, V, ...)                                                                    \
     do {                                                                                               \
@@ -475,6 +477,7 @@ MLXONE_API int mlxone_reorder_slots(void* state, long long entries, long long sl
     MLXONE_LAUNCH_CHECK("reorder_slots");
     return 0;
 }
+MLXONE_BY_WORDS(mlxone_reorder_slots)
 
 // storage [outer, pages, bytes] in place; block_table int32 [requests * beams, table_width], -1 where there is no page;
 // pages of hypotheses of one request that differ in content differ in number, and no page that moves has two owners.
@@ -494,3 +497,4 @@ MLXONE_API int mlxone_reorder_pages(void* storage, long long outer, long long pa
     MLXONE_LAUNCH_CHECK("reorder_pages");
     return 0;
 }
+MLXONE_BY_WORDS(mlxone_reorder_pages)

@@ -8,6 +8,7 @@
 // with a value that is not finite, or whose range is none, gets NaN as step and lowest: it stays visible.
 #include <cuda_fp16.h>
 
+#include "by_words.cuh"
 #include "packed_cache.cuh"
 
 namespace {
@@ -567,6 +568,7 @@ MLXONE_API int mlxone_pack_key_values(const void* keys, long long key_stride, co
     MLXONE_LAUNCH_CHECK("pack_key_values");
     return 0;
 }
+MLXONE_BY_WORDS(mlxone_pack_key_values)
 
 MLXONE_API int mlxone_read_key_values(const void* cache, const int* positions, const int* token_request,
                                       const int* block_table, int table_width, int page_size, int pages,
@@ -591,6 +593,7 @@ MLXONE_API int mlxone_read_key_values(const void* cache, const int* positions, c
     MLXONE_LAUNCH_CHECK("read_key_values");
     return 0;
 }
+MLXONE_BY_WORDS(mlxone_read_key_values)
 
 // Units whose range a block looks for: 256 keys, more where a warp that opens would find more than 128 ranges.
 static int units_of_chunk(int blocks, int open_size) {
@@ -663,3 +666,4 @@ MLXONE_API int mlxone_open_key_values(const void* cache, const int* block_table,
     MLXONE_LAUNCH_CHECK("open_key_values");
     return 0;
 }
+MLXONE_BY_WORDS(mlxone_open_key_values)

@@ -13,6 +13,7 @@ products of the values' parts (24 bits of every value, sums in 32 bits).
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Any
 
 import torch
@@ -43,6 +44,10 @@ def _ptr(tensor: torch.Tensor | None) -> int | None:
     return None if tensor is None else tensor.data_ptr()
 
 
+def _address(tensor: torch.Tensor | None) -> int:
+    return 0 if tensor is None else tensor.data_ptr()
+
+
 class CudaOps:
     name = "cuda"
 
@@ -63,24 +68,15 @@ class CudaOps:
         self.lib.mlxone_gated_recurrence_scratch.restype = ctypes.c_longlong
         self.lib.mlxone_beam_scratch.restype = ctypes.c_longlong
         self.lib.mlxone_open_factors.restype = ctypes.c_longlong
-        # (entry points that small calls go through: their arguments are converted by ctypes, which costs a
-        # fraction of wrapping each of them here)
-        pointer, whole, long, real = _c_void_p, _c_int, _c_ll, _c_float
-        for name, kinds in {
-                "mlxone_pack_key_values": [pointer, long, pointer, long, *[pointer] * 4, *[whole] * 6, pointer, whole,
-                                           pointer, pointer],
-                "mlxone_read_key_values": [*[pointer] * 4, *[whole] * 6, pointer, pointer, whole, pointer, pointer],
-                "mlxone_attention_packed": [*[pointer] * 3, *[whole] * 3, *[pointer] * 3, *[whole] * 5, real, whole,
-                                            pointer, whole, pointer, pointer],
-                "mlxone_open_key_values": [pointer, pointer, *[whole] * 3, pointer, pointer, *[whole] * 9, *[pointer] * 4,
-                                           long, pointer, pointer, whole, pointer],
-                "mlxone_attention_prefill_tcgen05_half": [*[pointer] * 3, *[whole] * 3, *[pointer] * 3, *[whole] * 5,
-                                                          real, *[whole] * 3, pointer, pointer, whole, *[pointer] * 4],
-                "mlxone_beam_select": [pointer, long, *[whole] * 3, *[pointer] * 3, whole, *[pointer] * 5, pointer],
-                "mlxone_reorder_slots": [pointer, *[long] * 3, pointer, pointer, whole, whole, pointer, pointer],
-                "mlxone_reorder_pages": [pointer, *[long] * 3, pointer, whole, *[pointer] * 3, *[whole] * 3, pointer,
-                                         pointer]}.items():
-            getattr(self.lib, name).argtypes = kinds
+        # (entry points that small calls go through take their arguments in one block, see ``_launch``)
+        self._by_words = {}
+        for name, words in {"mlxone_pack_key_values": "18q", "mlxone_read_key_values": "15q",
+                            "mlxone_open_key_values": "25q", "mlxone_attention_packed": "14qd5q",
+                            "mlxone_attention_prefill_tcgen05_half": "14qd10q", "mlxone_beam_select": "15q",
+                            "mlxone_reorder_slots": "10q", "mlxone_reorder_pages": "14q"}.items():
+            function = getattr(self.lib, name + "_words")
+            function.argtypes = [ctypes.c_char_p]
+            self._by_words[name] = (function, struct.Struct(words).pack)
         if self.lib.mlxone_abi_version() != 1:
             raise KernelBuildError("the CUDA extension is of another version; rebuild it")
         self.error_flag = torch.zeros(1, dtype=torch.int32, device=self.device)
@@ -182,10 +178,11 @@ class CudaOps:
             raise KernelError(self.lib.mlxone_last_error().decode())
         self.launches += 1
 
-    def _launch(self, function, *args) -> None:
-        """``_call`` of an entry point whose argument types are declared (see ``__init__``): plain numbers
-        and addresses."""
-        if function(*args, self._stream()) != 0:
+    def _launch(self, name: str, *args) -> None:
+        """``_call`` of an entry point that takes its arguments as a block of 8-byte words
+        (csrc/by_words.cuh): plain numbers and addresses, 0 for none."""
+        function, pack = self._by_words[name]
+        if function(pack(*args, self._stream())) != 0:
             raise KernelError(self.lib.mlxone_last_error().decode())
         self.launches += 1
 
@@ -1789,10 +1786,10 @@ class CudaOps:
                     partial = torch.empty(tokens * heads * splits * (head_dim + 2),
                                           dtype=torch.float32, device=self.device)
                 if factors:
-                    self._launch(self.lib.mlxone_attention_prefill_tcgen05_half, q.data_ptr(), view.kv.data_ptr(),
+                    self._launch("mlxone_attention_prefill_tcgen05_half", q.data_ptr(), view.kv.data_ptr(),
                                  table.data_ptr(), width, view.page_size, pages, starts.data_ptr(),
                                  history.data_ptr(), out.data_ptr(), tokens, rest, heads, kv_heads, head_dim, scale,
-                                 window or 0, keep_first, splits, _ptr(partial), _ptr(sinks), keys, *factors,
+                                 window or 0, keep_first, splits, _address(partial), _address(sinks), keys, *factors,
                                  self.error_flag.data_ptr())
                 else:
                     self._call("mlxone_attention_prefill_tcgen05_keep", _c_void_p(_ptr(q)),
@@ -2050,7 +2047,7 @@ class CudaOps:
             self._need_rows(rows, dtype, what)
             if rows.shape != wanted:
                 raise KernelError(f"{what} of a step of {ctx.tokens} tokens must be {wanted}, got {tuple(rows.shape)}")
-        self._launch(self.lib.mlxone_pack_key_values, keys.data_ptr(), keys.stride(0), values.data_ptr(),
+        self._launch("mlxone_pack_key_values", keys.data_ptr(), keys.stride(0), values.data_ptr(),
                      values.stride(0), ctx.positions.data_ptr(), ctx.token_request.data_ptr(),
                      ctx.request_start.data_ptr(), table.data_ptr(), table.shape[1], view.page_size, pages,
                      need.kv_heads, need.head_dim, ctx.tokens, view.kv.data_ptr(), code,
@@ -2063,7 +2060,7 @@ class CudaOps:
         need, table = view.need, view.block_table
         keys = torch.empty((ctx.tokens, need.kv_heads, need.head_dim), dtype=dtype, device=self.device)
         values = torch.empty_like(keys)
-        self._launch(self.lib.mlxone_read_key_values, view.kv.data_ptr(), ctx.positions.data_ptr(),
+        self._launch("mlxone_read_key_values", view.kv.data_ptr(), ctx.positions.data_ptr(),
                      ctx.token_request.data_ptr(), table.data_ptr(), table.shape[1], view.page_size, pages,
                      need.kv_heads, need.head_dim, ctx.tokens, keys.data_ptr(), values.data_ptr(), code,
                      self.error_flag.data_ptr())
@@ -2122,10 +2119,10 @@ class CudaOps:
                 partial = torch.empty(singles * heads * splits * (head_dim + 2), dtype=torch.float32,
                                       device=self.device)
                 self.launches += 1          # the merge kernel
-            self._launch(self.lib.mlxone_attention_packed, q.data_ptr(), view.kv.data_ptr(),
+            self._launch("mlxone_attention_packed", q.data_ptr(), view.kv.data_ptr(),
                          view.block_table.data_ptr(), width, view.page_size, pages, ctx.positions.data_ptr(),
-                         out.data_ptr(), _ptr(partial), singles, heads, kv_heads, head_dim, splits, scale, window,
-                         _ptr(sinks), code, self.error_flag.data_ptr())
+                         out.data_ptr(), _address(partial), singles, heads, kv_heads, head_dim, splits, scale, window,
+                         _address(sinks), code, self.error_flag.data_ptr())
         return out
 
     def _opened_attention(self, q, out, singles, bound, heads, kv_heads, head_dim, scale, window, ctx, view, pages, *,
@@ -2172,11 +2169,11 @@ class CudaOps:
             here = opened if count == at_once else opened.view(-1)[:opened.numel() // at_once * count].view(
                 2, rest * blocks, count, self.open_page, head_dim)
             # (windows with first positions that stay open everything)
-            self._launch(self.lib.mlxone_open_key_values, view.kv.data_ptr(), view.block_table.data_ptr(), width,
+            self._launch("mlxone_open_key_values", view.kv.data_ptr(), view.block_table.data_ptr(), width,
                          view.page_size, pages, ctx.request_start.data_ptr(), ctx.history.data_ptr(),
                          0 if keep_first else window, singles, rest, kv_heads, first, count, head_dim, blocks,
-                         self.open_page, here.data_ptr(), table.data_ptr(), _ptr(factors), _ptr(given),
-                         0 if given is None else query_factors.numel(), queries.data_ptr(), _ptr(query_factors), code)
+                         self.open_page, here.data_ptr(), table.data_ptr(), _address(factors), _address(given),
+                         0 if given is None else query_factors.numel(), queries.data_ptr(), _address(query_factors), code)
             self.launches += factors is not None          # the range of keys and values
             given = None
             plain = OpenedView(here, numbers, self.open_page, view.need, factors, query_factors)
@@ -2254,8 +2251,8 @@ class CudaOps:
         if rows:
             scratch = torch.empty(self.lib.mlxone_beam_scratch(requests, beams, vocab), dtype=torch.uint8,
                                   device=self.device)
-            self._launch(self.lib.mlxone_beam_select, logits.data_ptr(), logits.stride(0), requests, beams, vocab,
-                         scores.data_ptr(), _ptr(ended), _ptr(end_tokens),
+            self._launch("mlxone_beam_select", logits.data_ptr(), logits.stride(0), requests, beams, vocab,
+                         scores.data_ptr(), _address(ended), _address(end_tokens),
                          0 if end_tokens is None else end_tokens.numel(), scratch.data_ptr(), chosen.data_ptr(),
                          parents.data_ptr(), tokens.data_ptr(), over.data_ptr())
             self.launches += 1              # the sums, then the choice
@@ -2280,7 +2277,7 @@ class CudaOps:
         if requests == 0 or state.numel() == 0:
             return
         entries, count = state.shape[:2]
-        self._launch(self.lib.mlxone_reorder_slots, state.data_ptr(), entries, count,
+        self._launch("mlxone_reorder_slots", state.data_ptr(), entries, count,
                      state.numel() // (entries * count) * state.element_size(), slots.data_ptr(), parents.data_ptr(),
                      requests, beams, self.error_flag.data_ptr())
 
@@ -2304,7 +2301,7 @@ class CudaOps:
         if requests == 0 or storage.numel() == 0 or block_table.shape[1] == 0:
             return
         outer, pages = storage.shape[:2]
-        self._launch(self.lib.mlxone_reorder_pages, storage.data_ptr(), outer, pages,
+        self._launch("mlxone_reorder_pages", storage.data_ptr(), outer, pages,
                      storage.numel() // (outer * pages) * storage.element_size(), block_table.data_ptr(),
                      block_table.shape[1], parents.data_ptr(), starts.data_ptr(), lengths.data_ptr(), page_size,
                      requests, beams, self.error_flag.data_ptr())
