@@ -162,11 +162,16 @@ pack_kernel(const T* keys, long long key_stride, const T* values,
     const int sub = threadIdx.x % LANES;                     // this thread's place in its row
     const bool live_lane = sub * 8 < HD;
     const int rows = 2 * count;                              // keys' rows, then values'
+    // (where a row goes is looked up beside its load, not behind it)
+    unsigned char* const whole_unit = whole >= 0 ? unit_of(whole) : nullptr;
     for (int base = 0; base < rows; base += blockDim.x / LANES) {
         const int row = base + threadIdx.x / LANES;
         const bool live = row < rows && live_lane;
         const int part = row >= count ? 1 : 0;
         const int t = first + (live ? row - part * count : 0);
+        const bool imaged = whole >= 0 && t >= whole && t < whole + 16;
+        const int key = live ? positions[t] & 15 : 0;
+        unsigned char* unit = imaged ? image : live ? unit_of(t) : nullptr;
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = 0.f;
@@ -197,13 +202,11 @@ pack_kernel(const T* keys, long long key_stride, const T* values,
         const uint32_t bytes = sub & 1 ? spread(other >> 16) | spread(mine >> 16) << 4
                                        : spread(mine & 0xffffu) | spread(other & 0xffffu) << 4;
         if (live) {
-            const bool imaged = whole >= 0 && t >= whole && t < whole + 16;
-            unsigned char* unit = imaged ? image : unit_of(t);
             if (unit == nullptr) {
                 atomicExch(error_flag, ERROR_WRITE);
             } else {
                 unit += part * P::PART;
-                const int key = positions[t] & 15, run = sub >> 1;
+                const int run = sub >> 1;
                 const uint32_t words = fine ? (uint32_t)__bfloat16_as_ushort(step_stored) |
                                                   (uint32_t)__bfloat16_as_ushort(lowest_stored) << 16
                                             : 0x7fc07fc0u;
@@ -222,12 +225,11 @@ pack_kernel(const T* keys, long long key_stride, const T* values,
     }
     if (whole >= 0) {
         __syncthreads();
-        unsigned char* unit = unit_of(whole);
-        if (unit == nullptr) {
+        if (whole_unit == nullptr) {
             if (threadIdx.x == 0) atomicExch(error_flag, ERROR_WRITE);
         } else {
             for (int i = threadIdx.x; i < P::UNIT / 16; i += blockDim.x)
-                reinterpret_cast<uint4*>(unit)[i] = reinterpret_cast<const uint4*>(image)[i];
+                reinterpret_cast<uint4*>(whole_unit)[i] = reinterpret_cast<const uint4*>(image)[i];
         }
     }
 }
