@@ -2749,7 +2749,8 @@ def main() -> int:
                              "lightning_decode, experts_sorted, latent_prefill, latent_decode, state_space_prefill, "
                              "state_space_decode, channel_conv_prefill, channel_delta_prefill, "
                              "channel_delta_decode, recurrence_prefill, recurrence_decode, "
-                             "shaped_attention_prefill, shaped_attention_decode, decode_step (the "
+                             "shaped_attention_prefill, shaped_attention_decode, packed_attention, packed_portion, "
+                             "pack_key_values, beam_select, reorder_pages, reorder_slots, decode_step (the "
                              "whole step, eager, for a launch list), decode_timeline (where "
                              "the graph-replayed step's time goes, kernel by kernel)")
     parser.add_argument("--dependent-launches", type=int, default=1,
