@@ -89,7 +89,8 @@ __device__ __forceinline__ int place_in_row(int t, int e) {
     return (t >> 8) * PART + (e >> 2) * 1024 + (t & 255) * 4 + (e & 3);
 }
 
-// maxima [rows, parts * 256]; sums [rows, parts, 2]: maximum (of x log2 e) and sum of 2^(x log2 e - maximum).
+// maxima [rows, parts * 256]; sums [rows, parts, 2]: maximum and sum of exp(x - maximum). The maximum is a logit as it
+// is, so that a token that is certain has the logarithm 0.
 __global__ void __launch_bounds__(WARPS * 32)
 beam_sums_kernel(const float* logits, long long stride, int vocab, int beams, const float* scores,
                  const unsigned char* ended, float* maxima, float* sums_out, int* arrived) {
@@ -126,15 +127,15 @@ beam_sums_kernel(const float* logits, long long stride, int vocab, int beams, co
             value[v][i] = logit_of(value[v][i]);
             most = fmaxf(most, value[v][i]);
         }
-    const float top = fmaxf(most * LOG2E, NOTHING);
+    const float top = fmaxf(most, NOTHING);
     float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < 8; ++v)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[i & 1] += fast_exp2(fmaf(value[v][i], LOG2E, -top));
+        for (int i = 0; i < 4; ++i) sum[i & 1] += fast_exp2((value[v][i] - top) * LOG2E);
     maxima[((size_t)row * parts + part) * (WARPS * 32) + threadIdx.x] = most;
     const float warp_top = warp_max(top);
-    const float warp_sum_ = warp_sum((sum[0] + sum[1]) * fast_exp2(top - warp_top));
+    const float warp_sum_ = warp_sum((sum[0] + sum[1]) * fast_exp2((top - warp_top) * LOG2E));
     if (lane == 0) {
         tops[warp] = warp_top;
         sums[warp] = warp_sum_;
@@ -142,7 +143,7 @@ beam_sums_kernel(const float* logits, long long stride, int vocab, int beams, co
     __syncthreads();
     if (warp == 0) {
         const float all = warp_max(lane < WARPS ? tops[lane] : NOTHING);
-        const float total = warp_sum(lane < WARPS ? sums[lane] * fast_exp2(tops[lane] - all) : 0.f);
+        const float total = warp_sum(lane < WARPS ? sums[lane] * fast_exp2((tops[lane] - all) * LOG2E) : 0.f);
         if (lane == 0) {
             sums_out[((size_t)row * parts + part) * 2] = all;
             sums_out[((size_t)row * parts + part) * 2 + 1] = total;
@@ -205,18 +206,19 @@ beam_choice_kernel(const float* logits, long long stride, int vocab, const float
         const float* x = logits + (size_t)row * stride;
         if (threadIdx.x == 0) chosen_count = listed = 0;
         if (warp == WARPS - 1) {
-            // the logarithm of the row's sum, times log2 e
+            // the logarithm of the row's sum
             const float* part_sums = settled(sums_in) + (size_t)row * parts * 2;
             float top = NOTHING, sum = 0.f;
             for (int i = lane; i < parts; i += 32) top = fmaxf(top, part_sums[i * 2]);
             top = warp_max(top);
-            for (int i = lane; i < parts; i += 32) sum += part_sums[i * 2 + 1] * fast_exp2(part_sums[i * 2] - top);
+            for (int i = lane; i < parts; i += 32) sum += part_sums[i * 2 + 1] * fast_exp2((part_sums[i * 2] - top) * LOG2E);
             sum = warp_sum(sum);
             // (the logarithm of what is left of the sum without its power of two, in 0..1, is off by 2^-24)
             int power = 0;
             const float rest = frexpf(sum, &power);
             if (lane == 0)
-                whole_of_row = sum > 0.f ? (double)top + (double)(power - 1) + (double)log2f(2.f * rest) : (double)NAN;
+                whole_of_row = sum > 0.f ? (double)top + ((double)(power - 1) + (double)log2f(2.f * rest)) * 0.6931471805599453094
+                                         : (double)NAN;
         }
         // the largest maxima that each warp sees, and what they bound
         const int each = (beams + WARPS - 1) / WARPS, offered = each * WARPS;
@@ -295,7 +297,7 @@ beam_choice_kernel(const float* logits, long long stride, int vocab, const float
             if (isfinite(whole)) {
                 const unsigned long long best = sorted[threadIdx.x];
                 token = place_of(best);
-                key = ordered((double)score + ((double)value_of(best) - whole * 0.6931471805599453094));
+                key = ordered((double)score + ((double)value_of(best) - whole));
             }
         }
     }

@@ -99,6 +99,37 @@ def test_rows_of_wider_ones_and_replays(ops):
         assert all(torch.equal(a, b) for a, b in zip(again, ops.beam_select(rows, held)))
 
 
+@pytest.mark.parametrize("beams", [7, 8, 9, 12, 31])
+def test_ties_numbers_and_replays_of_many_hypotheses(ops, beams):
+    """Both ways in which a request's rows hand their candidates over, a cluster's (up to eight) and the last block's."""
+    generator = torch.Generator().manual_seed(beams)
+    rows, vocab = 3 * beams, 8200
+    logits = torch.randint(0, 3, (rows, vocab), generator=generator).float()
+    scores = torch.randint(-2, 1, (3, beams), generator=generator).float()
+    check(ops, logits, scores)
+    logits = 3 * torch.randn(rows, vocab, generator=generator)
+    logits[0, 5], logits[1], logits[2, 8195], logits[3, 1:] = math.nan, -math.inf, math.inf, -math.inf
+    scores[1, 2], scores[2, 0], scores[2, 1] = math.nan, -math.inf, math.inf
+    ended = torch.rand(3, beams, generator=generator) < 0.4
+    check(ops, logits, scores)
+    check(ops, logits, scores, ended=ended)
+    x, held, over = logits.to(DEVICE), scores.to(DEVICE), ended.to(DEVICE)
+    ends = torch.tensor([3, 8], dtype=torch.int32, device=DEVICE)
+    ops.beam_select(x, held, ended=over, end_tokens=ends)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first = ops.beam_select(x, held, ended=over, end_tokens=ends)
+        second = ops.beam_select(x, first[0], ended=first[3], end_tokens=ends)
+    for _ in range(3):
+        x.copy_(torch.randn(rows, vocab, generator=generator).to(DEVICE))
+        graph.replay()
+        again = [y.clone() for y in (*first, *second)]
+        one = ops.beam_select(x, held, ended=over, end_tokens=ends)
+        two = ops.beam_select(x, one[0], ended=one[3], end_tokens=ends)
+        assert all(torch.equal(a, b) for a, b in zip(again, (*one, *two)))
+
+
 @pytest.mark.parametrize("beams", [1, 2, 4, 5, 8, 13, 16, 32])
 @pytest.mark.parametrize("shape,dtype", [((3, 40), torch.bfloat16), ((2, 1024), torch.float32), ((7,), torch.uint8),
                                          ((5, 3), torch.float32), ((70000,), torch.uint8)])
