@@ -38,7 +38,7 @@ namespace {
 constexpr int WARPS = 8;
 constexpr int MAX_BEAMS = 32;
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float NOTHING = -1e30f;
+constexpr float NOTHING = -3.402823466e38f;      // a maximum of no logits: the lowest number, so that differences stay numbers
 constexpr int ERROR_PARENT = 10;       // a parent, slot or page outside its range
 
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -175,7 +175,8 @@ beam_choice_kernel(const float* logits, long long stride, int vocab, const float
     __shared__ unsigned long long sorted[MAX_BEAMS];
     __shared__ int chosen[CHOSEN];
     __shared__ uint32_t bounds[MAX_BEAMS];                       // as ranked() orders
-    __shared__ double whole_of_row;
+    __shared__ double log_of_sum;                                // (the logarithm of the row's sum, less its maximum)
+    __shared__ float top_of_row;
     __shared__ int chosen_count, listed, is_last;
     griddep_launch();
     griddep_wait();
@@ -206,7 +207,6 @@ beam_choice_kernel(const float* logits, long long stride, int vocab, const float
         const float* x = logits + (size_t)row * stride;
         if (threadIdx.x == 0) chosen_count = listed = 0;
         if (warp == WARPS - 1) {
-            // the logarithm of the row's sum
             const float* part_sums = settled(sums_in) + (size_t)row * parts * 2;
             float top = NOTHING, sum = 0.f;
             for (int i = lane; i < parts; i += 32) top = fmaxf(top, part_sums[i * 2]);
@@ -216,9 +216,11 @@ beam_choice_kernel(const float* logits, long long stride, int vocab, const float
             // (the logarithm of what is left of the sum without its power of two, in 0..1, is off by 2^-24)
             int power = 0;
             const float rest = frexpf(sum, &power);
-            if (lane == 0)
-                whole_of_row = sum > 0.f ? (double)top + ((double)(power - 1) + (double)log2f(2.f * rest)) * 0.6931471805599453094
-                                         : (double)NAN;
+            if (lane == 0) {
+                top_of_row = top;
+                log_of_sum = sum > 0.f ? ((double)(power - 1) + (double)log2f(2.f * rest)) * 0.6931471805599453094
+                                       : (double)NAN;
+            }
         }
         // the largest maxima that each warp sees, and what they bound
         const int each = (beams + WARPS - 1) / WARPS, offered = each * WARPS;
@@ -231,7 +233,8 @@ beam_choice_kernel(const float* logits, long long stride, int vocab, const float
             if (lane == __ffs((int)have) - 1) left = 0;
         }
         __syncthreads();
-        const double whole = whole_of_row;
+        const double below = log_of_sum;
+        const float top = top_of_row;
         const uint32_t mine = lane < offered ? bounds[lane] : 0u;
         int ahead = 0;
         for (int k = 0; k < offered; ++k) ahead += bounds[k] > mine || (bounds[k] == mine && k < lane);
@@ -294,10 +297,10 @@ beam_choice_kernel(const float* logits, long long stride, int vocab, const float
         __syncthreads();
         if ((int)threadIdx.x < beams) {
             key = ordered(minus);
-            if (isfinite(whole)) {
+            if (isfinite(below)) {
                 const unsigned long long best = sorted[threadIdx.x];
                 token = place_of(best);
-                key = ordered((double)score + ((double)value_of(best) - whole));
+                key = ordered((double)score + ((double)value_of(best) - (double)top - below));
             }
         }
     }

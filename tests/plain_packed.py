@@ -159,7 +159,6 @@ def attend(q, kv, table, page_size, portions, histories, heads, kv_heads, scale,
 def choose(logits, scores, ended=None, end_tokens=()):
     """Lists per request of (score, parent, token, ended): the best candidates, ties to the lowest place."""
     requests, beams = scores.shape
-    vocab = logits.shape[1]
     out = []
     for r in range(requests):
         found = []
@@ -172,9 +171,10 @@ def choose(logits, scores, ended=None, end_tokens=()):
             x = torch.where(torch.isnan(x), -math.inf, x)
             whole = float(torch.logsumexp(x, 0))
             if not math.isfinite(s) or not math.isfinite(whole):
-                x = torch.full((vocab,), -math.inf, dtype=torch.float64)
-                whole = s = 0.0
-            total = s + (x - whole)
+                found += [(-math.inf, b, v, int(v in end_tokens)) for v in range(beams)]
+                continue
+            # (x - maximum - the logarithm: the maximum may be too large for the logarithm to count beside it)
+            total = s + torch.log_softmax(x, 0)
             order = torch.sort(x, descending=True, stable=True).indices[:beams].tolist()
             found += [(float(total[v]), b, v, int(v in end_tokens)) for v in order]
         found.sort(key=lambda c: (-c[0], c[1], 0))           # (stable: a hypothesis' own are in order)

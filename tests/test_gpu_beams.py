@@ -74,6 +74,24 @@ def test_rows_that_are_not_numbers(ops):
     check(ops, logits, scores, ended=torch.tensor([[0, 1, 0, 0], [1, 0, 0, 1], [0, 1, 0, 1]], dtype=torch.uint8))
 
 
+@pytest.mark.parametrize("beams,vocab", [(3, 37), (4, 9000), (12, 20011)])
+def test_masks_of_the_lowest_value(ops, beams, vocab):
+    """A row that a mask of the type's lowest value leaves nothing of has that many equal tokens; one that is left
+    in a row is certain; beside tokens of minus infinity the masked ones are what there is."""
+    lowest = torch.finfo(torch.float32).min
+    logits = torch.full((2 * beams, vocab), lowest)
+    logits[1, vocab - 2] = 0.25
+    logits[2, ::2] = -math.inf
+    logits[beams + 1] = torch.randn(vocab, generator=torch.Generator().manual_seed(vocab))
+    logits[beams + 2] = -math.inf
+    scores = -torch.arange(2.0 * beams).view(2, beams) / 8
+    check(ops, logits, scores)
+    got, parents, tokens, _ = ops.beam_select(logits[:1].expand(beams, -1).to(DEVICE),
+                                              torch.tensor([[0.0] + [-math.inf] * (beams - 1)], device=DEVICE))
+    assert tokens.tolist() == [list(range(beams))] and not parents.any()
+    torch.testing.assert_close(got, torch.full_like(got, -math.log(vocab)), atol=1e-5, rtol=2.0 ** -22)
+
+
 def test_rows_of_wider_ones_and_replays(ops):
     """Rows that are slices, at any alignment; a captured choice with other contents."""
     generator = torch.Generator().manual_seed(4)
