@@ -2134,10 +2134,12 @@ class CudaOps:
         table = torch.empty(rest * blocks + rest + 1, dtype=torch.int32, device=self.device)
         queries, result = q, out
         if singles:
-            # the rest as a step of its own (the 32-bit kernels go by token, the others by request)
+            # the rest as a step of its own. The tensor cores' kernels go by request, by the table's starts; those
+            # that go by token (in 32 bits, or with the tensor cores switched off) need the rest's positions
+            # and requests beside its queries (one more launch, which the others are spared).
             positions, token_request = ctx.positions, ctx.token_request
-            if q.dtype == torch.float32:
-                positions, token_request = positions[singles:], token_request[singles:tokens] - singles
+            if not (self.tensor_core_attention and self.lib.mlxone_attention_mma_supports(head_dim, code)):
+                positions, token_request = positions[singles:tokens], token_request[singles:tokens] - singles
             step = StepContext(tokens=tokens - singles, requests=rest, token_ids=positions, positions=positions,
                                token_request=token_request, request_start=table[rest * blocks:],
                                history=ctx.history[singles:], max_portion=0, max_context=ctx.max_context)

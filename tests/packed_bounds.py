@@ -1,0 +1,90 @@
+"""Attention over a cache held in 4 bits in 64 bits, and how far a kernel's output may be off, element by element,
+by the roundings that the kernel has."""
+
+import torch
+
+import plain_packed as plain
+
+# What a kernel rounds, each by at most half a step, relative to the value: the keys, the weights of the values and
+# the values. "codes": codes are exact, scores 32-bit, the weight times a value's step has 11 bits, a value's
+# lowest comes in 32 bits. "half": pages opened in half-precision. "bfloat16": opened in bfloat16, read by kernels
+# that keep weights in 32 bits; "shaped": by tensor cores, whose weights are bfloat16 too.
+HALF, BF16 = 2.0 ** -11, 2.0 ** -8
+FORMS = dict(codes=(0.0, HALF, 0.0), half=(HALF, HALF, HALF), bfloat16=(BF16, 0.0, BF16), shaped=(BF16, BF16, BF16))
+
+
+def parts(kv, table, page, request, length, dim):
+    """(keys, values, the values' part above their group's lowest), float64 [length, heads, dim]."""
+    keys, values = plain.read(kv, table, page, request, length, dim)
+    zero = kv.clone()
+    zero[..., :8 * dim] = 0                                  # codes of 0: what is left is the lowest value
+    return keys, values, values - plain.read(zero, table, page, request, length, dim)[1]
+
+
+def attend(q, kv, table, page, portions, histories, heads, kv_heads, scale, forms, *, window=0, chunk=0, keep_first=0,
+           sinks=None, cap=0.0, slopes=None):
+    """(wanted, bound), float64 [tokens, heads, dim]. ``forms``: a name of FORMS for every request.
+
+    With p the exact weights, o the exact output and e_j how far score j may be off, the weights are off by
+    expm1(e_j) of themselves, numerator and denominator alike, which moves o by p_j expm1(e_j) |v_j - o| a key; the
+    numerator's own roundings by p_j |v_j| (that of the weight and that of the value). e_j: the keys' rounding times
+    scale sum |q_d k_jd|, dim additions that may cut at 2^-23 each, 2^-22 of the largest score for the exponent's
+    argument, 2^-21 for the exponential. What is below half-precision's normal numbers (powers of two bring the
+    largest to 2^7 or more) is off by 2^-32 of the largest. A value's sum has a sixteenth as many additions as keys,
+    and 64 for the merges. The result is rounded once."""
+    out, bound, group, dim, t = [], [], heads // kv_heads, q.shape[-1], 0
+    for r, (n, held) in enumerate(zip(portions, histories)):
+        of_key, of_weight, of_value = FORMS[forms[r]]
+        length = held + n
+        keys, values, above = parts(kv, table, page, r, length, dim)
+        place = torch.arange(length)[None]
+        position = torch.arange(held, length)[:, None]
+        seen = place <= position
+        if window:
+            seen &= (place > position - window) | (place < keep_first)
+        if chunk:
+            seen &= place >= position - position % chunk
+        rows, bounds = [], []
+        for h in range(heads):
+            k, v = keys[:, h // group], values[:, h // group]
+            x = q[t:t + n, h].double()
+            s, size = scale * x @ k.T, scale * x.abs() @ k.abs().T
+            e = size * (of_key + dim * 2.0 ** -23) + scale * dim * x.abs().amax(-1, keepdim=True) * k.abs().max() * 2.0 ** -32
+            if cap:
+                s = cap * torch.tanh(s / cap)                # (its slope is at most 1; a polynomial, or two approximations)
+                e = e + cap * 2.0 ** -16
+            if slopes is not None:
+                s = s - slopes[h].double() * (position - place)
+            s = torch.where(seen, s, -torch.inf)
+            top = torch.where(seen, s.abs(), 0.0).amax(-1, keepdim=True)
+            all_ = s if sinks is None else torch.cat([s, sinks[h].double().expand(n, 1)], 1)
+            p = torch.softmax(all_, -1)[:, :length]
+            o = p @ v
+            delta = torch.expm1(e + top * 2.0 ** -22 + 2.0 ** -21)
+            worst = torch.where(seen, delta, 0.0).amax(-1, keepdim=True)
+            off = torch.einsum("nj,njd->nd", p * delta, (v[None] - o[:, None]).abs())
+            if sinks is not None:                            # (the sink's own weight, exact but for the exponential)
+                off = off + o.abs() * (1 - p.sum(-1, keepdim=True)) * (worst + 2.0 ** -20)
+            rounded = above[:, h // group].abs() if forms[r] == "codes" else v.abs()
+            sums = (length / 16 + 64) * 2.0 ** -23
+            off = off / (1 - worst).clamp(min=1e-9) + (1 + worst) * (p @ (rounded * (of_weight + of_value)) + p @ v.abs() * sums)
+            off = off * (1 + BF16) + length * 2.0 ** -32 * v.abs().max()
+            rows.append(o)
+            bounds.append(off + BF16 * (o.abs() + off))
+        out.append(torch.stack(rows, 1))
+        bound.append(torch.stack(bounds, 1))
+        t += n
+    return torch.cat(out), torch.cat(bound)
+
+
+def check(got, want, bound, portions, share):
+    """Every element within its bound, and every bound a small part of what it bounds: less than ``share`` of the
+    largest output of its request and head."""
+    t = 0
+    for r, n in enumerate(portions):
+        most = want[t:t + n].abs().amax((0, 2))
+        assert (bound[t:t + n].amax((0, 2)) < share * most).all(), (r, (bound[t:t + n].amax((0, 2)) / most).tolist())
+        if got is not None:
+            off = (got[t:t + n] - want[t:t + n]).abs()
+            assert (off <= bound[t:t + n]).all(), (r, float((off / bound[t:t + n]).max()))
+        t += n
