@@ -401,7 +401,9 @@ range_kernel(const unsigned char* cache, const int* block_table, int table_width
 // + b, of the key heads from first_head on; rows behind the last token, and of units without a page, are zeros,
 // so that no reader meets a number that is none. A token whose keys or values are none has NaN for its keys and
 // zeros for its values: queries that see it get NaN by their scores, the others nothing, since a reader drops
-// scores that are masked but multiplies every value. `table` gets the page numbers and, behind them, where the
+// scores that are masked but multiplies every value. A key that a token of the step sees (by `window`, or as one
+// of the first keep_first positions) but that has no page is told of: its row of zeros would count as a
+// key, for the readers do not look whether an opened row had a page. So are keys behind the last opened page. `table` gets the page numbers and, behind them, where the
 // requests' tokens start, counted from the first one's. With `largest` (range_kernel's, `chunks` of them each) the
 // pages are half-precision, keys and values times the powers of two that bring the largest of a request and key
 // head to 2^9, whose inverses go to `factors` [requests, open heads, 2]: 11 bits of every number of 2^-23 of the
@@ -410,9 +412,9 @@ range_kernel(const unsigned char* cache, const int* block_table, int table_width
 template <typename T, int HD>
 __global__ void __launch_bounds__(256)
 open_kernel(const unsigned char* cache, const int* block_table, int table_width, int page_shift, int pages,
-            const int* request_start, const int* history, int span, int first_request, int first_head, int kv_heads,
-            int blocks, int open_size, long long half, T* opened, int* table, const float* largest, int chunks,
-            float* factors) {
+            const int* request_start, const int* history, int span, int window, int keep_first, int first_request,
+            int first_head, int kv_heads, int blocks, int open_size, long long half, T* opened, int* table,
+            const float* largest, int chunks, float* factors, int* error_flag) {
     using P = Packed<HD>;
     constexpr int THREADS = 8 * P::RUNS;                         // of a unit
     griddep_launch();
@@ -444,6 +446,8 @@ open_kernel(const unsigned char* cache, const int* block_table, int table_width,
     if (open_head == 0 && inside == 0 && unit % per_block == 0) {
         table[(size_t)r * blocks + open_block] = r * blocks + open_block;
         if (unit == 0) {
+            // (keys behind the last opened page: `blocks` comes from a bound that the host knows)
+            if (length > held && (length - 1) / open_size >= blocks) atomicExch(error_flag, ERROR_READ);
             int* starts = table + (size_t)gridDim.z * blocks;
             const int base = request_start[first_request];
             starts[r] = request_start[request] - base;
@@ -457,6 +461,9 @@ open_kernel(const unsigned char* cache, const int* block_table, int table_width,
     const int block = first >> page_shift;
     int page = seen && block < table_width ? block_table[(size_t)request * table_width + block] : -1;
     if (page >= pages) page = -1;
+    if (page < 0 && first < length && length > held &&
+        (first + 15 >= first_visible_key(held, window) || first < keep_first) && open_head == 0 && inside == 0)
+        atomicExch(error_flag, ERROR_READ);
     uint32_t words[8];
     float step[4], lowest[4];
 #pragma unroll
@@ -615,16 +622,17 @@ MLXONE_API long long mlxone_open_factors(int requests, int open_heads, int block
 
 // Requests first_request.. (`requests` of them) and key heads first_head.. (`open_heads` of kv_heads), `blocks`
 // pages of `open_size` tokens (a multiple of 16) for each request: opened [2, requests * blocks, open_heads,
-// open_size, head_dim], table int32 [requests * blocks + requests + 1]. `span`: see first_visible_key; units that
-// no token of the step sees are zeros. factors: null, or (bfloat16) mlxone_open_factors floats: the pages are then
+// open_size, head_dim], table int32 [requests * blocks + requests + 1]. `window`: as first_visible_key's span; units
+// that no token of the step sees by it are zeros (with keep_first > 0, the first positions that stay visible
+// behind a window, none are). A key that some token sees and that has no page raises the error flag. factors: null, or (bfloat16) mlxone_open_factors floats: the pages are then
 // half-precision, and the first requests * open_heads * 2 of them are what keys and values are to be multiplied by;
 // `rows` rows of q (bfloat16, head_dim values) go to `halves` and query_factors [rows] in the same manner.
 MLXONE_API int mlxone_open_key_values(const void* cache, const int* block_table, int table_width, int page_size,
-                                      int pages, const int* request_start, const int* history, int span,
-                                      int first_request, int requests, int kv_heads, int first_head,
+                                      int pages, const int* request_start, const int* history, int window,
+                                      int keep_first, int first_request, int requests, int kv_heads, int first_head,
                                       int open_heads, int head_dim, int blocks, int open_size, void* opened,
                                       int* table, float* factors, const void* q, long long rows, void* halves,
-                                      float* query_factors, int dtype, cudaStream_t stream) {
+                                      float* query_factors, int dtype, int* error_flag, cudaStream_t stream) {
     if (requests == 0) return 0;
     if (check_geometry("open_key_values", head_dim, page_size, pages, kv_heads, table_width, cache)) return 1;
     MLXONE_REQUIRE(requests > 0 && requests <= 65535 && first_request >= 0 && blocks > 0 && open_size >= 16 &&
@@ -634,6 +642,8 @@ MLXONE_API int mlxone_open_key_values(const void* cache, const int* block_table,
                                           (((size_t)q | (size_t)halves) & 15) == 0),
                    "open_key_values: half-precision pages take bfloat16 queries that start at a multiple of 16 bytes");
     MLXONE_REQUIRE(((size_t)opened & 15) == 0, "open_key_values: the output starts at a multiple of 16 bytes");
+    MLXONE_REQUIRE(keep_first >= 0 && error_flag != nullptr, "open_key_values: bad arguments");
+    const int span = keep_first > 0 ? 0 : window;
     const long long half = (long long)requests * blocks * open_heads * open_size * head_dim;
     const int page_shift = 31 - __builtin_clz((unsigned)page_size);
     const int chunk_units = units_of_chunk(blocks, open_size);
@@ -660,14 +670,14 @@ MLXONE_API int mlxone_open_key_values(const void* cache, const int* block_table,
 #define CALL(HD)                                                                                          \
     if (dtype == MLXONE_BF16)                                                                             \
         launch_kernel(open_kernel<bf16, HD>, grid, dim3(per * HD / 2), 0, stream, true, held,             \
-                      block_table, table_width, page_shift, pages, request_start, history, span,          \
-                      first_request, first_head, kv_heads, blocks, open_size, half, (bf16*)opened, table, \
-                      (const float*)largest, chunks, factors);                                            \
+                      block_table, table_width, page_shift, pages, request_start, history, span, window,  \
+                      keep_first, first_request, first_head, kv_heads, blocks, open_size, half,           \
+                      (bf16*)opened, table, (const float*)largest, chunks, factors, error_flag);          \
     else                                                                                                  \
         launch_kernel(open_kernel<float, HD>, grid, dim3(per * HD / 2), 0, stream, true, held,            \
-                      block_table, table_width, page_shift, pages, request_start, history, span,          \
-                      first_request, first_head, kv_heads, blocks, open_size, half, (float*)opened,       \
-                      table, (const float*)nullptr, chunks, (float*)nullptr)
+                      block_table, table_width, page_shift, pages, request_start, history, span, window,  \
+                      keep_first, first_request, first_head, kv_heads, blocks, open_size, half,           \
+                      (float*)opened, table, (const float*)nullptr, chunks, (float*)nullptr, error_flag)
     MLXONE_PACKED_DIMS(CALL)
 #undef CALL
     MLXONE_LAUNCH_CHECK("open_key_values");

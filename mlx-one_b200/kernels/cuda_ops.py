@@ -71,7 +71,7 @@ class CudaOps:
         # (entry points that small calls go through take their arguments in one block, see ``_launch``)
         self._by_words = {}
         for name, words in {"mlxone_pack_key_values": "18q", "mlxone_read_key_values": "15q",
-                            "mlxone_open_key_values": "25q", "mlxone_attention_packed": "14qd5q",
+                            "mlxone_open_key_values": "27q", "mlxone_attention_packed": "14qd5q",
                             "mlxone_attention_prefill_tcgen05_half": "14qd10q", "mlxone_beam_select": "15q",
                             "mlxone_reorder_slots": "10q", "mlxone_reorder_pages": "14q"}.items():
             function = getattr(self.lib, name + "_words")
@@ -2085,7 +2085,8 @@ class CudaOps:
         each (all of a step of single tokens) go to the kernel that reads the codes themselves; the
         others are opened into pages of the compute dtype, a scratch of this call, which the prefill
         kernels read: a portion has many queries for every key that is opened. So do single tokens whose
-        scores are shaped or that see first positions behind a window."""
+        scores are shaped or that see first positions behind a window. Keys without a page: the kernel over
+        codes does not see them, opening one that is to be seen raises the error flag."""
         pages, code = self._need_packed(view), _dtype_code(q.dtype)
         self._need(q, q.dtype, "q")
         tokens, requests, width = q.shape[0], ctx.requests, view.block_table.shape[1]
@@ -2098,6 +2099,7 @@ class CudaOps:
         if chunk:
             window = self._span(window, chunk)
         window = int(window or 0)
+        keep_first = int(keep_first or 0) if window > 0 else 0
         if sinks is not None:
             self._need(sinks, torch.float32, "sinks")
             if sinks.numel() != heads:
@@ -2105,7 +2107,7 @@ class CudaOps:
         if out is None:
             out = torch.empty((tokens, heads * head_dim), dtype=q.dtype, device=self.device)
         singles = requests if ctx.max_portion == 1 and tokens == requests else min(ctx.leading_single, requests)
-        if score_cap or slopes is not None or (keep_first and window > 0):
+        if score_cap or slopes is not None or keep_first:
             singles = 0
         bound = min(ctx.max_context, width * view.page_size)
         if requests > singles and tokens > singles:
@@ -2170,12 +2172,12 @@ class CudaOps:
             count = min(at_once, kv_heads - first)
             here = opened if count == at_once else opened.view(-1)[:opened.numel() // at_once * count].view(
                 2, rest * blocks, count, self.open_page, head_dim)
-            # (windows with first positions that stay open everything)
             self._launch("mlxone_open_key_values", view.kv.data_ptr(), view.block_table.data_ptr(), width,
                          view.page_size, pages, ctx.request_start.data_ptr(), ctx.history.data_ptr(),
-                         0 if keep_first else window, singles, rest, kv_heads, first, count, head_dim, blocks,
+                         window, keep_first, singles, rest, kv_heads, first, count, head_dim, blocks,
                          self.open_page, here.data_ptr(), table.data_ptr(), _address(factors), _address(given),
-                         0 if given is None else query_factors.numel(), queries.data_ptr(), _address(query_factors), code)
+                         0 if given is None else query_factors.numel(), queries.data_ptr(), _address(query_factors), code,
+                         self.error_flag.data_ptr())
             self.launches += factors is not None          # the range of keys and values
             given = None
             plain = OpenedView(here, numbers, self.open_page, view.need, factors, query_factors)

@@ -8,6 +8,7 @@ import packed_bounds
 import plain_packed as plain
 from test_gpu_kernels import make_batch, ops  # noqa: F401  (fixture)
 from test_gpu_packed_cache import rows_of
+from mlx_one_b200.kernels import KernelError
 from mlx_one_b200.parts.base import PackedView, PagedKeyValues
 
 pytestmark = pytest.mark.gpu
@@ -53,3 +54,50 @@ def test_without_tensor_cores(ops, heads, kv_heads, dim, page, portions, histori
                        **(dict(cap=cap) if cap else {}))
     finally:
         ops.tensor_core_attention = held
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+@pytest.mark.parametrize("how,block,told", [
+    (dict(), 0, True), (dict(), 2, True), (dict(), 3, False), (dict(window=17), 0, False), (dict(window=18), 0, True),
+    (dict(window=17, keep_first=1), 0, True), (dict(window=1, keep_first=16), 1, False), (dict(chunk=32), 1, False),
+    (dict(chunk=64), 1, True), (dict(score_cap=5.0), 1, True)])
+def test_a_key_of_a_portion_without_a_page_is_told_of(ops, dtype, how, block, told):
+    """Opened pages hold zeros there, which their readers would take for a key: an error, unless no token of the
+    portion sees it. (Positions 32 to 39 behind 32 keys in pages of 16: the first sees back to 32 - window + 1.)"""
+    ctx, table, pages = make_batch([1, 8], [40, 32], 16, DEVICE)
+    ctx.leading_single = 1
+    view = PackedView(torch.zeros(pages, 2, 1, 2, 576, dtype=torch.uint8, device=DEVICE), table, 16, PagedKeyValues(2, 64))
+    q = torch.randn(9, 4, 64, device=DEVICE).to(dtype)
+    call = {**dict(heads=4, kv_heads=2, head_dim=64, scale=0.125, window=None, ctx=ctx, view=view), **how}
+    ops.paged_attention(q, **call)
+    ops.check_errors()                                       # (nothing is missing yet)
+    table[1, block] = -1
+    ops.paged_attention(q, **call)
+    if told:
+        with pytest.raises(KernelError, match="no page"):
+            ops.check_errors()
+    else:
+        ops.check_errors()
+    # a single token's key is not seen, without a word; nor are the keys of a request that brings no token
+    if "window" not in how and "chunk" not in how and "score_cap" not in how:
+        table[1, block] = pages - 1
+        table[0, 0] = -1
+        ctx.request_start[2] = 1
+        table[1, 0] = -1
+        ops.paged_attention(q, **call)
+        ops.check_errors()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+def test_keys_behind_the_bound_are_told_of(ops, dtype):
+    """A step whose ``max_context`` is less than what the device's numbers say."""
+    ctx, table, pages = make_batch([8], [122], 16, DEVICE)
+    view = PackedView(torch.zeros(pages, 2, 1, 2, 576, dtype=torch.uint8, device=DEVICE), table, 16, PagedKeyValues(2, 64))
+    q = torch.randn(8, 4, 64, device=DEVICE).to(dtype)
+    call = dict(heads=4, kv_heads=2, head_dim=64, scale=0.125, window=None, ctx=ctx, view=view)
+    ops.paged_attention(q, **call)
+    ops.check_errors()
+    ctx.max_context = 128                                    # (two opened pages of 64; position 129 is in the third)
+    ops.paged_attention(q, **call)
+    with pytest.raises(KernelError, match="no page"):
+        ops.check_errors()
