@@ -371,11 +371,12 @@ class Runner:
             max_portion = max(len(e.tokens) for e in entries)
             # (a loop's later steps run with this context too, their positions further on)
             later = loop[0] - 1 if loop is not None else 0
-            max_context = max(c.length + len(e.tokens) for c, e in zip(caches, entries)) + later
+            contexts = [c.length + len(e.tokens) + later for c, e in zip(caches, entries)]
+            max_context, rest_context = max(contexts), max(contexts[singles:], default=0)
             host = {"history": history, "request_start": starts}
         else:
             # bounds that hold for every step of this shape, however its tokens are split
-            max_portion = tokens - requests + 1
+            max_portion, rest_context = tokens - requests + 1, 0
             max_context = min([self.model.spec.max_positions] +
                               [w * self.cache.page_size for w, g in zip(widths, paged)
                                if g.need.window is None])
@@ -385,7 +386,8 @@ class Runner:
             positions=on_device("positions"), token_request=on_device("token_request"),
             request_start=on_device("request_start"), history=on_device("history"),
             max_portion=max_portion, max_context=max_context, views=views, host=host,
-            replayable=captured is not None and self.use_graphs, leading_single=singles)
+            replayable=captured is not None and self.use_graphs, leading_single=singles,
+            rest_context=rest_context)
 
         device_fed = any(e.from_device for e in entries)
 

@@ -151,8 +151,8 @@ class CudaOps:
         # 100; four of 64 tokens 54 / 50; 16 of 32 / 48 / 64 tokens 93 / 88, 139 / 121, 145 / 155. 8 heads:
         # 64 portions of 32 tokens 183 / 166; 16 of 64 82 / 87.
         self.delta_chunk_from = 64
-        # packed pages opened for a step's portions: tokens of an opened page, and bytes of scratch (a call
-        # that needs more takes some key heads after the others)
+        # packed pages opened for a step's portions: tokens of an opened page, and bytes of opened pages at a
+        # time (a call that needs more takes some key heads, or requests, after the others)
         self.open_page = 64
         self.open_bytes = 1 << 29
         self._packed_cluster = self.lib.mlxone_attention_packed_cluster()
@@ -2111,7 +2111,7 @@ class CudaOps:
             singles = 0
         bound = min(ctx.max_context, width * view.page_size)
         if requests > singles and tokens > singles:
-            self._opened_attention(q, out, singles, bound, heads, kv_heads, head_dim, scale, window, ctx, view, pages,
+            self._opened_attention(q, out, singles, heads, kv_heads, head_dim, scale, window, ctx, view, pages,
                                    sinks=sinks, keep_first=keep_first, score_cap=score_cap, slopes=slopes,
                                    least_slope=least_slope)
         if singles:
@@ -2127,12 +2127,38 @@ class CudaOps:
                          _address(sinks), code, self.error_flag.data_ptr())
         return out
 
-    def _opened_attention(self, q, out, singles, bound, heads, kv_heads, head_dim, scale, window, ctx, view, pages, *,
-                          sinks, keep_first, score_cap, slopes, least_slope) -> None:
-        """The requests of a step behind the first ``singles``, whose keys are opened."""
+    def _opened_attention(self, q, out, singles, heads, kv_heads, head_dim, scale, window, ctx, view, pages, **how) -> None:
+        """The requests of a step behind the first ``singles``, whose keys are opened. The pages that are opened at
+        a time take up to ``open_bytes``, or what one key head of one request takes if that is more: what needs
+        more goes some key heads after the others, or some requests."""
         tokens, rest = q.shape[0], ctx.requests - singles
-        blocks, code = max(-(-bound // self.open_page), 1), _dtype_code(q.dtype)
-        group, width = heads // kv_heads, view.block_table.shape[1]
+        width, code = view.block_table.shape[1], _dtype_code(q.dtype)
+        # (the keys of requests that are not opened need no room)
+        context = ctx.rest_context if singles and ctx.rest_context else ctx.max_context
+        blocks = max(-(-min(context, width * view.page_size) // self.open_page), 1)
+        each = 2 * blocks * self.open_page * head_dim * q.element_size()     # bytes of a request's key head
+        # (never as a step of single tokens: their kernels read pages ahead of the wait for the kernel before
+        # them, which here is the one that fills the pages)
+        longest = dict(max_portion=max(ctx.max_portion, 2), max_context=context)
+        at_once = max(self.open_bytes // each, 1)                            # requests, a key head of each
+        if rest > at_once:
+            # Some requests after the others, each time as a step of all tokens whose others belong to the first (or
+            # last) request's first position: how many tokens there are of each is for the device to know, and
+            # the tensor cores' kernels, which go by request, leave the others' rows alone.
+            owner = ctx.token_request[:tokens]
+            for first in range(singles, ctx.requests, at_once):
+                count = min(at_once, ctx.requests - first)
+                mine = (owner >= first) & (owner < first + count)
+                positions = torch.where(mine, ctx.positions[:tokens], 0)
+                step = StepContext(tokens=tokens, requests=count, token_ids=positions, positions=positions,
+                                   token_request=(owner - first).clamp_(0, count - 1),
+                                   request_start=ctx.request_start[first:], history=ctx.history[first:], **longest)
+                table = torch.empty(count * blocks + count + 1, dtype=torch.int32, device=self.device)
+                part = torch.empty_like(out)
+                self._attend_opened(q, part, step, first, table, blocks, heads, kv_heads, head_dim, scale, window, ctx,
+                                    view, pages, **how)
+                out.copy_(torch.where(mine[:, None], part, out))
+            return
         table = torch.empty(rest * blocks + rest + 1, dtype=torch.int32, device=self.device)
         queries, result = q, out
         if singles:
@@ -2144,18 +2170,23 @@ class CudaOps:
                 positions, token_request = positions[singles:tokens], token_request[singles:tokens] - singles
             step = StepContext(tokens=tokens - singles, requests=rest, token_ids=positions, positions=positions,
                                token_request=token_request, request_start=table[rest * blocks:],
-                               history=ctx.history[singles:], max_portion=0, max_context=ctx.max_context)
+                               history=ctx.history[singles:], **longest)
             queries, result = q.view(tokens, heads, head_dim)[singles:], out[singles:]
         else:
             step = StepContext(tokens=tokens, requests=rest, token_ids=ctx.token_ids, positions=ctx.positions,
                                token_request=ctx.token_request, request_start=ctx.request_start,
-                               history=ctx.history, max_portion=0, max_context=ctx.max_context)
-        # (never as a step of single tokens: their kernels read pages ahead of the wait for the kernel before
-        # them, which here is the one that fills the pages)
-        step.max_portion = max(ctx.max_portion, 2)
-        each = 2 * rest * blocks * self.open_page * head_dim * q.element_size()      # bytes a key head
+                               history=ctx.history, **longest)
+        self._attend_opened(queries, result, step, singles, table, blocks, heads, kv_heads, head_dim, scale, window, ctx,
+                            view, pages, **how)
+
+    def _attend_opened(self, queries, result, step, first_request, table, blocks, heads, kv_heads, head_dim, scale, window,
+                       ctx, view, pages, *, sinks, keep_first, score_cap, slopes, least_slope) -> None:
+        """Opens the keys of ``step.requests`` requests of ``ctx`` from ``first_request`` on, ``blocks`` pages of
+        each, and runs ``step`` over them. ``table``: where the opened pages' block table and the requests' starts go."""
+        rest, group, code = step.requests, heads // kv_heads, _dtype_code(queries.dtype)
+        each = 2 * rest * blocks * self.open_page * head_dim * queries.element_size()      # bytes a key head
         at_once = max(min(self.open_bytes // each, kv_heads), 1)
-        opened = torch.empty((2, rest * blocks, at_once, self.open_page, head_dim), dtype=q.dtype,
+        opened = torch.empty((2, rest * blocks, at_once, self.open_page, head_dim), dtype=queries.dtype,
                              device=self.device)
         numbers = table[:rest * blocks].view(rest, blocks)
         # Everything in half-precision: keys, values and weights then keep 11 bits, not bfloat16's 8 (portions of
@@ -2163,18 +2194,19 @@ class CudaOps:
         # rounding; they take 81 us instead of 77, for the range of keys and values is
         # looked for first). The kernels of shaped scores have no such form.
         given = factors = query_factors = None
-        if q.dtype == torch.bfloat16 and self.tensor_core_attention and not score_cap and slopes is None:
+        if queries.dtype == torch.bfloat16 and self.tensor_core_attention and not score_cap and slopes is None:
             factors = torch.empty(self.lib.mlxone_open_factors(rest, at_once, blocks, self.open_page),
                                   dtype=torch.float32, device=self.device)
-            given, queries = queries, torch.empty((queries.shape[0], heads, head_dim), dtype=q.dtype, device=self.device)
+            given, queries = queries, torch.empty((queries.shape[0], heads, head_dim), dtype=queries.dtype,
+                                                  device=self.device)
             query_factors = torch.empty((queries.shape[0], heads), dtype=torch.float32, device=self.device)
         for first in range(0, kv_heads, at_once):
             count = min(at_once, kv_heads - first)
             here = opened if count == at_once else opened.view(-1)[:opened.numel() // at_once * count].view(
                 2, rest * blocks, count, self.open_page, head_dim)
-            self._launch("mlxone_open_key_values", view.kv.data_ptr(), view.block_table.data_ptr(), width,
-                         view.page_size, pages, ctx.request_start.data_ptr(), ctx.history.data_ptr(),
-                         window, keep_first, singles, rest, kv_heads, first, count, head_dim, blocks,
+            self._launch("mlxone_open_key_values", view.kv.data_ptr(), view.block_table.data_ptr(),
+                         view.block_table.shape[1], view.page_size, pages, ctx.request_start.data_ptr(), ctx.history.data_ptr(),
+                         window, keep_first, first_request, rest, kv_heads, first, count, head_dim, blocks,
                          self.open_page, here.data_ptr(), table.data_ptr(), _address(factors), _address(given),
                          0 if given is None else query_factors.numel(), queries.data_ptr(), _address(query_factors), code,
                          self.error_flag.data_ptr())

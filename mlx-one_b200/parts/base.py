@@ -144,6 +144,9 @@ class StepContext:
     # shape, so it holds for every replay. A mixer may give these tokens to a kernel made for
     # single tokens and the rest to another.
     leading_single: int = 0
+    # largest history + portion of the requests behind the leading single tokens (host, as max_context);
+    # 0: no such bound, max_context holds for all
+    rest_context: int = 0
     # What a layer leaves for later layers of the same step, by name (a tensor of the step's tokens:
     # the values that later layers mix theirs with). Nothing of it outlives the step.
     shared: dict = field(default_factory=dict)

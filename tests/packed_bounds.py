@@ -8,9 +8,11 @@ import plain_packed as plain
 # What a kernel rounds, each by at most half a step, relative to the value: the keys, the weights of the values and
 # the values. "codes": codes are exact, scores 32-bit, the weight times a value's step has 11 bits, a value's
 # lowest comes in 32 bits. "half": pages opened in half-precision. "bfloat16": opened in bfloat16, read by kernels
-# that keep weights in 32 bits; "shaped": by tensor cores, whose weights are bfloat16 too.
-HALF, BF16 = 2.0 ** -11, 2.0 ** -8
-FORMS = dict(codes=(0.0, HALF, 0.0), half=(HALF, HALF, HALF), bfloat16=(BF16, 0.0, BF16), shaped=(BF16, BF16, BF16))
+# that keep weights in 32 bits; "shaped": by tensor cores, whose weights are bfloat16 too. "float32": everything in
+# 32 bits, four roundings each, over codes (less 8) as over opened pages.
+HALF, BF16, F32 = 2.0 ** -11, 2.0 ** -8, 2.0 ** -22
+FORMS = dict(codes=(0.0, HALF, 0.0), half=(HALF, HALF, HALF), bfloat16=(BF16, 0.0, BF16), shaped=(BF16, BF16, BF16),
+             float32=(F32, F32, F32))
 
 
 def parts(kv, table, page, request, length, dim):
@@ -30,11 +32,13 @@ def attend(q, kv, table, page, portions, histories, heads, kv_heads, scale, form
     numerator's own roundings by p_j |v_j| (that of the weight and that of the value). e_j: the keys' rounding times
     scale sum |q_d k_jd|, dim additions that may cut at 2^-23 each, 2^-22 of the largest score for the exponent's
     argument, 2^-21 for the exponential. What is below half-precision's normal numbers (powers of two bring the
-    largest to 2^7 or more) is off by 2^-32 of the largest. A value's sum has a sixteenth as many additions as keys,
-    and 64 for the merges. The result is rounded once."""
+    largest to 2^7 or more) is off by 2^-32 of the largest. A value's sum has a sixteenth as many additions as keys
+    (in 32 bits as many as keys), and 64 for the merges, of the value and of what is above its group's lowest. The
+    result is rounded once."""
     out, bound, group, dim, t = [], [], heads // kv_heads, q.shape[-1], 0
     for r, (n, held) in enumerate(zip(portions, histories)):
         of_key, of_weight, of_value = FORMS[forms[r]]
+        of_result = 2.0 ** -24 if forms[r] == "float32" else BF16
         length = held + n
         keys, values, above = parts(kv, table, page, r, length, dim)
         place = torch.arange(length)[None]
@@ -66,11 +70,12 @@ def attend(q, kv, table, page, portions, histories, heads, kv_heads, scale, form
             if sinks is not None:                            # (the sink's own weight, exact but for the exponential)
                 off = off + o.abs() * (1 - p.sum(-1, keepdim=True)) * (worst + 2.0 ** -20)
             rounded = above[:, h // group].abs() if forms[r] == "codes" else v.abs()
-            sums = (length / 16 + 64) * 2.0 ** -23
-            off = off / (1 - worst).clamp(min=1e-9) + (1 + worst) * (p @ (rounded * (of_weight + of_value)) + p @ v.abs() * sums)
+            sums = (length / (1 if forms[r] == "float32" else 16) + 64) * 2.0 ** -23
+            off = off / (1 - worst).clamp(min=1e-9) + (1 + worst) * (
+                p @ (rounded * (of_weight + of_value)) + p @ (v.abs() + above[:, h // group].abs()) * sums)
             off = off * (1 + BF16) + length * 2.0 ** -32 * v.abs().max()
             rows.append(o)
-            bounds.append(off + BF16 * (o.abs() + off))
+            bounds.append(off + of_result * (o.abs() + off))
         out.append(torch.stack(rows, 1))
         bound.append(torch.stack(bounds, 1))
         t += n

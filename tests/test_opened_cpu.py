@@ -37,10 +37,10 @@ class Ops(CudaOps):
         if isinstance(view, PackedView):
             return super().paged_attention(q, view=view, out=out, **how)
         assert isinstance(view, PagedView)
-        # (a number that tells whose row it is: the query's own first value)
+        # (a row tells whose query it is and in which call it was answered)
         rows = q.reshape(how["ctx"].tokens, how["heads"], how["head_dim"])
         self.read.append((rows.clone(), view, how))
-        got = rows[:, :, :1].expand(-1, -1, how["head_dim"]).reshape(how["ctx"].tokens, -1).clone()
+        got = (rows[:, :, :1] + 64 * len(self.read)).expand(-1, -1, how["head_dim"]).reshape(how["ctx"].tokens, -1).clone()
         if out is None:
             return got
         out.copy_(got)
@@ -84,3 +84,85 @@ def test_a_row_goes_with_its_own_position_and_request(dtype, tensor_cores, porti
     assert torch.equal(inner.token_request, ctx.token_request[leading:] - leading)
     assert 0 <= int(inner.token_request.min()) and int(inner.token_request.max()) < view.block_table.shape[0]
     assert rows[:, 0, 0].tolist() == list(range(leading, ctx.tokens))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("room,requests", [(1 << 29, 5), (1, 1), (2.5, 2), (11, 5)])
+def test_opened_pages_stay_within_their_room(dtype, room, requests):
+    """``open_bytes`` holds for all that is opened at a time, whatever of it is many: ``room`` key heads of one
+    request allow ``requests`` requests at once, and as many key heads of these as there is room for. Every row is answered with its own request's keys."""
+    portions, histories, leading = [1, 1, 3, 1, 5, 2, 4], [9, 70, 100, 0, 20, 6, 40], 2
+    ops, ctx = Ops(), step(portions, histories, leading)
+    ops.tensor_core_attention = False
+    blocks, each = 2, 2 * 2 * 64 * 32 * torch.empty((), dtype=dtype).element_size()
+    ops.open_bytes = int(room * each) if room < 1 << 29 else room
+    out = torch.full((ctx.tokens, 8 * 32), -1.0, dtype=dtype)
+    attend(ops, ctx, dtype, kv_heads=4, out=out)
+    calls = 0
+    for first in range(leading, len(portions), requests):
+        count = min(requests, len(portions) - first)
+        heads = max(min(int(room // count), 4), 1)
+        for head in range(0, 4, heads):
+            rows, view, how = ops.read[calls]
+            inner, calls = how["ctx"], calls + 1
+            assert view.kv.shape == (2, count * blocks, heads, 64, 32) and inner.requests == count
+            assert view.kv.numel() * view.kv.element_size() <= max(ops.open_bytes, each)
+            opening = [args for name, args in ops.launched if name == "mlxone_open_key_values"][calls - 1]
+            assert opening[9:13] == (first, count, 4, head)
+            mine = (ctx.token_request >= first) & (ctx.token_request < first + count)
+            if inner.tokens != ctx.tokens:                   # (all of the rest at once: the rest by itself)
+                mine = mine[leading:]
+                assert mine.all() and count == len(portions) - leading
+            skipped = ctx.tokens - inner.tokens
+            assert torch.equal(inner.positions[mine], ctx.positions[skipped:][mine])
+            assert torch.equal(inner.token_request[mine], ctx.token_request[skipped:][mine] - first)
+            # (no row reads outside the table, and tokens of one request stay neighbours)
+            assert 0 <= int(inner.token_request.min()) and int(inner.token_request.max()) < count
+            assert (inner.token_request.diff() >= 0).all() and inner.positions.min() >= 0
+            assert (inner.positions[~mine] == 0).all()
+            if skipped == 0:
+                assert torch.equal(inner.history, ctx.history[first:])
+                assert torch.equal(inner.request_start, ctx.request_start[first:])
+            for t in torch.nonzero(ctx.token_request.ge(first) & ctx.token_request.lt(first + count)).view(-1).tolist():
+                got = out[t].view(8, 32)[2 * head:2 * (head + heads)]
+                assert (got == t + 64 * calls).all(), (t, calls)
+    assert calls == len(ops.read)
+    assert (out[:leading] == -1).all()                       # (the single tokens' kernel's)
+
+
+def test_room_for_the_keys_that_are_opened():
+    """A long single token beside short portions: pages for the portions' keys only, where the step says how long they are."""
+    portions, histories = [1, 20, 30], [5000, 0, 10]
+    for rest, blocks in ((40, 1), (0, 79)):
+        ops, ctx = Ops(), step(portions, histories, 1)
+        ctx.rest_context = rest
+        attend(ops, ctx, torch.float32, width=400)
+        (_, view, how), = ops.read
+        assert view.block_table.shape == (2, blocks) and how["ctx"].max_context == (rest or 5001)
+    # single tokens whose scores are shaped are opened too
+    ops, ctx = Ops(), step(portions, histories, 1)
+    ctx.rest_context = 40
+    attend(ops, ctx, torch.float32, width=400, score_cap=5.0)
+    assert ops.read[0][1].block_table.shape == (3, 79)
+
+
+def test_a_step_says_how_long_its_portions_are(tmp_path):
+    """The runner's bound of the requests behind the leading single tokens."""
+    from mlx_one_b200.cache import CacheManager
+    from mlx_one_b200.engine.loading import load_model
+    from mlx_one_b200.engine.runner import Runner, StepEntry
+    from plain_ops import PlainOps
+    from tiny_models import make_model_dir
+
+    model = load_model(make_model_dir("A", tmp_path, dtype=torch.float32), "float32", "cpu", ops=PlainOps()).model
+    cache = CacheManager(model.cache_needs, page_size=4, capacity_tokens=256, max_requests=4, dtype=torch.float32,
+                         device="cpu")
+    runner = Runner(model, cache)
+    steps, forward = [], model.forward
+    model.forward = lambda ctx: steps.append(ctx) or forward(ctx)
+    for request in "abc":
+        cache.open(request)
+    runner.step([StepEntry("a", [3] * 40, (39,))])
+    runner.step([StepEntry("a", [3], (0,)), StepEntry("b", [3] * 5, (4,)), StepEntry("c", [3] * 7, (6,))])
+    runner.step([StepEntry("a", [3], (0,)), StepEntry("b", [3], (0,))])
+    assert [(c.leading_single, c.rest_context, c.max_context) for c in steps] == [(0, 40, 40), (1, 7, 41), (2, 0, 42)]
