@@ -27,8 +27,8 @@ def attention_case(ops, heads, kv_heads, dim, page, portions, histories, forms, 
         both = [rows_of(n, kv_heads, dim, torch.float32, 10 * r + seed + 5 * which, 0.3) for which in (0, 1)]
         plain.pack(kv, table.cpu(), page, range(n), [r] * n, (both[0] * of_keys).to(dtype), (both[1] * of_values).to(dtype))
     q = (torch.randn(ctx.tokens, heads, dim, generator=torch.Generator().manual_seed(seed + 1)) * of_queries).to(dtype)
-    want, bound = packed_bounds.attend(q, kv, table.cpu(), page, portions, histories, heads, kv_heads, dim ** -0.5, forms,
-                                       **how)
+    want, bound, variance = packed_bounds.attend(q, kv, table.cpu(), page, portions, histories, heads, kv_heads, dim ** -0.5, forms,
+                                                 **how)
     call = dict(how, scale=dim ** -0.5, ctx=ctx, view=PackedView(kv.to(DEVICE), table, page, PagedKeyValues(kv_heads, dim)))
     if "cap" in call:
         call["score_cap"] = call.pop("cap")
@@ -39,6 +39,10 @@ def attention_case(ops, heads, kv_heads, dim, page, portions, histories, forms, 
                               **{"window": None, **call}).view(ctx.tokens, heads, dim).cpu().double()
     ops.check_errors()
     packed_bounds.check(got, want, bound, portions, share or (0.25 if {"bfloat16", "shaped"} & set(forms) else 0.06))
+    by_token = [form for n, form in zip(portions, forms) for _ in range(n)]
+    for form in {"codes", "half"} & set(forms):
+        rows = torch.tensor([f == form for f in by_token])
+        packed_bounds.check_mean(got[rows], want[rows], variance[rows], heads // kv_heads)
     return got
 
 
@@ -167,3 +171,62 @@ def test_portions_beside_a_long_single_token(ops):
     portions, histories, forms = [1, 20, 30], [4000, 0, 10], ["codes", "half", "half"]
     for bound in (0, 40):
         attention_case(ops, 8, 2, 64, 16, portions, histories, forms, leading=1, rest_context=bound, share=0.1)
+
+
+SHAPES = [(8, 2, 64, 16), (4, 4, 32, 16), (12, 1, 96, 32), (10, 2, 128, 64), (3, 1, 64, 128), (16, 2, 64, 16)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", SHAPES)
+@pytest.mark.parametrize("histories", [[0], [14, 15, 16, 31, 32], [300, 0, 5, 127], [1500, 33]])
+@pytest.mark.parametrize("window,with_sinks", [(0, False), (33, True)])
+def test_single_tokens(ops, dtype, heads, kv_heads, dim, page, histories, window, with_sinks):
+    """One token a request over codes: weights times steps of 11 bits, everything else in 32."""
+    sinks = torch.linspace(-1, 1, heads) if with_sinks else None
+    forms = ["float32" if dtype == F32 else "codes"] * len(histories)
+    attention_case(ops, heads, kv_heads, dim, page, [1] * len(histories), histories, forms, dtype=dtype, window=window,
+                   sinks=sinks, seed=3)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", SHAPES)
+@pytest.mark.parametrize("portions,histories,leading", [
+    ([5], [0], 0), ([1, 1, 37], [40, 9, 0], 2), ([70, 1, 16], [3, 100, 200], 0), ([1, 130], [15, 65], 1), ([300], [700], 0)])
+@pytest.mark.parametrize("window,with_sinks", [(0, False), (40, False), (0, True), (50, True)])
+def test_portions(ops, dtype, heads, kv_heads, dim, page, portions, histories, leading, window, with_sinks):
+    """Opened in half-precision: 11 bits of keys, weights and values."""
+    sinks = torch.linspace(-1, 1, heads) if with_sinks else None
+    forms = ["float32"] * len(portions) if dtype == F32 else ["codes"] * leading + ["half"] * (len(portions) - leading)
+    attention_case(ops, heads, kv_heads, dim, page, portions, histories, forms, leading=leading, dtype=dtype, window=window,
+                   sinks=sinks, seed=4)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("portions,histories,leading", [([1, 1], [40, 90], 2), ([30, 1], [50, 7], 0), ([1, 60], [90, 40], 1)])
+@pytest.mark.parametrize("how", [dict(cap=20.0), dict(cap=5.0, slopes=SLOPES), dict(slopes=SLOPES), dict(chunk=32),
+                                 dict(window=24, keep_first=5)])
+def test_shaped_scores(ops, dtype, portions, histories, leading, how):
+    """Caps and slopes: opened in bfloat16, single tokens too. First positions: in half-precision. Chunks: as without."""
+    form = "float32" if dtype == F32 else "half" if "chunk" in how or "keep_first" in how else "shaped"
+    forms = [form] * len(portions)
+    if "chunk" in how and dtype == BF16:
+        forms[:leading] = ["codes"] * leading
+    attention_case(ops, 6, 2, 64, 16, portions, histories, forms, leading=leading, dtype=dtype, seed=5, **how)
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (96, 32), (128, 64), (32, 16)])
+@pytest.mark.parametrize("of_keys,of_queries,of_values", [
+    (1e-30, 1e30, 1e-30), (1e-30, 1e-30, 1e30), (1e5, 1e-5, 2e4), (1e30, 1e-30, 1.0)])
+@pytest.mark.parametrize("window", [0, 24])
+def test_any_size(ops, dim, page, of_keys, of_queries, of_values, window):
+    """Beyond half-precision's range: everything is times powers of two of its own."""
+    attention_case(ops, 8, 2, dim, page, [1, 40, 21], [300, 30, 100], ["codes", "half", "half"], leading=1, window=window,
+                   seed=6, of_keys=of_keys, of_queries=of_queries, of_values=of_values)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(8, 4, 64, 16), (8, 4, 128, 32), (8, 4, 32, 16), (8, 4, 96, 16)])
+def test_roundings_in_the_mean(ops, heads, kv_heads, dim, page):
+    """Rows enough to tell 8 bits of the keys alone from 11, and over opened pages of the values alone (computed with them
+    the ratio is 1.2 to 2.7, with 11 bits 0.93 to 0.97)."""
+    attention_case(ops, heads, kv_heads, dim, page, [1] * 16 + [60] * 6, [300] * 16 + [250] * 6, ["codes"] * 16 + ["half"] * 6,
+                   leading=16, seed=7)
