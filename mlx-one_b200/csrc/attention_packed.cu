@@ -21,8 +21,10 @@
 // of the values; the codes are centred (code - 8, exact in bfloat16) and the outputs added up in 32-bit
 // registers, tile by tile, so that no sum is longer or larger than it must be.
 //
-// What bounds it: the bytes of the codes, 72 a key and key head of 64 (keys and values), against 290 instructions
-// of a warp for 32 keys, half of them shifts, masks and maxima that issue every other cycle. One block = one
+// What bounds it: latency. Of the time of 32 requests of 4,096 keys, the bytes of the codes (72 a key and key head of
+// 64, keys and values) keep DRAM busy for 38 %, 290 instructions of a warp for 32 keys the issue slots for 47 % (61 %
+// of the cycles in which an SM works), the ALU pipe 47 %, the tensor pipe 21 %: with the 16 warps an SM that 128
+// registers and the rings allow, 0.97 of 3.25 warps a scheduler are ready on average. One block = one
 // (request, key head, up to 8 of its query heads, split of the keys); its 8 warps take tiles of 64 keys (Ring) in
 // turn, each through a ring of its own that bulk copies fill (one copy brings the keys and values of 16 tokens):
 // no barrier of the block before the end. The warps are merged in shared memory, the splits of up to 8 blocks
@@ -31,7 +33,7 @@
 // Measured, 32 heads over 8 key heads of 64, us on the GPU: 32 requests of 4,096 keys 24.1 (75.5 MB, 3.1 TB/s; 11.3
 // at the copy rate; issue slots taken in 61 % of the cycles that an SM works, 256 blocks on 296 places), one of
 // 509 keys 4.0 (launch and three loads one after the other), four of 30,011 keys with heads of 128 38.2 (3.8
-// TB/s). Instructions, not bytes: 10 to 16 warps a block (26.8 to 30.3 against 24.2 us) or tiles of 32 keys with
+// TB/s). 10 to 16 warps a block (26.8 to 30.3 against 24.2 us; an SM then has room for one block) or tiles of 32 keys with
 // heads of 64 (26.9) are slower, and so is more than one block a request and key head where the blocks find no
 // place at once (packed_splits in kernels/cuda_ops.py has the rule).
 //

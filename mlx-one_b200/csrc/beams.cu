@@ -8,8 +8,10 @@
 //   beam_choice a block per row. With the ceil(B / 8) largest of what each of its 8 warps sees of the row's thread
 //               maxima the B-th largest of those bounds the B best from below (B threads have a value of that
 //               size at least), so only the values of the few threads whose maximum reaches it are read again;
-//               those that reach it are ordered by counting who is ahead. Where ties make them many, the row is
-//               walked value by value instead. A request's candidates are ordered in the same way by the first block
+//               those that reach it are ordered by counting who is ahead. Where they are many the row is walked
+//               value by value instead: with ties, and with small vocabularies, for the maxima of p parts of 8,192
+//               lie with 2 p of the 8 warps, whose offers are too few for a bound in one part from three hypotheses
+//               on, in two from five, in three with 7, 8, 13 to 16 and 19 or more. A request's candidates are ordered in the same way by the first block
 //               of its cluster, or (more than eight hypotheses) by its last block to arrive: a counter in the call's
 //               own scratch, set to zero by the kernel before.
 // Within a row logits are compared as they are, between rows sums in 64 bits: no order is lost to rounding. A
@@ -18,7 +20,9 @@
 //
 // Measured, us on the GPU: one request of four hypotheses over 65,536 logits 7.7 (two launches; the choice waits
 // for the maxima, the chosen logits and its neighbours in turn), 32 of eight (60 MB are wanted) 22.0: 2.7 TB/s, 9.2 at
-// the copy rate. About half of that is the sums' reading, half the choice, which waits rather than works. Sorted
+// the copy rate. About half of that is the sums' reading, half the choice, which waits rather than works. Rows
+// that are walked cost more than longer ones with a bound: four hypotheses over 1,000 / 8,192 / 16,384 tokens 19.2 / 22.4 /
+// 6.9, eight over 16,384 / 24,576 / 32,000 28.8 / 36.5 / 8.9, 32 requests of eight 57.8 / 72.1 / 15.0. Sorted
 // lists by insertion instead of the bound took 47, a part's best kept in registers 31, lists in shared memory 35.
 //
 // Reordering. In place: hypothesis b takes over what hypothesis parent(b) held, both of the same request. A
@@ -280,7 +284,7 @@ beam_choice_kernel(const float* logits, long long stride, int vocab, const float
                 if (better < beams) sorted[better] = rank;
             }
         } else {
-            // ties, or hardly a logit above minus infinity: eight sorted lists, then one
+            // ties, a small vocabulary, or hardly a logit above minus infinity: eight sorted lists, then one
             __syncthreads();
             Best best;
             for (int from = 0; from < vocab; from += WARPS * 32) {

@@ -597,8 +597,9 @@ class Engine:
         compete with hypotheses that have ended; ranked by sum / (tokens, an end token counted) **
         ``length_penalty`` (-10 to 10), best first (fewer where there are fewer continuations). ``options`` name the
         number of tokens and ``ignore_eos``; sampling and stop strings have no place here. The search holds
-        the engine's turn to its end: other requests wait. It needs ``beams`` free requests of the cache and
-        pages for prompt and tokens of each (``CacheCapacityError``)."""
+        the engine's turn to its end: other requests wait, their time limits running on, and it has none of its own.
+        It needs ``beams`` free requests of the cache and pages for prompt and tokens of each
+        (``CacheCapacityError``)."""
         options = self._options(options, option_kwargs)
         if options.temperature or options.top_k is not None or options.top_p != 1.0 or options.stop:
             raise ValueError("a beam search takes no sampling options and no stop strings")
