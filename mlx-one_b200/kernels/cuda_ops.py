@@ -1705,7 +1705,11 @@ class CudaOps:
         tanh(s / c); ``slopes`` (float32 [heads] or None): then they lose slope * (query's position
         - key's); ``least_slope`` is their minimum on the host. ``view`` may be a ``PackedView``: keys
         and values held in 4 bits (``_packed_attention``). ``out``: where the result goes, if not into a
-        tensor of its own."""
+        tensor of its own: contiguous, of the queries' type, [tokens, heads * head_dim]."""
+        if out is not None:
+            self._need(out, q.dtype, "out")
+            if out.shape != (q.shape[0], heads * head_dim):
+                raise KernelError(f"out must be {(q.shape[0], heads * head_dim)}, got {tuple(out.shape)}")
         if isinstance(view, PackedView):
             return self._packed_attention(q, heads, kv_heads, head_dim, scale, window, ctx, view,
                                           sinks=sinks, chunk=chunk, keep_first=keep_first,

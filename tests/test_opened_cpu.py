@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import plain_packed as plain
-from mlx_one_b200.kernels.cuda_ops import CudaOps
+from mlx_one_b200.kernels.cuda_ops import CudaOps, KernelError
 from mlx_one_b200.parts.base import PackedView, PagedKeyValues, PagedView, StepContext, packed_part_bytes
 
 
@@ -166,3 +166,25 @@ def test_a_step_says_how_long_its_portions_are(tmp_path):
     runner.step([StepEntry("a", [3], (0,)), StepEntry("b", [3] * 5, (4,)), StepEntry("c", [3] * 7, (6,))])
     runner.step([StepEntry("a", [3], (0,)), StepEntry("b", [3], (0,))])
     assert [(c.leading_single, c.rest_context, c.max_context) for c in steps] == [(0, 40, 40), (1, 7, 41), (2, 0, 42)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("leading", [0, 2])
+def test_results_that_are_refused(dtype, leading):
+    """A given ``out`` is as large as the result and of its type, over packed pages and over plain ones."""
+    ctx = step([1, 1, 3], [4, 0, 9], leading)
+    width = 4 * 32
+    good = torch.zeros(5, width, dtype=dtype)
+    attend(Ops(), ctx, dtype, out=good)
+    other = torch.bfloat16 if dtype == torch.float32 else torch.float32
+    for bad in (good[:4], good[:, :64].contiguous(), torch.zeros(5, 2 * width, dtype=dtype)[:, ::2], good.to(other),
+                torch.zeros(6, width, dtype=dtype), good.view(5, 4, 32), good.view(-1), good.to("meta")):
+        ops = Ops()
+        with pytest.raises(KernelError, match="out must"):
+            attend(ops, ctx, dtype, out=bad)
+        plainly = PagedView(torch.zeros(2, 4, 2, 16, 32, dtype=dtype), torch.zeros((3, 8), dtype=torch.int32), 16,
+                            PagedKeyValues(2, 32))
+        with pytest.raises(KernelError, match="out must"):
+            CudaOps.paged_attention(ops, torch.zeros(5, 4, 32, dtype=dtype), heads=4, kv_heads=2, head_dim=32, scale=1.0,
+                                    window=None, ctx=ctx, view=plainly, out=bad)
+        assert not ops.launched and not ops.read
