@@ -2017,8 +2017,8 @@ class CudaOps:
 
     # ---- keys and values held in 4 bits
 
-    def _need_packed(self, view) -> int:
-        """Checks a view of packed pages; returns how many pages there are."""
+    def _need_packed(self, view, requests: int) -> int:
+        """Checks a view of packed pages for a step of ``requests`` requests; returns how many pages there are."""
         kv, need, size, table = view.kv, view.need, view.page_size, view.block_table
         geometry = (need.kv_heads, need.head_dim, need.planes, size)
         shape = self._packed_shapes.get(geometry)
@@ -2036,6 +2036,8 @@ class CudaOps:
         if table.dtype != torch.int32 or table.dim() != 2:
             raise KernelError(f"a block table must be int32 [requests, width], got {table.dtype} {tuple(table.shape)}")
         self._need(table, torch.int32, "block table")
+        if table.shape[0] < requests:
+            raise KernelError("a block table needs a row for every request")
         return kv.shape[0]
 
     def pack_key_values(self, keys, values, *, ctx, view):
@@ -2044,7 +2046,7 @@ class CudaOps:
         ``view``. Every group of a token's values (64; 32 where 64 do not divide the head) is held as its
         lowest value and a step in bfloat16 and a code of 0 to 15 a value, the nearest; a group with a
         value that is not finite reads as NaN. Other tokens' bytes stay as they are."""
-        pages, code = self._need_packed(view), _dtype_code(keys.dtype)
+        pages, code = self._need_packed(view, ctx.requests), _dtype_code(keys.dtype)
         need, table = view.need, view.block_table
         wanted, dtype = (ctx.tokens, need.kv_heads * need.head_dim), keys.dtype
         for rows, what in ((keys, "keys"), (values, "values")):
@@ -2060,7 +2062,7 @@ class CudaOps:
     def read_key_values(self, *, ctx, view, dtype=torch.bfloat16):
         """What attention finds at the step's tokens' places in packed pages: (keys, values), each
         [tokens, kv_heads, head_dim] in ``dtype``."""
-        pages, code = self._need_packed(view), _dtype_code(dtype)
+        pages, code = self._need_packed(view, ctx.requests), _dtype_code(dtype)
         need, table = view.need, view.block_table
         keys = torch.empty((ctx.tokens, need.kv_heads, need.head_dim), dtype=dtype, device=self.device)
         values = torch.empty_like(keys)
@@ -2073,7 +2075,7 @@ class CudaOps:
     def _prepare_packed(self, qkv, *, kv_heads, ctx, view, write, **how):
         """qk_norm_rope_store for packed pages: the same kernels write keys and values in the compute
         dtype, one row a token, and a second one packs them."""
-        self._need_packed(view)
+        self._need_packed(view, ctx.requests)
         tokens, row = qkv.shape[0], view.need.head_dim
         ready = torch.empty((2, max(tokens, 1), kv_heads, 1, row), dtype=qkv.dtype, device=self.device)
         # (without a table a token's row is its own page)
@@ -2091,15 +2093,13 @@ class CudaOps:
         kernels read: a portion has many queries for every key that is opened. So do single tokens whose
         scores are shaped or that see first positions behind a window. Keys without a page: the kernel over
         codes does not see them, opening one that is to be seen raises the error flag."""
-        pages, code = self._need_packed(view), _dtype_code(q.dtype)
+        pages, code = self._need_packed(view, ctx.requests), _dtype_code(q.dtype)
         self._need(q, q.dtype, "q")
         tokens, requests, width = q.shape[0], ctx.requests, view.block_table.shape[1]
         if q.numel() != tokens * heads * head_dim or heads % kv_heads or \
                 (kv_heads, head_dim) != (view.need.kv_heads, view.need.head_dim):
             raise KernelError(f"queries {tuple(q.shape)} of {heads} heads of {head_dim} do not fit packed pages "
                               f"of {view.need.kv_heads} heads of {view.need.head_dim}")
-        if view.block_table.shape[0] < requests:
-            raise KernelError("a block table needs a row for every request")
         if chunk:
             window = self._span(window, chunk)
         window = int(window or 0)

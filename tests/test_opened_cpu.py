@@ -188,3 +188,18 @@ def test_results_that_are_refused(dtype, leading):
             CudaOps.paged_attention(ops, torch.zeros(5, 4, 32, dtype=dtype), heads=4, kv_heads=2, head_dim=32, scale=1.0,
                                     window=None, ctx=ctx, view=plainly, out=bad)
         assert not ops.launched and not ops.read
+
+
+def test_tables_with_too_few_rows():
+    """Writing and reading back look a request's pages up in its row of the block table, as attention does."""
+    ops, ctx = Ops(), step([2, 3], [0, 4], 0)
+    pages, rows = plain.empty_pages(3, 2, 16, 32), torch.zeros(5, 64)
+    for table, good in ((torch.zeros((1, 4), dtype=torch.int32), False), (torch.zeros((2, 4), dtype=torch.int32), True)):
+        view = PackedView(pages, table, 16, PagedKeyValues(2, 32))
+        for call in (lambda: ops.pack_key_values(rows, rows, ctx=ctx, view=view), lambda: ops.read_key_values(ctx=ctx, view=view)):
+            if good:
+                call()
+            else:
+                with pytest.raises(KernelError, match="a row for every request"):
+                    call()
+    assert len(ops.launched) == 2
